@@ -542,6 +542,128 @@ int32_t tqb_kv_cache_num_layers(const tqb_kv_cache *c);
 size_t tqb_kv_cache_memory_usage(const tqb_kv_cache *c);          /* attention.rs:414-428 */
 size_t tqb_kv_cache_fp16_equivalent_memory(const tqb_kv_cache *c); /* attention.rs:437-440 */
 
+/* =====================================================================================
+ * 6. Paged cache: requests of different lengths in one batch.  No counterpart in the reference, whose caches hold one
+ *    sequence each.  The rows are those of section 4 (MaxNorm, every block on the outlier codebook: bits as
+ *    tqb_block_quantize stores them), kept in pages of page_size tokens.  A page holds the same token range of every
+ *    KV head of a layer; token t of a request lies in the page block_table[request][t / page_size] at row t % page_size,
+ *    and its SLOT is page * page_size + t % page_size.  All pointers are device pointers owned by the caller.
+ * ===================================================================================== */
+
+/* The arrays of one layer: indices [num_pages, num_kv_heads, page_size, head_dim*bits/8] u8 and scales
+ * [num_pages, num_kv_heads, page_size, head_dim/32] u16, each 16-byte aligned.  head_dim 64, 128 or 256; bits 3 or 4;
+ * page_size a power of two from 16 to 1024. */
+typedef struct tqb_paged_layer {
+    uint8_t *k_indices;
+    uint16_t *k_scales;
+    uint8_t *v_indices;
+    uint16_t *v_scales;
+    int32_t num_pages;
+    int32_t num_kv_heads;
+    int32_t page_size;
+    int32_t head_dim;
+    int32_t bits;
+    int32_t reserved;
+} tqb_paged_layer;
+
+/* Most requests of one plan or attention call (TQB_ERR_TOO_LARGE beyond). */
+#define TQB_PAGED_MAX_REQUESTS 4096
+
+/* state: four words on the device, {free pages left, 0, status of the last plan or release, 0}. */
+#define TQB_PLAN_OK 0
+#define TQB_PLAN_OUT_OF_PAGES 1   /* plan: more pages needed than free; release: the list of free pages is too short */
+#define TQB_PLAN_BAD_LENGTH 2     /* a negative length, or one beyond max_blocks * page_size */
+#define TQB_PLAN_OVER_CAPACITY 3  /* more new tokens than `capacity` */
+
+/* Block tables, slot map and positions of a step from the requests' lengths, on the device and in one launch.
+ * Request r holds seq_lens[r] tokens and brings new_tokens[r].  Pages that it lacks are taken from the end of the list
+ * free_pages[0 .. state[0]) in the order of the requests and entered in block_table (rows table_stride entries apart).
+ *   cu [num_requests + 1]    first new token of each request, then their number
+ *   slots, positions [capacity]   of every new token; behind the last one slot -1 and position 0
+ *   kv_lens [num_requests]   seq_lens + new_tokens; may be seq_lens itself
+ *   state_out                the new state; may be `state` itself.  state[1] is used during the call and left 0.
+ * Where the step cannot be planned state_out[2] says why, no page is taken, no table entry written, every slot is
+ * -1, cu is 0 and kv_lens = seq_lens.  Calls that share `state` must be ordered. */
+int tqb_paged_plan(const int32_t *seq_lens, const int32_t *new_tokens, int32_t num_requests, int32_t *block_table,
+                   int64_t table_stride, int32_t max_blocks, const int32_t *free_pages, int32_t *state, int32_t page_size,
+                   int64_t *slots, int32_t *positions, int32_t capacity, int32_t *cu, int32_t *kv_lens,
+                   int32_t *state_out, tqb_stream_t stream);
+/* Gives the pages of the requests with mask[r] != 0 back: appended to free_pages (room for free_capacity entries) in the
+ * order of requests and blocks; their seq_lens become 0 and their table entries -1. */
+int tqb_paged_release(const uint8_t *mask, int32_t *seq_lens, int32_t num_requests, int32_t *block_table,
+                      int64_t table_stride, int32_t max_blocks, int32_t *free_pages, int32_t free_capacity, int32_t *state,
+                      int32_t page_size, tqb_stream_t stream);
+
+/* Norms of queries and keys for each head, with the position rotation in the same pass:
+ *   y = x / sqrt(mean(x^2) + eps) * weight           (TQB_ROPE_NO_NORM: y = x; a NULL weight: 1)
+ *   (y_a, y_b) -> (y_a cos - y_b sin, y_b cos + y_a sin),  angle = position * inv_freq[i], i < rot_dim / 2,
+ *   with (a, b) = (i, i + rot_dim/2), or (2i, 2i + 1) with TQB_ROPE_INTERLEAVED; elements from rot_dim on keep y.
+ * Computed in f32 from angles reduced in f64, rounded once.  q [num_tokens, num_q_heads, head_dim] and k
+ * [num_tokens, num_kv_heads, head_dim] of `dtype` with the given strides in elements (the last dimension dense, rows
+ * 16-byte aligned); q_out / k_out may be q / k themselves with the same strides, and overlap nothing otherwise.
+ * head_dim 64, 128 or 256; rot_dim a multiple of 16 up to head_dim (0: no rotation).  q or k may be NULL. */
+#define TQB_ROPE_INTERLEAVED 1
+#define TQB_ROPE_NO_NORM 2
+#define TQB_ROPE_POSITIONS_64 4   /* positions are int64 */
+typedef struct tqb_rope_params {
+    const void *q;
+    void *q_out;
+    const void *k;
+    void *k_out;
+    int64_t q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride;
+    int64_t k_token_stride, k_head_stride, k_out_token_stride, k_out_head_stride;
+    const void *q_weight;        /* [head_dim] of `dtype`, or NULL */
+    const void *k_weight;
+    const void *positions;       /* [num_tokens] int32 (or int64) */
+    const float *inv_freq;       /* [rot_dim / 2] */
+    int32_t num_tokens, num_q_heads, num_kv_heads, head_dim, rot_dim, dtype, flags;
+    float eps;
+} tqb_rope_params;
+int tqb_qk_norm_rope(const tqb_rope_params *p, tqb_stream_t stream);
+
+/* Packs the rows k, v [num_tokens, num_kv_heads, head_dim] (strides in elements) into their slots, one launch.  The bytes
+ * are those of tqb_block_quantize.  Rows whose slot lies outside [0, num_pages * page_size) are not stored; no other two
+ * rows may have the same slot. */
+int tqb_paged_append(const tqb_paged_layer *layer, const void *k, int64_t k_token_stride, int64_t k_head_stride,
+                     const void *v, int64_t v_token_stride, int64_t v_head_stride, int32_t dtype, const int64_t *slots,
+                     int32_t num_tokens, tqb_stream_t stream);
+/* tqb_qk_norm_rope with the keys going into their slots instead of k_out (rounded to `dtype` first: the bytes are those
+ * of the two calls one after the other), and the values with them.  p->k_out is written too unless NULL. */
+int tqb_paged_append_rope(const tqb_paged_layer *layer, const tqb_rope_params *p, const void *v, int64_t v_token_stride,
+                          int64_t v_head_stride, const int64_t *slots, tqb_stream_t stream);
+/* The rows at n slots, dequantized (the values of tqb_block_dequantize): k_out, v_out [n, num_kv_heads, head_dim] of
+ * out_dtype.  Slots outside the pages give rows of zeros. */
+int tqb_paged_dequantize(const tqb_paged_layer *layer, const int64_t *slots, int64_t n, void *k_out, void *v_out,
+                         int32_t out_dtype, tqb_stream_t stream);
+
+/* Attention of one new token of each request over its pages.
+ *   q, out [num_requests, num_q_heads, head_dim], q rows q_row_stride elements apart (0: dense), 16-byte aligned
+ *   block_table [num_requests, max_blocks], rows table_stride entries apart;  kv_lens [num_requests]
+ * Request r attends to its first kv_lens[r] tokens (the new one stored already).  A request without tokens gets
+ * zeros.  Lengths beyond max_blocks * page_size are cut there, and the tokens of a page outside [0, num_pages) are left out.
+ * The work is split over the lengths on the device, so that a captured call serves any lengths later.
+ * scratch: tqb_paged_scratch_bytes() bytes whose first TQB_PAGED_TICKET_BYTES the caller has zero-filled once; every
+ * completed call leaves them zero.  Two calls that may run at the same time need a scratch each. */
+#define TQB_PAGED_TICKET_BYTES 8192
+typedef struct tqb_paged_attention_params {
+    const void *q;
+    void *out;
+    const int32_t *block_table;
+    const int32_t *kv_lens;
+    void *scratch;
+    size_t scratch_bytes;
+    int64_t q_row_stride;
+    int64_t table_stride;
+    int32_t max_blocks;
+    int32_t num_requests;
+    int32_t num_q_heads;
+    int32_t q_dtype;
+    int32_t out_dtype;
+    float softmax_scale;
+} tqb_paged_attention_params;
+size_t tqb_paged_scratch_bytes(int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim);
+int tqb_paged_attention(const tqb_paged_layer *layer, const tqb_paged_attention_params *p, tqb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -12,3 +12,5 @@ from .api import (  # noqa: F401
     dequantize_vec, estimate_inner_product, lse_combine, pack_indices, packed_bytes, precompute_query_projections,
     qjl_attention_scores, qjl_quantize_batch, quantize_batch, quantize_vec, quantize_with_qjl, query_projections,
     rademacher_bits, unpack_indices, weighted_values)
+from .paged import (  # noqa: F401
+    PagedLayer, PagedPqoCache, PagedStep, QkNormRope, paged_plan, paged_release)

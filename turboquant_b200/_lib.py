@@ -38,6 +38,31 @@ class TqbDecodeParams(ctypes.Structure):
                 ("softmax_scale", c_float), ("flags", c_int32), ("append_k", c_void_p), ("append_v", c_void_p)]
 
 
+class TqbPagedLayer(ctypes.Structure):
+    """tqb_paged_layer."""
+    _fields_ = [("k_indices", c_void_p), ("k_scales", c_void_p), ("v_indices", c_void_p), ("v_scales", c_void_p),
+                ("num_pages", c_int32), ("num_kv_heads", c_int32), ("page_size", c_int32), ("head_dim", c_int32),
+                ("bits", c_int32), ("reserved", c_int32)]
+
+
+class TqbRopeParams(ctypes.Structure):
+    """tqb_rope_params."""
+    _fields_ = ([(n, c_void_p) for n in ("q", "q_out", "k", "k_out")] +
+                [(f"{x}{y}_stride", c_int64) for x in ("q_", "q_out_") for y in ("token", "head")] +
+                [(f"{x}{y}_stride", c_int64) for x in ("k_", "k_out_") for y in ("token", "head")] +
+                [(n, c_void_p) for n in ("q_weight", "k_weight", "positions", "inv_freq")] +
+                [(n, c_int32) for n in ("num_tokens", "num_q_heads", "num_kv_heads", "head_dim", "rot_dim", "dtype", "flags")] +
+                [("eps", c_float)])
+
+
+class TqbPagedAttentionParams(ctypes.Structure):
+    """tqb_paged_attention_params."""
+    _fields_ = [("q", c_void_p), ("out", c_void_p), ("block_table", c_void_p), ("kv_lens", c_void_p), ("scratch", c_void_p),
+                ("scratch_bytes", c_size_t), ("q_row_stride", c_int64), ("table_stride", c_int64), ("max_blocks", c_int32),
+                ("num_requests", c_int32), ("num_q_heads", c_int32), ("q_dtype", c_int32), ("out_dtype", c_int32),
+                ("softmax_scale", c_float)]
+
+
 def declared_symbols(header_path=HEADER_PATH):
     """Names of every function declared in the public header."""
     text = open(header_path).read()
@@ -130,6 +155,14 @@ def _declare(lib):
         "tqb_tq_cache_reset": (c_int, [P]),
         "tqb_tq_cache_memory_usage": (S, [P]),
         "tqb_tq_cache_qjl_ptrs": (c_int, [P, I, P, P, P]),
+        "tqb_paged_plan": (c_int, [P, P, I, P, L, I, P, P, I, P, P, I, P, P, P, P]),
+        "tqb_paged_release": (c_int, [P, P, I, P, L, I, P, I, P, I, P]),
+        "tqb_qk_norm_rope": (c_int, [P, P]),
+        "tqb_paged_append": (c_int, [P, P, L, L, P, L, L, I, P, I, P]),
+        "tqb_paged_append_rope": (c_int, [P, P, P, L, L, P, P]),
+        "tqb_paged_dequantize": (c_int, [P, P, L, P, P, I, P]),
+        "tqb_paged_scratch_bytes": (S, [I, I, I]),
+        "tqb_paged_attention": (c_int, [P, P, P]),
         "tqb_kv_cache_create": (c_int, [P, I, U, P]),
         "tqb_kv_cache_destroy": (None, [P]),
         "tqb_kv_cache_push_batch": (c_int, [P, I, P, P, L, L, P]),
