@@ -665,6 +665,8 @@ int check_paged_layer(const tqb_paged_layer* l) {
     if (l->head_dim != 64 && l->head_dim != 128 && l->head_dim != 256) return TQB_ERR_UNSUPPORTED;
     if (l->page_size < 16 || l->page_size > 1024 || (l->page_size & (l->page_size - 1)) != 0) return TQB_ERR_INVALID_ARGUMENT;
     if (l->num_pages < 0 || l->num_kv_heads <= 0) return TQB_ERR_INVALID_ARGUMENT;
+    // rows are counted in 32 bits: 2^32 rows of the smallest kind are 206 GB
+    if ((unsigned long long)l->num_pages * l->num_kv_heads > (1ull << 32) / l->page_size - 1) return TQB_ERR_TOO_LARGE;
     if (l->num_pages == 0) return TQB_OK;
     if (!l->k_indices || !l->k_scales || !l->v_indices || !l->v_scales) return TQB_ERR_NULL_POINTER;
     if (!aligned16(l->k_indices) || !aligned16(l->k_scales) || !aligned16(l->v_indices) || !aligned16(l->v_scales)) return TQB_ERR_MISALIGNED;

@@ -40,6 +40,8 @@ struct PagedArgs {
     float cent[16];
 };
 
+int launch_paged_mma(const PagedArgs& a, int head_dim, cudaStream_t s);   // 4-bit, 16-bit queries, some page
+
 struct Segment {
     int req, kvh, head0, heads;   // query heads head0 .. head0 + heads - 1 of the request
     int t0, t1;                   // its tokens
