@@ -644,7 +644,7 @@ int tqb_paged_dequantize(const tqb_paged_layer *layer, const int64_t *slots, int
  * The work is split over the lengths on the device, so that a captured call serves any lengths later.
  * scratch: tqb_paged_scratch_bytes() bytes whose first TQB_PAGED_TICKET_BYTES the caller has zero-filled once; every
  * completed call leaves them zero.  Two calls that may run at the same time need a scratch each. */
-#define TQB_PAGED_TICKET_BYTES 8192
+#define TQB_PAGED_TICKET_BYTES 16384
 typedef struct tqb_paged_attention_params {
     const void *q;
     void *out;

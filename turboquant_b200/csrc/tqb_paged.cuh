@@ -2,6 +2,8 @@
 #pragma once
 #include <math.h>
 
+#include <atomic>
+
 #include "tqb_common.cuh"
 
 namespace tqb {
@@ -14,6 +16,23 @@ inline float block_sign_magnitude() {
     volatile float inv = 1.0f / sqrtf(32.0f);
     volatile float s = sqrtf(32.0f);
     return inv * s;
+}
+
+// More than 48 KB of shared memory, the static part included, is a property of the kernel on a device: set once for each.
+template <auto* KERNEL>
+int allow_shared(int bytes) {
+    static std::atomic<unsigned long long> configured{0};
+    if (bytes <= 32 * 1024) return TQB_OK;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = -1;
+    if (dev >= 0 && ((configured.load(std::memory_order_acquire) >> dev) & 1ull)) return TQB_OK;
+    const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) {
+        set_cuda_error(e);
+        return TQB_ERR_CUDA;
+    }
+    if (dev >= 0) configured.fetch_or(1ull << dev, std::memory_order_release);
+    return TQB_OK;
 }
 
 }  // namespace tqb

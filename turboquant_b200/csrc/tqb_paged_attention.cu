@@ -10,21 +10,21 @@
 namespace tqb {
 namespace {
 
-// One token a warp at a time, one lane a dim of every block, all in f32.
+// One token a warp at a time, one lane a dim of every block, all in f32: f32 queries (whose precision the 16-bit weights of
+// the tensor-core kernel would lose), and layers without pages.
 template <int NB, int BITS>
 __global__ void __launch_bounds__(kWorkThreads) paged_simple_kernel(const __grid_constant__ PagedArgs a) {
-    constexpr int D = NB * 32, kWarps = kWorkThreads / 32;
-    __shared__ float s_m[kWarps][kSegHeads], s_l[kWarps][kSegHeads];
+    constexpr int D = NB * 32;
     __shared__ float s_cent[16];
-    extern __shared__ float s_o[];   // [kWarps][kSegHeads][D]
+    __shared__ Fragments s_frag;
+    extern __shared__ float s_o[];   // [2 kWorkWarps][kSegHeads][D]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid < 16) s_cent[tid] = a.cent[tid];
-    WorkLine line(a);
-    write_empty<NB>(a);
+    if (tid < 2 * kWorkWarps) s_frag.used[tid] = 0;
+    WorkLine line(a);   // (its barriers stand before the first use of what is set above)
     const int page_mask = (1 << a.page_shift) - 1;
-    while (line.more()) {
-        const Segment s = line.next();
-        __syncthreads();   // s_cent; and the last segment's end has read s_o
+    Segment s;
+    while (line.next(s)) {
         float q[kSegHeads][NB], o[kSegHeads][NB], m[kSegHeads], l[kSegHeads];
 #pragma unroll
         for (int h = 0; h < kSegHeads; ++h) {
@@ -37,7 +37,7 @@ __global__ void __launch_bounds__(kWorkThreads) paged_simple_kernel(const __grid
                 q[h][b] = wht32_across(q[h][b], lane) * (1.0f / sqrtf((float)kBlock)) * block_sign(lane, a.sign_mag) * a.qk_const;
             }
         }
-        for (int t = s.t0 + warp; t < s.t1; t += kWarps) {
+        for (int t = s.t0; t < s.t1; ++t) {
             const int page = a.table[s.req * a.table_stride + (t >> a.page_shift)];
             if ((unsigned)page >= (unsigned)a.num_pages) continue;
             const size_t row = (((size_t)page * a.hkv + s.kvh) << a.page_shift) + (t & page_mask);
@@ -69,23 +69,33 @@ __global__ void __launch_bounds__(kWorkThreads) paged_simple_kernel(const __grid
                 for (int b = 0; b < NB; ++b) o[h][b] = fmaf(o[h][b], keep, p * v[b]);
             }
         }
+        const int slot = 2 * warp + (s.begins ? 1 : 0);
 #pragma unroll
         for (int h = 0; h < kSegHeads; ++h) {
-            if (lane == 0) {
-                s_m[warp][h] = m[h];
-                s_l[warp][h] = l[h];
-            }
+            if (h >= s.heads) break;
 #pragma unroll
-            for (int b = 0; b < NB; ++b) s_o[(warp * kSegHeads + h) * D + b * 32 + lane] = o[h][b];
+            for (int b = 0; b < NB; ++b) {
+                if (s.whole()) write_block<NB>(a, s.req, s.head0 + h, b, lane, o[h][b], l[h]);
+                else s_o[(slot * kSegHeads + h) * D + b * 32 + lane] = o[h][b];
+            }
+            if (!s.whole() && lane == 0) {
+                s_frag.m[slot][h] = m[h];
+                s_frag.l[slot][h] = l[h];
+            }
         }
-        __syncthreads();
-        finish_segment<NB>(a, s, s_m, s_l, [&](int w, int h, int d) { return s_o[(w * kSegHeads + h) * D + d]; });
+        if (!s.whole() && lane == 0) {
+            s_frag.seg[slot] = s;
+            s_frag.used[slot] = 1;
+        }
     }
+    finish<NB>(a, s_frag, [&](int c, int h, int d) { return s_o[(c * kSegHeads + h) * D + d]; });
+    write_empty<NB>(a);
 }
 
 template <int NB, int BITS>
 int launch_simple(const PagedArgs& a, cudaStream_t s) {
-    const size_t dyn = sizeof(float) * (kWorkThreads / 32) * kSegHeads * NB * 32;
+    const int dyn = (int)sizeof(float) * 2 * kWorkWarps * kSegHeads * NB * 32;
+    if (int st = allow_shared<paged_simple_kernel<NB, BITS>>(dyn)) return st;
     paged_simple_kernel<NB, BITS><<<148 * 4, kWorkThreads, dyn, s>>>(a);
     return check_launch(s);
 }
@@ -141,6 +151,8 @@ int tqb_paged_attention(const tqb_paged_layer* layer, const tqb_paged_attention_
     a.table_stride = p->table_stride;
     a.requests = p->num_requests;
     a.max_blocks = p->max_blocks;
+    const int64_t max_len = (int64_t)p->max_blocks * layer->page_size;
+    a.max_len = (int)(max_len < 0x7fffff00 ? max_len : 0x7fffff00);   // (whole groups stay below 2^31)
     while ((1 << a.page_shift) < layer->page_size) ++a.page_shift;
     a.num_pages = layer->num_pages;
     a.hkv = layer->num_kv_heads;

@@ -1,9 +1,9 @@
 // Attention of one new token of each request over the paged packed cache, 16-bit queries: the tensor-core kernel.
 //
-// Four warps share a segment (tqb_paged_work.cuh): warp w takes the groups of 16 tokens w, w + 4, .. of it.  The work is one
-// pass over the packed bytes with the running maximum and sum of a softmax; at the measured copy bandwidth an SM
-// scheduler has about 400 issue slots for 16 tokens of a KV head (4-bit, 2304 bytes), and that, not the MMAs, is what the
-// layout below is about.
+// Every warp takes its segments (tqb_paged_work.cuh) by itself, two groups of 16 tokens a step, the next two in flight.  The work
+// is one pass over the packed bytes with the running maximum and sum of a softmax; at the measured copy bandwidth an SM
+// scheduler has about 400 issue slots for 16 tokens of a KV head (4-bit, head_dim 128: 2304 bytes), and that, not the MMAs, is
+// what the layout below is about.
 //
 // Scores S = K~ Q~^T (mma.sync s8 x s8 -> s32, one 32-block an instruction): rows are 16 tokens, a code c enters as the byte
 //   16 (c - 7.5), two logic operations for four codes; the rotated query enters as a 16-bit integer in two base-256 digits,
@@ -27,8 +27,6 @@
 #include "tqb_paged_work.cuh"
 
 #include <float.h>
-
-#include <atomic>
 
 namespace tqb {
 namespace {
@@ -56,9 +54,7 @@ __device__ __forceinline__ void codes_to_subnormals(uint32_t w, uint32_t (&x)[4]
 constexpr uint32_t kCentreEven = 0x800f800fu;   // -7.5 2^-23 as a subnormal f16, twice
 constexpr uint32_t kCentreOdd = 0x80f080f0u;    // -7.5 2^-19
 
-__device__ __forceinline__ uint32_t scaled(uint32_t p, uint32_t scales) {   // p |s|, two f16 values
-    return h2_as_u32(__hmul2(u32_as_h2(p), __habs2(u32_as_h2(scales))));
-}
+__device__ __forceinline__ uint32_t product(uint32_t a, uint32_t b) { return h2_as_u32(__hmul2(u32_as_h2(a), u32_as_h2(b))); }
 
 template <int NB>
 struct Shape {
@@ -66,32 +62,44 @@ struct Shape {
     static constexpr int kIdx = kGroupTokens * kRow;    // of a stage's K (or V) codes
     static constexpr int kSc = 2 * NB;                  // of a token's scales
     static constexpr int kStage = 2 * kIdx + 2 * kGroupTokens * kSc;   // [K codes][V codes][K scales][V scales]
-    static constexpr int kWarpRing = kRing * kStage;
+    static constexpr int kWarpRing = kRing * kStage;      // of a warp
     // 16-byte piece c of token row t lies at piece c ^ swizzle(t): the eight rows of an ldmatrix hit different banks
     __device__ static __forceinline__ int swizzle(int t) { return NB == 2 ? (t >> 2) & 1 : NB == 4 ? (t >> 1) & 3 : t & 7; }
 };
 
 template <int NB, int HG>
-struct Plan {   // CTAs of an SM, by registers and shared memory
-    static constexpr int kCtas = NB == 8 ? (HG == 8 ? 2 : 3) : HG == 8 ? 4 : 5;
+struct Plan {
+    using G = Shape<NB>;
+    static constexpr int kSets = HG == 4 ? 1 : 2;                 // MMAs of a block's scores
+    static constexpr int kFragment = HG * NB * 32 * 4;            // outputs of a segment
+    static constexpr int kDigits = kSets * NB * 32 * 8;           // the queries' MMA fragments
+    static constexpr int kWarpBytes = G::kWarpRing + kFragment + kDigits;   // [ring][fragment that began before][digits]
+    static constexpr int kBytes = kWorkWarps * kWarpBytes;
+    // CTAs of an SM: by shared memory, and so that registers do not spill
+    static constexpr int kByShared = 227 * 1024 / (kBytes + 4096), kByRegs = NB == 8 ? (HG == 8 ? 2 : 3) : HG == 8 ? 4 : NB == 2 ? 5 : 4;
+    static constexpr int kCtas = kByShared < kByRegs ? kByShared : kByRegs;
 };
 
 template <int NB, int HG>
 __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_kernel(const __grid_constant__ PagedArgs a) {
     using G = Shape<NB>;
-    constexpr int D = NB * 32, kWarps = kWorkThreads / 32, kE = HG == 4 ? 1 : 2, kPairs = NB / 2;
-    constexpr int kSets = HG == 4 ? 1 : 2;   // MMAs of a block's scores
-    extern __shared__ __align__(128) unsigned char s_ring[];
-    __shared__ float s_q[HG][D];
-    __shared__ __align__(16) uint2 s_qfr[kSets][NB][32];
-    __shared__ float s_qsc[kSegHeads];
-    __shared__ float s_m[kWarps][kSegHeads], s_l[kWarps][kSegHeads];
-    float* s_o = reinterpret_cast<float*>(s_ring);   // [kWarps][HG][D], when the rings are idle
-    static_assert(kWarps * HG * D * 4 <= kWarps * G::kWarpRing, "outputs do not fit into the rings");
+    using L = Plan<NB, HG>;
+    constexpr int D = NB * 32, kE = HG == 4 ? 1 : 2, kPairs = NB / 2;
+    constexpr int kO = HG == 4 ? 2 : 4;               // outputs that a lane holds of an MMA tile
+    extern __shared__ __align__(128) unsigned char s_dyn[];
+    __shared__ Fragments s_frag;
 
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = lane >> 2, j = lane & 3;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, j = lane & 3;
     const float step = 2.0f * a.cent[15] / 15.0f;
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_ring) + warp * G::kWarpRing;
+    unsigned char* const s_warp = s_dyn + warp * L::kWarpBytes;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_warp);
+    unsigned char* const s_digits = s_warp + G::kWarpRing + L::kFragment;
+    const uint32_t digits = (uint32_t)__cvta_generic_to_shared(s_digits) + lane * 8;
+    const uint32_t halves = 2 * ring + kInFlight * G::kStage;   // (one half's address) + (the other's)
+    static_assert(kRing == 2 * kInFlight && kStepGroups == kInFlight, "the ring has two halves of a step each");
+    static_assert(L::kFragment <= G::kWarpRing, "a segment's outputs do not fit into the ring");
+    // a fragment's outputs [HG][D]: that of the warp's last segment lies in its idle ring
+    auto fragment = [&](int slot) { return reinterpret_cast<float*>(s_dyn + (slot >> 1) * L::kWarpBytes + ((slot & 1) ? 0 : G::kWarpRing)); };
     // ldmatrix: lane l gives the row address of token 8 ((l >> 3) & 1) + (l & 7), block 2 pair + (l >> 4)
     const int tok = 8 * ((lane >> 3) & 1) + (lane & 7);
     const uint32_t off_k = tok * G::kRow + (((lane >> 4) ^ G::swizzle(tok)) << 4);   // ^ 32 pair
@@ -101,73 +109,122 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
     const uint32_t off_ps = 2 * G::kIdx + lane * G::kSc;   // K scales of tokens 0..15, V scales behind them
     const int mask = (1 << a.page_shift) - 1;
 
-    WorkLine line(a);
-    write_empty<NB>(a);
-    while (line.more()) {
-        const Segment s = line.next();
-        __syncthreads();   // the last segment's end has read the shared arrays
+    if (threadIdx.x < 2 * kWorkWarps) s_frag.used[threadIdx.x] = 0;
+    WorkLine line(a);   // (its barriers stand before the first use of what is set above)
 
-        // ---- queries: rotated, scaled to integers, cut into digits ----
-        {
-            const float inv_sqrt = 1.0f / sqrtf((float)kBlock), sg = block_sign(lane, a.sign_mag);
-#pragma unroll 4
-            for (int u = warp; u < HG * NB; u += kWarps) {
-                const int hh = u / NB, b = u - hh * NB;
-                float v = hh < s.heads ? load_as_f32(a.q, a.q_dtype, (size_t)s.req * a.q_stride + (size_t)(s.head0 + hh) * D + b * 32 + lane) : 0.0f;
-                s_q[hh][b * 32 + lane] = wht32_across(v, lane) * inv_sqrt * sg;
-            }
-        }
-        // ---- the segment's groups of this warp ----
-        const int first = s.t0 + warp * kGroupTokens, last = s.t1 - 1;
-        const int groups = first < s.t1 ? (s.t1 - first + kTile - 1) / kTile : 0;
-        const int steps = (groups + kStepGroups - 1) / kStepGroups * kStepGroups;
-        const int32_t* table = a.table + (size_t)s.req * a.table_stride;
-        auto page_of = [&](int i) { return table[min(first + i * kTile, last) >> a.page_shift]; };
-        __syncthreads();
-        for (int hh = warp; hh < HG; hh += kWarps) {
-            uint32_t top = 0;   // of the bits, so that NaN is above infinity
-#pragma unroll
-            for (int i = 0; i < NB; ++i) top = max(top, __float_as_uint(s_q[hh][lane + 32 * i]) & 0x7fffffffu);
-            top = __reduce_max_sync(0xffffffffu, top);
-            const float m = __uint_as_float(top);
-            if (lane == 0) s_qsc[hh] = m <= FLT_MAX ? m : __uint_as_float(0x7fc00000u);   // not finite: every score is NaN
-        }
-        __syncthreads();
-        for (int b = warp; b < NB; b += kWarps) {
-            const int hh = HG == 4 ? n >> 1 : n;
-            const float m = s_qsc[hh], inv = m > 0.0f && m <= FLT_MAX ? kQMax / m : 0.0f;
-            uint32_t d0[2] = {0u, 0u}, d1[2] = {0u, 0u};   // [dims 8j + even | 8j + odd]
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float x = s_q[hh][32 * b + 8 * j + 2 * i + half];
-                    const int v = inv > 0.0f ? __float2int_rn(x * inv) : 0;
-                    const int lo = (int)(signed char)(v & 0xff);
-                    d0[half] |= (uint32_t)(lo & 0xff) << (8 * i);
-                    d1[half] |= (uint32_t)(((v - lo) >> 8) & 0xff) << (8 * i);
+    // ---- copies of a segment's groups, one behind the other ----
+    Segment s{};
+    int to_copy;                              // first token of the group that is copied next
+    int page_now, page_next;                  // pages 32 k + lane of the segment, for this k and the next
+    bool some_bad = false;                    // some page does not exist (of those looked at so far)
+    const uint8_t *kp, *vp;
+    const uint16_t* sp;
+    auto page_at = [&](int i) {               // of the segment's i-th page
+        const int page = a.table[s.req * a.table_stride + min((s.t0 >> a.page_shift) + i, (s.t1 - 1) >> a.page_shift)];
+        const bool bad = (unsigned)page >= (unsigned)a.num_pages;
+        some_bad |= __any_sync(0xffffffffu, bad) != 0;
+        return bad ? 0 : page;
+    };
+    auto open = [&]() {
+        some_bad = false;
+        to_copy = s.t0;
+        page_now = page_at(lane);
+        page_next = (s.t1 - 1) >> a.page_shift >= (s.t0 >> a.page_shift) + 32 ? page_at(32 + lane) : 0;
+    };
+    auto fill = [&](uint32_t st) {
+        if (to_copy < s.t1) {
+            if ((to_copy & mask) == 0 || to_copy == s.t0) {
+                const int i = (to_copy >> a.page_shift) - (s.t0 >> a.page_shift);
+                if (i > 0 && (i & 31) == 0) {
+                    page_now = page_next;
+                    page_next = page_at(i + 32 + lane);
                 }
-            if (HG == 4) {
-                s_qfr[0][b][lane] = (n & 1) ? make_uint2(d0[0], d0[1]) : make_uint2(d1[0], d1[1]);
-            } else {
-                s_qfr[0][b][lane] = make_uint2(d1[0], d1[1]);
-                s_qfr[kSets - 1][b][lane] = make_uint2(d0[0], d0[1]);
+                const int page = __shfl_sync(0xffffffffu, page_now, i & 31);
+                const uint32_t row = (((uint32_t)page * a.hkv + s.kvh) << a.page_shift) + (to_copy & mask);
+                kp = a.kb + (size_t)row * G::kRow + lane * 16;
+                vp = a.vb + (size_t)row * G::kRow + lane * 16;
+                sp = (lane < 16 ? a.ks : a.vs) + (size_t)(row + (lane & 15)) * NB;
             }
-        }
-        float qsc[kE];
+            // whole groups, also where the request ends inside: the page has the room
 #pragma unroll
-        for (int e = 0; e < kE; ++e) qsc[e] = s_qsc[HG == 4 ? j : 2 * j + e] * (a.qk_const * step / (kQMax * 16.0f));
-        __syncthreads();
-        const uint32_t qfr = (uint32_t)__cvta_generic_to_shared(&s_qfr[0][0][lane]);
+            for (int p = 0; p < G::kRow / 32; ++p) {
+                const uint32_t d = st + (NB == 8 && (p & 1) ? off_p ^ 64 : off_p) + p * 512;
+                cp_async16(d, kp + p * 512);
+                cp_async16(d + G::kIdx, vp + p * 512);
+            }
+            cp_async_small<G::kSc>(st + off_ps, sp);
+            kp += G::kIdx;
+            vp += G::kIdx;
+            sp += kGroupTokens * NB;
+        }
+        cp_async_commit();
+        to_copy += kGroupTokens;
+    };
+
+    while (line.next(s)) {
+        // ---- queries: rotated, scaled to integers, cut into digits ----
+        open();
+        float qsc[kE];
+        {
+            constexpr int kAtOnce = HG * NB <= 32 ? HG : 4;   // heads
+            const float inv_sqrt = 1.0f / sqrtf((float)kBlock), sg = block_sign(lane, a.sign_mag);
+            const size_t q0 = (size_t)s.req * a.q_stride + (size_t)s.head0 * D + lane;
+#pragma unroll
+            for (int e = 0; e < kE; ++e) qsc[e] = 0.0f;
+            // Byte i of k-slots 4j' + i of fragment (b, 4n' + j') is dim 32 b + 8 j' + 2 i (first word) or one above it (second), of
+            // column n': this lane's dim has j' = lane / 8, i = lane / 2 % 4, word lane % 2
+            unsigned char* const at = s_digits + (lane >> 3) * 8 + (lane & 1) * 4 + ((lane >> 1) & 3);
+#pragma unroll
+            for (int h0 = 0; h0 < HG; h0 += kAtOnce) {
+                float v[kAtOnce][NB];
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) v[i][b] = h0 + i < s.heads ? load_as_f32(a.q, a.q_dtype, q0 + (h0 + i) * D + b * 32) : 0.0f;
+                if (h0 == 0) {
+#pragma unroll
+                    for (int i = 0; i < kInFlight; ++i) fill(ring + i * G::kStage);
+                }
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    const int h = h0 + i;
+                    uint32_t top = 0;   // of the bits, so that NaN is above infinity
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        v[i][b] = wht32_across(v[i][b], lane) * inv_sqrt * sg;
+                        top = max(top, __float_as_uint(v[i][b]) & 0x7fffffffu);
+                    }
+                    float m = __uint_as_float(__reduce_max_sync(0xffffffffu, top));
+                    if (!(m <= FLT_MAX)) m = __uint_as_float(0x7fc00000u);   // not finite: every score is NaN
+                    const float inv = m > 0.0f ? kQMax / m : 0.0f;
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        // (inv is infinite where the largest component is below 1e-34)
+                        const int x = inv <= FLT_MAX ? __float2int_rn(v[i][b] * inv) : 0;
+                        const int lo = (int)(signed char)(x & 0xff), hi = (x - lo) >> 8;
+                        if (HG == 4) {
+                            at[b * 256 + (2 * h) * 32] = (unsigned char)hi;
+                            at[b * 256 + (2 * h + 1) * 32] = (unsigned char)lo;
+                        } else {
+                            at[b * 256 + h * 32] = (unsigned char)hi;
+                            at[(NB + b) * 256 + h * 32] = (unsigned char)lo;
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < kE; ++e)
+                        if (h == (HG == 4 ? j : 2 * j + e)) qsc[e] = m * (a.qk_const * step / (kQMax * 16.0f));
+                }
+            }
+            __syncwarp();
+        }
 
         float shift = kShift;
         float m_ref[kE], l_run[kE];
-        float o[NB][2][HG == 4 ? 2 : 4];
+        float o[NB][2][kO];
         for (;;) {
-            float thr[kE];
 #pragma unroll
             for (int e = 0; e < kE; ++e) {
-                m_ref[e] = thr[e] = kNoScore;
+                m_ref[e] = kNoScore;
                 l_run[e] = 0.0f;
             }
 #pragma unroll
@@ -175,70 +232,19 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
 #pragma unroll
                 for (int m = 0; m < 2; ++m)
 #pragma unroll
-                    for (int i = 0; i < (HG == 4 ? 2 : 4); ++i) o[b][m][i] = 0.0f;
-            int page_now = page_of(lane), page_next = page_of(32 + lane);
-            uint32_t bad = 0;   // groups in flight whose page does not exist: bit (group & 31)
-            uint32_t st_fill = ring, st = ring;
-            auto fill = [&](int i) {
-                if ((i & 31) == 0 && i > 0) {
-                    page_now = page_next;
-                    page_next = page_of(i + 32 + lane);
-                }
-                int page = __shfl_sync(0xffffffffu, page_now, i & 31);
-                const uint32_t bit = 1u << (i & 31);
-                bad &= ~bit;
-                if ((unsigned)page >= (unsigned)a.num_pages) {
-                    bad |= bit;
-                    page = 0;
-                }
-                if (i < steps) {
-                    const int gs = first + i * kTile;
-                    const uint32_t base = ((uint32_t)page * a.hkv + s.kvh) << a.page_shift;
-                    const uint16_t* scb = (lane < 16 ? a.ks : a.vs);
-                    if (gs + kGroupTokens <= s.t1) {
-                        const uint32_t row = base + (gs & mask);
-                        const uint8_t* k = a.kb + (size_t)row * G::kRow + lane * 16;
-                        const uint8_t* v = a.vb + (size_t)row * G::kRow + lane * 16;
+                    for (int i = 0; i < kO; ++i) o[b][m][i] = 0.0f;
+            uint32_t st = ring;
+            for (int t0 = s.t0; t0 < s.t1; t0 += kStepGroups * kGroupTokens) {
+                const uint32_t st_other = halves - st;
 #pragma unroll
-                        for (int p = 0; p < G::kRow / 32; ++p) {
-                            const uint32_t d = st_fill + (NB == 8 && (p & 1) ? off_p ^ 64 : off_p) + p * 512;
-                            cp_async16(d, k + p * 512);
-                            cp_async16(d + G::kIdx, v + p * 512);
-                        }
-                        cp_async_small<G::kSc>(st_fill + off_ps, scb + (size_t)(row + (lane & 15)) * NB);
-                    } else {   // rows behind the segment's last token read that one; they are masked
-#pragma unroll
-                        for (int p = 0; p < G::kRow / 32; ++p) {
-                            const uint32_t row = base + (min(gs + piece_t + p * (32 / NB), last) & mask);
-                            const size_t at = (size_t)row * G::kRow + piece_c * 16;
-                            const uint32_t d = st_fill + (NB == 8 && (p & 1) ? off_p ^ 64 : off_p) + p * 512;
-                            cp_async16(d, a.kb + at);
-                            cp_async16(d + G::kIdx, a.vb + at);
-                        }
-                        const uint32_t row = base + (min(gs + (lane & 15), last) & mask);
-                        cp_async_small<G::kSc>(st_fill + off_ps, scb + (size_t)row * NB);
-                    }
-                }
-                cp_async_commit();
-                st_fill = st_fill + G::kStage == ring + G::kWarpRing ? ring : st_fill + G::kStage;
-            };
-#pragma unroll
-            for (int i = 0; i < kInFlight; ++i) fill(i);
-            for (int it = 0; it < steps; it += kStepGroups) {
-#pragma unroll
-                for (int u = 0; u < kStepGroups; ++u) fill(it + kInFlight + u);
+                for (int u = 0; u < kStepGroups; ++u) fill(st_other + u * G::kStage);
                 cp_async_wait<kInFlight>();
                 __syncwarp();
-                uint32_t stu[kStepGroups];
-#pragma unroll
-                for (int u = 0; u < kStepGroups; ++u) {
-                    stu[u] = st;
-                    st = st + G::kStage == ring + G::kWarpRing ? ring : st + G::kStage;
-                }
                 // ---- scores ----
-                float sc[kStepGroups][2][kE];
+                float raw[kStepGroups][2][kE];
                 static_for<0, kStepGroups>([&](auto u_) {
                     constexpr int u = decltype(u_)::value;
+                    const uint32_t stu = st + u * G::kStage;
                     float acc[2][kE];
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
@@ -247,30 +253,30 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
                     static_for<0, kPairs>([&](auto p_) {
                         constexpr int p = decltype(p_)::value;
                         uint32_t kw[4];
-                        ldsm4_o<0>(stu[u] + (off_k ^ (32 * p)), kw);
-                        const uint32_t sa = lds32_o<4 * p>(stu[u] + off_s), sb = lds32_o<4 * p + 8 * G::kSc>(stu[u] + off_s);
+                        ldsm4_o<0>(stu + (off_k ^ (32 * p)), kw);
+                        const uint32_t sa = lds32_o<4 * p>(stu + off_s) & 0x7fff7fffu, sb = lds32_o<4 * p + 8 * G::kSc>(stu + off_s) & 0x7fff7fffu;
                         static_for<0, 2>([&](auto i_) {
                             constexpr int i = decltype(i_)::value, b = 2 * p + i;
-                            const float ka = fabsf(i ? __high2float(u32_as_h2(sa)) : __low2float(u32_as_h2(sa)));
-                            const float kb = fabsf(i ? __high2float(u32_as_h2(sb)) : __low2float(u32_as_h2(sb)));
+                            const float ka = i ? __high2float(u32_as_h2(sa)) : __low2float(u32_as_h2(sa));
+                            const float kc = i ? __high2float(u32_as_h2(sb)) : __low2float(u32_as_h2(sb));
                             // c ^ 8 is the two's complement of c - 8; at the top of a byte with bit 3 set below it: 16 (c - 7.5)
-                            const uint32_t u0 = kw[2 * i] ^ 0x88888888u, u1 = kw[2 * i + 1] ^ 0x88888888u;
-                            const uint32_t a0 = lop3_and_or(u0 << 4, 0xF0F0F0F0u, 0x08080808u), a2 = lop3_and_or(u0, 0xF0F0F0F0u, 0x08080808u);
-                            const uint32_t a1 = lop3_and_or(u1 << 4, 0xF0F0F0F0u, 0x08080808u), a3 = lop3_and_or(u1, 0xF0F0F0F0u, 0x08080808u);
-                            const uint2 qa = lds64_o<b * 256>(qfr);
+                            const uint32_t u0 = kw[2 * i], u1 = kw[2 * i + 1];
+                            const uint32_t a0 = lop3_xor_select(u0 << 4, 0xF0F0F0F0u, 0x88888888u), a2 = lop3_xor_select(u0, 0xF0F0F0F0u, 0x88888888u);
+                            const uint32_t a1 = lop3_xor_select(u1 << 4, 0xF0F0F0F0u, 0x88888888u), a3 = lop3_xor_select(u1, 0xF0F0F0F0u, 0x88888888u);
+                            const uint2 qa = lds64_o<b * 256>(digits);
                             int hi[4];
                             imma16832(hi, a0, a1, a2, a3, qa.x, qa.y);
-                            if (HG == 4) {
+                            if constexpr (HG == 4) {
                                 acc[0][0] = fmaf(ka, (float)(hi[0] * 256 + hi[1]), acc[0][0]);
-                                acc[1][0] = fmaf(kb, (float)(hi[2] * 256 + hi[3]), acc[1][0]);
+                                acc[1][0] = fmaf(kc, (float)(hi[2] * 256 + hi[3]), acc[1][0]);
                             } else {
-                                const uint2 qb = lds64_o<(NB + b) * 256>(qfr);
+                                const uint2 qb = lds64_o<(NB + b) * 256>(digits);
                                 int lo[4];
                                 imma16832(lo, a0, a1, a2, a3, qb.x, qb.y);
 #pragma unroll
                                 for (int e = 0; e < kE; ++e) {
                                     acc[0][e] = fmaf(ka, (float)(hi[e] * 256 + lo[e]), acc[0][e]);
-                                    acc[1][e] = fmaf(kb, (float)(hi[2 + e] * 256 + lo[2 + e]), acc[1][e]);
+                                    acc[1][e] = fmaf(kc, (float)(hi[2 + e] * 256 + lo[2 + e]), acc[1][e]);
                                 }
                             }
                         });
@@ -278,189 +284,203 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
 #pragma unroll
-                        for (int e = 0; e < kE; ++e) sc[u][t][e] = acc[t][e] * qsc[e];
-                    const int gs = first + (it + u) * kTile;
-                    const bool none = (bad >> ((it + u) & 31)) & 1u;
-                    if (none || gs + kGroupTokens > s.t1) {
+                        for (int e = 0; e < kE; ++e) raw[u][t][e] = acc[t][e];
+                });
+                // Tokens behind the segment's end and those of pages that do not exist: no score, and no scale of theirs meets a
+                // zero weight (it may be infinite or NaN).
+                bool out[kStepGroups][2];
+                uint32_t sv_mask[kStepGroups][2];
+#pragma unroll
+                for (int u = 0; u < kStepGroups; ++u)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        out[u][t] = false;
+                        sv_mask[u][t] = 0x7fff7fffu;
+                    }
+                if (some_bad || t0 + kStepGroups * kGroupTokens > s.t1) {
+#pragma unroll
+                    for (int u = 0; u < kStepGroups; ++u) {
+                        const int gs = t0 + u * kGroupTokens;
+                        const bool none = some_bad && (unsigned)a.table[s.req * a.table_stride + (min(gs, s.t1 - 1) >> a.page_shift)] >= (unsigned)a.num_pages;
 #pragma unroll
                         for (int t = 0; t < 2; ++t)
                             if (none || gs + n + 8 * t >= s.t1) {
-#pragma unroll
-                                for (int e = 0; e < kE; ++e) sc[u][t][e] = -INFINITY;
+                                out[u][t] = true;
+                                sv_mask[u][t] = 0u;
                             }
                     }
-                });
+                }
                 // ---- softmax ----
+                float x[kStepGroups][2][kE];
                 bool over = false;
-                float top[kE];
 #pragma unroll
                 for (int e = 0; e < kE; ++e) {
-                    top[e] = fmaxf(fmaxf(sc[0][0][e], sc[0][1][e]), fmaxf(sc[1][0][e], sc[1][1][e]));
-                    over |= top[e] > thr[e];
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int u = 0; u < kStepGroups; ++u)
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            x[u][t][e] = out[u][t] ? -INFINITY : fmaf(raw[u][t][e], qsc[e], -m_ref[e]);
+                            top = fmaxf(top, x[u][t][e]);
+                        }
+                    over |= top > shift + kLazy;
                 }
                 if (__any_sync(0xffffffffu, over)) {
-                    float keep[kE];
 #pragma unroll
                     for (int e = 0; e < kE; ++e) {
-                        float mx = top[e];
+                        float mx = -INFINITY;
+#pragma unroll
+                        for (int u = 0; u < kStepGroups; ++u)
+#pragma unroll
+                            for (int t = 0; t < 2; ++t)
+                                if (!out[u][t]) mx = fmaxf(mx, raw[u][t][e] * qsc[e]);
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                        const float m_new = mx > thr[e] ? mx - shift : m_ref[e];
-                        keep[e] = ex2(m_ref[e] - m_new);
+                        const float m_new = fmaxf(m_ref[e], mx - shift), keep = ex2(m_ref[e] - m_new);
                         m_ref[e] = m_new;
-                        thr[e] = m_new + (shift + kLazy);
-                        l_run[e] *= keep[e];
+                        l_run[e] *= keep;
+#pragma unroll
+                        for (int u = 0; u < kStepGroups; ++u)
+#pragma unroll
+                            for (int t = 0; t < 2; ++t) x[u][t][e] = out[u][t] ? -INFINITY : fmaf(raw[u][t][e], qsc[e], -m_new);
+#pragma unroll
+                        for (int b = 0; b < NB; ++b)
+#pragma unroll
+                            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                                for (int i = 0; i < kO; ++i)
+                                    if (HG == 4 || i % 2 == e) o[b][m][i] *= keep;
                     }
-#pragma unroll
-                    for (int b = 0; b < NB; ++b)
-#pragma unroll
-                        for (int m = 0; m < 2; ++m) {
-                            if (HG == 4) {
-                                o[b][m][0] *= keep[0];
-                                o[b][m][1] *= keep[0];
-                            } else {
-#pragma unroll
-                                for (int i = 0; i < (HG == 4 ? 2 : 4); ++i) o[b][m][i] *= keep[i % kE];
-                            }
-                        }
                 }
                 // ---- P' = p |s_v| as B fragments ----
                 uint32_t pq[kStepGroups][HG == 4 ? kPairs : NB][2];   // [octet]
                 static_for<0, kStepGroups>([&](auto u_) {
                     constexpr int u = decltype(u_)::value;
+                    const uint32_t stu = st + u * G::kStage;
                     static_for<0, 2>([&](auto t_) {
                         constexpr int t = decltype(t_)::value;
                         float p[kE];
 #pragma unroll
                         for (int e = 0; e < kE; ++e) {
-                            p[e] = ex2(sc[u][t][e] - m_ref[e]);
+                            p[e] = ex2(x[u][t][e]);
                             l_run[e] += p[e];
                         }
                         const uint32_t ph = h2_as_u32(__floats2half2_rn(p[0], p[kE - 1]));
                         static_for<0, kPairs>([&](auto p_) {
                             constexpr int pr = decltype(p_)::value;
-                            const uint32_t sv = lds32_o<16 * G::kSc + 8 * t * G::kSc + 4 * pr>(stu[u] + off_s);
-                            if (HG == 4) {   // columns 2j, 2j + 1: head j with the scales of blocks 2 pr, 2 pr + 1
-                                pq[u][pr][t] = movmatrix_trans(scaled(ph, sv));
-                            } else {         // columns 2j, 2j + 1: heads 2j, 2j + 1
-                                pq[u][2 * pr][t] = movmatrix_trans(scaled(ph, __byte_perm(sv, sv, 0x1010)));
-                                pq[u][2 * pr + (HG == 4 ? 0 : 1)][t] = movmatrix_trans(scaled(ph, __byte_perm(sv, sv, 0x3232)));
+                            const uint32_t sv = lds32_o<16 * G::kSc + 8 * t * G::kSc + 4 * pr>(stu + off_s) & sv_mask[u][t];
+                            if constexpr (HG == 4) {   // columns 2j, 2j + 1: head j with the scales of blocks 2 pr, 2 pr + 1
+                                pq[u][pr][t] = movmatrix_trans(product(ph, sv));
+                            } else {                   // columns 2j, 2j + 1: heads 2j, 2j + 1
+                                pq[u][2 * pr][t] = movmatrix_trans(product(ph, __byte_perm(sv, sv, 0x1010)));
+                                pq[u][2 * pr + 1][t] = movmatrix_trans(product(ph, __byte_perm(sv, sv, 0x3232)));
                             }
                         });
                     });
                 });
                 // ---- O^T += V^T P' ----
+                const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                 static_for<0, kPairs>([&](auto p_) {
                     constexpr int pr = decltype(p_)::value;
                     uint32_t vw[kStepGroups][4];
 #pragma unroll
-                    for (int u = 0; u < kStepGroups; ++u) ldsm4t_o<G::kIdx>(stu[u] + (off_k ^ (32 * pr)), vw[u]);
+                    for (int u = 0; u < kStepGroups; ++u) ldsm4t_o<G::kIdx>(st + u * G::kStage + (off_k ^ (32 * pr)), vw[u]);
                     float centre[4];
-                    if (HG == 4) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) centre[i] = 0.0f;
-#pragma unroll
-                        for (int u = 0; u < kStepGroups; ++u)
-                            mma16816(centre, kCentreEven, kCentreOdd, kCentreEven, kCentreOdd, pq[u][pr][0], pq[u][pr][1]);
-                    }
                     static_for<0, 2>([&](auto i_) {
                         constexpr int i = decltype(i_)::value, b = 2 * pr + i, f = HG == 4 ? pr : b;
-                        if (HG == 8) {
+                        if (HG == 8 || i == 0) {
+                            mma16816_from(centre, zero, kCentreEven, kCentreOdd, kCentreEven, kCentreOdd, pq[0][f][0], pq[0][f][1]);
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) centre[k] = 0.0f;
-#pragma unroll
-                            for (int u = 0; u < kStepGroups; ++u)
+                            for (int u = 1; u < kStepGroups; ++u)
                                 mma16816(centre, kCentreEven, kCentreOdd, kCentreEven, kCentreOdd, pq[u][f][0], pq[u][f][1]);
                         }
                         float acc[2][4];
-#pragma unroll
-                        for (int m = 0; m < 2; ++m)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) acc[m][k] = centre[k];
 #pragma unroll
                         for (int u = 0; u < kStepGroups; ++u) {
                             uint32_t xa[4], xb[4];   // tokens 2j, 2j + 1 and 2j + 8, 2j + 9: codes 4n .. 4n + 3 of the block
                             codes_to_subnormals(vw[u][2 * i], xa);
                             codes_to_subnormals(vw[u][2 * i + 1], xb);
 #pragma unroll
-                            for (int m = 0; m < 2; ++m)
-                                mma16816(acc[m], xa[2 * m], xa[2 * m + 1], xb[2 * m], xb[2 * m + 1], pq[u][f][0], pq[u][f][1]);
-                        }
-#pragma unroll
-                        for (int m = 0; m < 2; ++m) {
-                            if (HG == 4) {
-                                o[b][m][0] += acc[m][i];
-                                o[b][m][1] += acc[m][2 + i];
-                            } else {
-#pragma unroll
-                                for (int k = 0; k < (HG == 4 ? 2 : 4); ++k) o[b][m][k] += acc[m][k];
+                            for (int m = 0; m < 2; ++m) {
+                                if (u == 0) mma16816_from(acc[m], centre, xa[2 * m], xa[2 * m + 1], xb[2 * m], xb[2 * m + 1], pq[u][f][0], pq[u][f][1]);
+                                else mma16816(acc[m], xa[2 * m], xa[2 * m + 1], xb[2 * m], xb[2 * m + 1], pq[u][f][0], pq[u][f][1]);
                             }
                         }
+#pragma unroll
+                        for (int m = 0; m < 2; ++m)
+#pragma unroll
+                            for (int k = 0; k < kO; ++k) o[b][m][k] += HG == 4 ? acc[m][2 * k + i] : acc[m][k];
                     });
                 });
                 __syncwarp();   // the stages may be filled again
+                st = st_other;
             }
             cp_async_wait<0>();
+            __syncwarp();
             bool finite = true;
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
                 for (int m = 0; m < 2; ++m)
 #pragma unroll
-                    for (int i = 0; i < (HG == 4 ? 2 : 4); ++i) finite = finite && fabsf(o[b][m][i]) <= FLT_MAX;
-            // (also: all rings are idle now)
-            if (!__syncthreads_or(finite ? 0 : 1) || shift < 0.0f) break;
-            shift -= 6.0f;   // 8, 2, -4: p |s_v| is at most 65504 with the last
+                    for (int i = 0; i < kO; ++i) finite = finite && fabsf(o[b][m][i]) <= FLT_MAX;
+            if (__all_sync(0xffffffffu, finite) || shift < 0.0f) break;
+            shift -= 6.0f;   // 8, 2, -4: with the last, p |s_v| is at most 65504
+            open();
+#pragma unroll
+            for (int i = 0; i < kInFlight; ++i) fill(ring + i * G::kStage);
         }
 
-        // ---- the warps' parts ----
-#pragma unroll
-        for (int e = 0; e < kE; ++e) {
-            float l = l_run[e];
-            l += __shfl_xor_sync(0xffffffffu, l, 4);
-            l += __shfl_xor_sync(0xffffffffu, l, 8);
-            l += __shfl_xor_sync(0xffffffffu, l, 16);
-            if (n == 0) {
-                s_m[warp][HG == 4 ? j : 2 * j + e] = m_ref[e];
-                s_l[warp][HG == 4 ? j : 2 * j + e] = l;
-            }
-        }
+        // ---- the segment's end ----
+        const bool whole = s.whole();
+        const int slot = 2 * warp + (s.begins ? 1 : 0);
+        float* const to = fragment(slot);
         const float even = step * 8388608.0f, odd = step * 524288.0f;   // 2^23, 2^19
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
                 const int d = 32 * b + 4 * n + 2 * m;   // rows n / n + 8 of the MMA are dims d / d + 1
-                if (HG == 4) {
-                    *reinterpret_cast<float2*>(s_o + (warp * HG + j) * D + d) = make_float2(o[b][m][0] * even, o[b][m][1] * odd);
-                } else {
 #pragma unroll
-                    for (int e = 0; e < kE; ++e)
-                        *reinterpret_cast<float2*>(s_o + (warp * HG + 2 * j + e) * D + d) = make_float2(o[b][m][e] * even, o[b][m][(HG == 4 ? 0 : 2) + e] * odd);
+                for (int e = 0; e < kE; ++e)
+                    *reinterpret_cast<float2*>(to + (HG == 4 ? j : 2 * j + e) * D + d) = make_float2(o[b][m][e] * even, o[b][m][kO / 2 + e] * odd);
+            }
+#pragma unroll
+        for (int e = 0; e < kE; ++e) {
+            l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 4);
+            l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 8);
+            l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 16);
+            if (!whole && n == 0) {
+                s_frag.m[slot][HG == 4 ? j : 2 * j + e] = m_ref[e];
+                s_frag.l[slot][HG == 4 ? j : 2 * j + e] = l_run[e];
+            }
+        }
+        if (!whole && lane == 0) {
+            s_frag.seg[slot] = s;
+            s_frag.used[slot] = 1;
+        }
+        __syncwarp();
+        if (whole) {
+#pragma unroll
+            for (int h = 0; h < HG; ++h) {
+                const float l = __shfl_sync(0xffffffffu, l_run[h % kE], h / kE);
+                if (h < s.heads) {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) write_block<NB>(a, s.req, s.head0 + h, b, lane, to[h * D + b * 32 + lane], l);
                 }
             }
-        __syncthreads();
-        finish_segment<NB>(a, s, s_m, s_l, [&](int w, int h, int d) { return s_o[(w * HG + h) * D + d]; });
+            __syncwarp();
+        }
     }
+    finish<NB>(a, s_frag, [&](int c, int h, int d) { return fragment(c)[h * D + d]; });
+    write_empty<NB>(a);
 }
 
 template <int NB, int HG>
 int launch(const PagedArgs& a, cudaStream_t s) {
-    const int dyn = (kWorkThreads / 32) * Shape<NB>::kWarpRing;
-    // more than 48 KB of dynamic shared memory is a property of the kernel on a device: set once for each
-    static std::atomic<unsigned long long> configured{0};
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = -1;
-    if (dev < 0 || !((configured.load(std::memory_order_acquire) >> dev) & 1ull)) {
-        const cudaError_t e = cudaFuncSetAttribute(paged_mma_kernel<NB, HG>, cudaFuncAttributeMaxDynamicSharedMemorySize, dyn);
-        if (e != cudaSuccess) {
-            set_cuda_error(e);
-            return TQB_ERR_CUDA;
-        }
-        if (dev >= 0) configured.fetch_or(1ull << dev, std::memory_order_release);
-    }
-    paged_mma_kernel<NB, HG><<<148 * Plan<NB, HG>::kCtas, kWorkThreads, dyn, s>>>(a);
+    if (int st = allow_shared<paged_mma_kernel<NB, HG>>(Plan<NB, HG>::kBytes)) return st;
+    paged_mma_kernel<NB, HG><<<148 * Plan<NB, HG>::kCtas, kWorkThreads, Plan<NB, HG>::kBytes, s>>>(a);
     return check_launch(s);
 }
 

@@ -1,23 +1,31 @@
 // How the kernels of the paged attention share their work, and how the shares are joined.
 //
-// The work of a call is a line of tiles of kTile tokens: request after request, within a request KV head after KV head
-// (a group of more than eight query heads counts as several), within a head token after token.  CTA i of n takes the tiles
-// [i W / n, (i + 1) W / n): equal shares whatever the lengths are, worked out on the device from the lengths, so that a
-// captured launch serves any batch.  A share is cut into segments, one for each (request, head) that it touches.  A segment
-// that is the whole of its (request, head) is written to the output; otherwise its sum, maximum and un-normalised output go
-// to the scratch (a CTA has at most two such segments: its first and its last), and the CTA that arrives last at the
-// (request, head)'s ticket joins them in the order of the CTAs.  The result depends on the lengths alone.
+// The work of a call is a line of groups of 16 tokens: request after request, within a request KV head after KV head (a group
+// of more than eight query heads counts as several), within a head token after token; kOpenCost units stand before each
+// (request, head) for what it takes to begin one.  Every WARP takes an equal run of the line, whatever the lengths are,
+// worked out on the device from the lengths, so that a captured launch serves any batch.  A run is cut into segments, one
+// for each (request, head) that it touches.  A warp writes a segment that is the whole of its (request, head) to the
+// output by itself.  It has at most two others: one that began before it and one that goes on behind it.  These stay in
+// shared memory until the CTA's four warps are done and are joined there, and what crosses the CTA's ends goes to the
+// scratch (again at most two parts), where the CTA that arrives last at the (request, head)'s ticket joins the parts in the
+// order of the CTAs.  The result depends on the lengths alone.
+//
+// Measured at 128 requests of 62 to 1,000 tokens (8 KV heads, 4-bit): with CTAs instead of warps taking the runs, every
+// short segment paid its loads' latency and eight block barriers: 64 us.
 #pragma once
 #include "tqb_common.cuh"
 #include "tqb_paged.cuh"
 
 namespace tqb {
 
-constexpr int kTile = 64;            // tokens
+constexpr int kRunTokens = 16;       // of a group
+constexpr int kOpenCost = 2;         // groups that beginning a segment is worth
 constexpr int kSegHeads = 8;         // query heads of a segment, at most
-constexpr int kWorkThreads = 128;
+constexpr int kWorkWarps = 4;
+constexpr int kWorkThreads = 32 * kWorkWarps;
 constexpr int kMaxCtas = 148 * 8;    // of a launch: sizes tickets and partials
-static_assert(kMaxCtas * 4 <= TQB_PAGED_TICKET_BYTES, "a ticket for each CTA");
+constexpr int kMaxRound = 36;        // parts joined at a time, at most
+static_assert(kMaxCtas * 3 * 4 <= TQB_PAGED_TICKET_BYTES, "tickets of the last round, and of the slots for the one before it");
 constexpr float kNoScore = -1.0e30f; // finite stand-in for -inf: differences of two of them are 0
 
 struct PagedArgs {
@@ -33,7 +41,7 @@ struct PagedArgs {
     float* part_ml;      // [kMaxCtas][2][kSegHeads][2]: maximum (log2 units), sum
     float* part_out;     // [kMaxCtas][2][kSegHeads][D], rotated domain
     long long q_stride, table_stride;
-    int requests, max_blocks, page_shift, num_pages, hkv, group, vheads, splits;   // vheads = hkv * splits
+    int requests, max_blocks, max_len, page_shift, num_pages, hkv, group, vheads, splits;   // vheads = hkv * splits
     int q_dtype, out_dtype;
     float qk_const;      // softmax_scale * log2(e)
     float sign_mag;
@@ -45,106 +53,114 @@ int launch_paged_mma(const PagedArgs& a, int head_dim, cudaStream_t s);   // 4-b
 struct Segment {
     int req, kvh, head0, heads;   // query heads head0 .. head0 + heads - 1 of the request
     int t0, t1;                   // its tokens
-    bool whole;
-    int first, parts;             // not whole: the first CTA of the (request, head), and how many there are
-    int slot;                     // where this CTA's part goes: cta * 2 + (0: it began before this CTA, 1: it goes on behind it)
+    bool begins, ends;            // it has the first, the last token of its (request, head)
+    int cta0, ctas;               // the CTAs that share the (request, head)
+    __device__ __forceinline__ bool whole() const { return begins && ends; }
 };
 
+typedef unsigned long long Units;
+__device__ __forceinline__ Units divide(Units x, Units y) {   // (a 64-bit division is some 100 instructions in a row)
+    return ((x | y) >> 32) == 0 ? (unsigned)x / (unsigned)y : x / y;
+}
+
+// A warp's run of the line.
 struct WorkLine {
     const PagedArgs& a;
-    long long total, ctas, cur, end, base;   // tiles; base: first tile of request `req`
-    int req, tiles, len;
+    Units total, quot, rem;       // a run has quot units, the first `rem` runs one more
+    Units cur, end, base;         // base: where request `req` begins
+    int req, len;
 
-    __device__ __forceinline__ int length(int r) const {
-        const long long cap = min((long long)a.max_blocks << a.page_shift, 0x7fffffc0ll);
-        return (int)min((long long)max(a.lens[r], 0), cap);
+    __device__ __forceinline__ int length(int r) const { return min(max(a.lens[r], 0), a.max_len); }
+    static __device__ __forceinline__ unsigned groups_of(int len) { return (unsigned)(len + kRunTokens - 1) / kRunTokens; }
+    static __device__ __forceinline__ unsigned units_of(int len) { return len > 0 ? kOpenCost + groups_of(len) : 0u; }
+    __device__ __forceinline__ int owner(Units x) const {   // the run that unit x belongs to
+        const Units split = rem * (quot + 1);
+        return (int)(x < split ? divide(x, quot + 1) : rem + divide(x - split, quot));
     }
-    static __device__ __forceinline__ int tiles_of(int len) { return (len + kTile - 1) / kTile; }
 
     // All threads of the CTA.  Reads every request's length (4 bytes each, from L2): two block barriers.
     __device__ __forceinline__ explicit WorkLine(const PagedArgs& args) : a(args) {
-        __shared__ long long s_sum[kWorkThreads / 32];
-        __shared__ long long s_base;
-        __shared__ int s_req;
+        __shared__ Units s_sum[kWorkWarps], s_begin[kWorkThreads];
         const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
         const int per = (a.requests + kWorkThreads - 1) / kWorkThreads, r0 = min(tid * per, a.requests), r1 = min(r0 + per, a.requests);
-        long long mine = 0;
-        for (int r = r0; r < r1; ++r) mine += tiles_of(length(r));
-        long long incl = mine;
+        Units mine = 0;
+        for (int r = r0; r < r1; ++r) mine += units_of(length(r));
+        Units incl = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long x = __shfl_up_sync(0xffffffffu, incl, o);
+            const Units x = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += x;
         }
         if (lane == 31) s_sum[warp] = incl;
         __syncthreads();
         total = 0;
-        long long before = incl - mine;
+        Units before = incl - mine;
 #pragma unroll
-        for (int w = 0; w < kWorkThreads / 32; ++w) {
+        for (int w = 0; w < kWorkWarps; ++w) {
             if (w < warp) before += s_sum[w];
             total += s_sum[w];
         }
-        total *= a.vheads;
-        ctas = min((long long)gridDim.x, total);
-        cur = end = base = 0;
-        req = tiles = len = 0;
-        if ((long long)blockIdx.x >= ctas) return;   // (the same for the whole CTA)
-        cur = blockIdx.x * total / ctas;
-        end = (blockIdx.x + 1) * total / ctas;
-        const long long at = before * a.vheads;
-        if (at <= cur && cur < at + mine * a.vheads) {
-            long long b = at;
-            int r = r0;
-            for (; r < r1 - 1; ++r) {
-                const long long n = (long long)tiles_of(length(r)) * a.vheads;
-                if (cur < b + n) break;
-                b += n;
-            }
-            s_req = r;
-            s_base = b;
-        }
+        s_begin[tid] = before;
         __syncthreads();
-        req = s_req;
-        base = s_base;
+        total *= a.vheads;
+        // as many runs as the longest run needs: it is no longer with them, and fewer parts are joined
+        const unsigned most = gridDim.x * kWorkWarps, i = blockIdx.x * kWorkWarps + warp;
+        const Units longest = divide(total + most - 1, most), runs = longest > 0 ? divide(total + longest - 1, longest) : 0;
+        cur = end = base = 0;
+        quot = rem = 0;
+        req = len = 0;
+        if (i >= runs) return;
+        quot = divide(total, runs);
+        rem = total - quot * runs;
+        cur = i * quot + min((Units)i, rem);
+        end = cur + quot + (i < rem ? 1 : 0);
+        // the last of the threads' requests that begin at or before `cur`: four threads a lane, then their requests
+        int chunk = 0;
+#pragma unroll
+        for (int k = 0; k < kWorkWarps; ++k) chunk += __popc(__ballot_sync(0xffffffffu, s_begin[32 * k + lane] * a.vheads <= cur));
+        --chunk;   // (threads behind the last request begin at the total)
+        Units b = s_begin[chunk] * a.vheads;
+        req = min(chunk * per, a.requests - 1);
         len = length(req);
-        tiles = tiles_of(len);
-        if (tiles == 0) end = cur;
+        while (req + 1 < a.requests && cur >= b + (Units)units_of(len) * a.vheads) {
+            b += (Units)units_of(len) * a.vheads;
+            len = length(++req);
+        }
+        base = b;
+        if (len == 0) end = cur;   // not reached while the lengths stay as they are
     }
 
-    __device__ __forceinline__ bool more() const { return cur < end; }
-
-    // The segment at `cur`; moves on behind it.
-    __device__ __forceinline__ Segment next() {
-        Segment s;
-        const long long off = cur - base;
-        const int vh = (int)(off / tiles), t = (int)(off - (long long)vh * tiles);
-        const int n = (int)min((long long)(tiles - t), end - cur);
-        s.req = req;
-        s.kvh = vh / a.splits;
-        const int g0 = (vh - s.kvh * a.splits) * kSegHeads;
-        s.head0 = s.kvh * a.group + g0;
-        s.heads = min(a.group - g0, kSegHeads);
-        s.t0 = t * kTile;
-        s.t1 = min((t + n) * kTile, len);
-        s.whole = n == tiles;
-        s.first = 0;
-        s.parts = 1;
-        s.slot = blockIdx.x * 2 + (t == 0 ? 1 : 0);
-        if (!s.whole) {   // tile x belongs to CTA floor(((x + 1) ctas - 1) / total)
-            const long long x0 = cur - t, x1 = x0 + tiles - 1;
-            s.first = (int)(((x0 + 1) * ctas - 1) / total);
-            s.parts = (int)(((x1 + 1) * ctas - 1) / total) - s.first + 1;
+    // The next segment; false at the run's end.
+    __device__ __forceinline__ bool next(Segment& s) {
+        while (cur < end) {
+            const unsigned groups = groups_of(len), units = kOpenCost + groups, vh = (unsigned)divide(cur - base, units);
+            const Units start = base + (Units)vh * units;
+            const unsigned u0 = (unsigned)(cur - start), u1 = (unsigned)min((Units)units, u0 + (end - cur));
+            const unsigned g0 = max(u0, (unsigned)kOpenCost) - kOpenCost, g1 = max(u1, (unsigned)kOpenCost) - kOpenCost;
+            s.req = req;
+            s.kvh = (int)vh / a.splits;
+            const int h0 = ((int)vh - s.kvh * a.splits) * kSegHeads;
+            s.head0 = s.kvh * a.group + h0;
+            s.heads = min(a.group - h0, kSegHeads);
+            s.t0 = (int)g0 * kRunTokens;
+            s.t1 = min((int)g1 * kRunTokens, len);
+            s.begins = g0 == 0;
+            s.ends = g1 == groups;
+            s.cta0 = s.ctas = 0;
+            if (!s.whole()) {
+                s.cta0 = owner(start + kOpenCost) / kWorkWarps;
+                s.ctas = owner(start + units - 1) / kWorkWarps - s.cta0 + 1;
+            }
+            cur += u1 - u0;
+            if (cur < end && cur == base + (Units)units * a.vheads) {
+                base = cur;
+                len = 0;
+                while (len == 0 && req + 1 < a.requests) len = length(++req);
+                if (len == 0) end = cur;   // not reached while the lengths stay as they are
+            }
+            if (g1 > g0) return true;
         }
-        cur += n;
-        if (cur < end && cur == base + (long long)tiles * a.vheads) {
-            base = cur;
-            len = 0;
-            while (len == 0 && req + 1 < a.requests) len = length(++req);
-            tiles = tiles_of(len);
-            if (tiles == 0) end = cur;   // not reached while the lengths stay as they are
-        }
-        return s;
+        return false;
     }
 };
 
@@ -179,79 +195,171 @@ __device__ __forceinline__ void store_as(void* p, int dtype, size_t i, float v) 
     else reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
-// Rotated sum O over the softmax sum L of (head, block b), one lane a dim, back through the rotation and out.
+// Rotated output O of (query head `head`, block b), one lane a dim, over the softmax sum L, back through the rotation and out.
 template <int NB>
-__device__ __forceinline__ void write_block(const PagedArgs& a, const Segment& s, int hh, int b, int lane, float O, float L) {
+__device__ __forceinline__ void write_block(const PagedArgs& a, int req, int head, int b, int lane, float O, float L) {
     const float r = wht32_across(O * block_sign(lane, a.sign_mag), lane) * (1.0f / sqrtf((float)kBlock));
     // L is 0 where no page of the request can be read
-    store_as(a.out, a.out_dtype, ((size_t)s.req * a.hkv * a.group + s.head0 + hh) * (NB * 32) + b * 32 + lane, L == 0.0f ? 0.0f : r / L);
+    store_as(a.out, a.out_dtype, ((size_t)req * a.hkv * a.group + head) * (NB * 32) + b * 32 + lane, L == 0.0f ? 0.0f : r / L);
 }
 
-// The segment's end, by all threads of the CTA: `value(warp, head, dim)` is a warp's un-normalised rotated output relative to
-// its maximum s_m[warp][head], s_l its sum.  A (head, block) unit a warp at a time.
-template <int NB, typename F>
-__device__ __forceinline__ void finish_segment(const PagedArgs& a, const Segment& s, const float (*s_m)[kSegHeads], const float (*s_l)[kSegHeads], F value) {
-    constexpr int kWarps = kWorkThreads / 32, D = NB * 32;
-    __shared__ int s_arrived;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int u = warp; u < s.heads * NB; u += kWarps) {
-        const int hh = u / NB, b = u - hh * NB;
-        float M = s_m[0][hh];
-#pragma unroll
-        for (int w = 1; w < kWarps; ++w) M = fmaxf(M, s_m[w][hh]);
-        float L = 0.0f, O = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const float e = exp2_fast(s_m[w][hh] - M);
-            L = fmaf(s_l[w][hh], e, L);
-            O = fmaf(value(w, hh, b * 32 + lane), e, O);
-        }
-        if (s.whole) {
-            write_block<NB>(a, s, hh, b, lane, O, L);
-        } else {
-            const size_t at = (size_t)s.slot * kSegHeads + hh;
-            a.part_out[at * D + b * 32 + lane] = O;
-            if (b == 0 && lane == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(M, L);
-        }
+// How many of a (request, head)'s parts are joined at a time: up to 16 at once, more of them in two rounds.  (A round is a
+// fence, a ticket and two dependent trips to L2, about 2.5 us; 93 parts in one round took a CTA 30 us.)
+__device__ __forceinline__ int parts_per_round(int parts) { return parts <= 16 ? parts : parts <= 64 ? 8 : parts <= 256 ? 16 : kMaxRound; }
+static_assert(kMaxRound * kMaxRound >= kMaxCtas, "two rounds are enough");
+
+// One arrival at a ticket of `want`, after everything that the CTA's threads have written; true for the last one, whose
+// threads then see what the others have written.
+__device__ __forceinline__ bool last_arrival(unsigned* ticket, int want) {
+    __shared__ int s_last;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        unsigned old;
+        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;\n" : "=r"(old) : "l"(ticket) : "memory");
+        s_last = old == (unsigned)(want - 1);
+        if (s_last) *ticket = 0u;   // ready for the next call
     }
-    if (s.whole) return;
-    __threadfence();
     __syncthreads();
-    if (threadIdx.x == 0) s_arrived = atomicAdd(a.tickets + s.first, 1u) == (unsigned)(s.parts - 1);
-    __syncthreads();
-    if (!s_arrived) return;
-    __threadfence();
-    for (int u = warp; u < s.heads * NB; u += kWarps) {
-        const int hh = u / NB, b = u - hh * NB;
-        // part 0 is the second slot of CTA `first`, part i the first slot of CTA first + i
-        auto at = [&](int i) { return (size_t)((s.first + i) * 2 + (i == 0 ? 1 : 0)) * kSegHeads + hh; };
-        float M = kNoScore;
-        for (int i = lane; i < s.parts; i += 32) M = fmaxf(M, __ldcg(a.part_ml + at(i) * 2));
+    return s_last != 0;
+}
+
+// Where part i of a (request, head) lies: of the first CTA the second slot, of the others the first.
+__device__ __forceinline__ size_t part_at(int cta0, int i) { return (size_t)((cta0 + i) * 2 + (i == 0 ? 1 : 0)) * kSegHeads; }
+
+// Joins parts i0, i0 + stride, .. (`count` <= kMaxRound of them) of a (request, head): into the output, or into the place
+// of part i0.
+template <int NB>
+__device__ __forceinline__ void join_parts(const PagedArgs& a, const Segment& s, int i0, int stride, int count, bool to_out) {
+    constexpr int D = NB * 32, kUnits = 4;
+    __shared__ float s_w[kSegHeads][kMaxRound], s_L[kSegHeads];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int hh = warp; hh < s.heads; hh += kWorkWarps) {
+        float2 ml[(kMaxRound + 31) / 32];
+        float M = kNoScore, L = 0.0f;
+#pragma unroll
+        for (int k = 0; k < (kMaxRound + 31) / 32; ++k) {
+            const int i = k * 32 + lane;
+            ml[k] = i < count ? __ldcg(reinterpret_cast<const float2*>(a.part_ml + (part_at(s.cta0, i0 + i * stride) + hh) * 2)) : make_float2(kNoScore, 0.0f);
+            M = fmaxf(M, ml[k].x);
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        float L = 0.0f, O = 0.0f;
-        for (int i0 = 0; i0 < s.parts; i0 += 32) {
-            float w = 0.0f;
-            if (i0 + lane < s.parts) {
-                const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.part_ml + at(i0 + lane) * 2));
-                w = exp2_fast(ml.x - M);
-                L = fmaf(ml.y, w, L);
-            }
-            const int n = min(32, s.parts - i0);
-            for (int i = 0; i < n; i += 8) {
-                float v[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] = i + k < n ? __ldcg(a.part_out + at(i0 + i + k) * D + b * 32 + lane) : 0.0f;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) O = fmaf(v[k], __shfl_sync(0xffffffffu, w, (i + k) & 31), O);
+        for (int k = 0; k < (kMaxRound + 31) / 32; ++k) {
+            const int i = k * 32 + lane;
+            const float w = exp2_fast(ml[k].x - M);
+            if (i < count) {
+                s_w[hh][i] = w;
+                L = fmaf(ml[k].y, w, L);
             }
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-        write_block<NB>(a, s, hh, b, lane, O, L);
+        if (lane == 0) {
+            s_L[hh] = L;
+            if (!to_out) *reinterpret_cast<float2*>(a.part_ml + (part_at(s.cta0, i0) + hh) * 2) = make_float2(M, L);
+        }
     }
     __syncthreads();
-    if (threadIdx.x == 0) a.tickets[s.first] = 0u;   // ready for the next call
+    const int units = s.heads * NB;
+    for (int u0 = warp; u0 < units; u0 += kWorkWarps * kUnits) {   // four (head, block) units at a time: their loads are in flight together
+        float O[kUnits];
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k) O[k] = 0.0f;
+        for (int i = 0; i < count; i += 4) {
+            float v[4][kUnits];
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int k = 0; k < kUnits; ++k) {
+                    const int u = u0 + k * kWorkWarps;
+                    v[x][k] = i + x < count && u < units ? __ldcg(a.part_out + part_at(s.cta0, i0 + (i + x) * stride) * D + u * 32 + lane) : 0.0f;
+                }
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int k = 0; k < kUnits; ++k) {
+                    const int u = u0 + k * kWorkWarps;
+                    if (i + x < count && u < units) O[k] = fmaf(v[x][k], s_w[u / NB][i + x], O[k]);
+                }
+        }
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k) {
+            const int u = u0 + k * kWorkWarps;
+            if (u < units) {
+                if (to_out) write_block<NB>(a, s.req, s.head0 + u / NB, u % NB, lane, O[k], s_L[u / NB]);
+                else a.part_out[part_at(s.cta0, i0) * D + u * 32 + lane] = O[k];
+            }
+        }
+    }
+    __syncthreads();   // s_w is free again
+}
+
+// A CTA's segments that are not whole: of each warp the one that began before it (slot 2 w) and the one that goes on behind it
+// (slot 2 w + 1).  A segment that began before the warp and goes on behind it has slot 2 w.
+struct Fragments {
+    Segment seg[2 * kWorkWarps];
+    float m[2 * kWorkWarps][kSegHeads], l[2 * kWorkWarps][kSegHeads];   // maximum (log2 units) and sum
+    int used[2 * kWorkWarps];
+};
+
+// The CTA's end, by all of its threads: value(slot, head, dim) is a fragment's un-normalised rotated output.
+template <int NB, typename F>
+__device__ __forceinline__ void finish(const PagedArgs& a, const Fragments& f, F value) {
+    constexpr int D = NB * 32;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __syncthreads();
+    int crossing[2] = {-1, -1};   // a slot of the (request, head) that crosses the CTA's beginning | only its end
+    for (int c0 = 0; c0 < 2 * kWorkWarps;) {
+        if (!f.used[c0]) {
+            ++c0;
+            continue;
+        }
+        int c1 = c0 + 1;   // the fragments of one (request, head): up to the next odd slot
+        while (c1 < 2 * kWorkWarps && (!f.used[c1] || (c1 & 1) == 0)) ++c1;
+        int last = c0;
+        for (int c = c0 + 1; c < c1; ++c)
+            if (f.used[c]) last = c;
+        const Segment& s = f.seg[c0];
+        const bool done = s.begins && f.seg[last].ends;
+        const int side = s.begins ? 1 : 0;
+        if (!done) crossing[side] = c0;
+        for (int u = warp; u < s.heads * NB; u += kWorkWarps) {
+            const int hh = u / NB, b = u - hh * NB;
+            float M = kNoScore;
+            for (int c = c0; c <= last; ++c)
+                if (f.used[c]) M = fmaxf(M, f.m[c][hh]);
+            float L = 0.0f, O = 0.0f;
+            for (int c = c0; c <= last; ++c)
+                if (f.used[c]) {
+                    const float e = exp2_fast(f.m[c][hh] - M);
+                    L = fmaf(f.l[c][hh], e, L);
+                    O = fmaf(value(c, hh, b * 32 + lane), e, O);
+                }
+            if (done) {
+                write_block<NB>(a, s.req, s.head0 + hh, b, lane, O, L);
+            } else {
+                const size_t at = (size_t)(blockIdx.x * 2 + side) * kSegHeads + hh;
+                a.part_out[at * D + b * 32 + lane] = O;
+                if (b == 0 && lane == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(M, L);
+            }
+        }
+        c0 = c1;
+    }
+#pragma unroll 1
+    for (int side = 0; side < 2; ++side) {
+        if (crossing[side] < 0) continue;
+        const Segment& s = f.seg[crossing[side]];
+        const int per = parts_per_round(s.ctas);
+        int rounds = s.ctas;
+        if (per < s.ctas) {
+            const int mine = (int)blockIdx.x - s.cta0, i0 = mine / per * per, count = min(per, s.ctas - i0);
+            rounds = (s.ctas + per - 1) / per;
+            if (!last_arrival(a.tickets + kMaxCtas + (s.cta0 + i0) * 2 + (i0 == 0 ? 1 : 0), count)) continue;
+            join_parts<NB>(a, s, i0, 1, count, false);
+        }
+        if (last_arrival(a.tickets + s.cta0, rounds)) join_parts<NB>(a, s, 0, per < s.ctas ? per : 1, rounds, true);
+    }
 }
 
 // Requests without tokens get zeros.
@@ -259,7 +367,7 @@ template <int NB>
 __device__ __forceinline__ void write_empty(const PagedArgs& a) {
     const int row = a.hkv * a.group * NB * 32;
     for (int r = blockIdx.x; r < a.requests; r += gridDim.x) {
-        if (a.lens[r] > 0 && a.max_blocks > 0) continue;
+        if (a.lens[r] > 0 && a.max_len > 0) continue;
         for (int i = threadIdx.x; i < row; i += kWorkThreads) store_as(a.out, a.out_dtype, (size_t)r * row + i, 0.0f);
     }
 }

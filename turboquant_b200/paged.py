@@ -14,7 +14,7 @@ from ._lib import TqbPagedAttentionParams, TqbPagedLayer, TqbRopeParams, lib
 from .api import ALL_BLOCKS, TQB_ERR_UNSUPPORTED, DecodeOutput, DimensionMismatch, QuantNormMode, TqbRuntimeError, check
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_TICKET_BYTES = 8192   # TQB_PAGED_TICKET_BYTES
+_TICKET_BYTES = 16384   # TQB_PAGED_TICKET_BYTES
 _INTERLEAVED, _NO_NORM, _POSITIONS_64 = 1, 2, 4
 _PLAN_STATUS = {1: "not enough free pages", 2: "a request's length is negative or beyond its block table",
                 3: "more new tokens than the plan's capacity"}
