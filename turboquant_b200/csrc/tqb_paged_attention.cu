@@ -17,7 +17,7 @@ __global__ void __launch_bounds__(kWorkThreads) paged_simple_kernel(const __grid
     constexpr int D = NB * 32;
     __shared__ float s_cent[16];
     __shared__ Fragments s_frag;
-    extern __shared__ float s_o[];   // [2 kWorkWarps][kSegHeads][D]
+    extern __shared__ __align__(16) float s_o[];   // [2 kWorkWarps][kSegHeads][D]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid < 16) s_cent[tid] = a.cent[tid];
     if (tid < 2 * kWorkWarps) s_frag.used[tid] = 0;
@@ -69,15 +69,12 @@ __global__ void __launch_bounds__(kWorkThreads) paged_simple_kernel(const __grid
                 for (int b = 0; b < NB; ++b) o[h][b] = fmaf(o[h][b], keep, p * v[b]);
             }
         }
+        // (a whole segment's outputs pass through the slot of the warp's last one)
         const int slot = 2 * warp + (s.begins ? 1 : 0);
 #pragma unroll
         for (int h = 0; h < kSegHeads; ++h) {
-            if (h >= s.heads) break;
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                if (s.whole()) write_block<NB>(a, s.req, s.head0 + h, b, lane, o[h][b], l[h]);
-                else s_o[(slot * kSegHeads + h) * D + b * 32 + lane] = o[h][b];
-            }
+            for (int b = 0; b < NB; ++b) s_o[(slot * kSegHeads + h) * D + b * 32 + lane] = o[h][b];
             if (!s.whole() && lane == 0) {
                 s_frag.m[slot][h] = m[h];
                 s_frag.l[slot][h] = l[h];
@@ -87,8 +84,20 @@ __global__ void __launch_bounds__(kWorkThreads) paged_simple_kernel(const __grid
             s_frag.seg[slot] = s;
             s_frag.used[slot] = 1;
         }
+        __syncwarp();
+        if (s.whole()) {
+            const int quads = s.heads * (D / 4);
+            for (int x0 = 0; x0 < quads; x0 += 32) {
+                const int x = min(x0 + lane, quads - 1), hh = x / (D / 4);
+                float L = l[0];
+#pragma unroll
+                for (int h = 1; h < kSegHeads; ++h) L = h == hh ? l[h] : L;
+                write_quad<NB>(a, s, x, x0 + lane < quads, reinterpret_cast<const float4*>(s_o + slot * kSegHeads * D)[x], L);
+            }
+            __syncwarp();
+        }
     }
-    finish<NB>(a, s_frag, [&](int c, int h, int d) { return s_o[(c * kSegHeads + h) * D + d]; });
+    finish<NB>(a, s_frag, [&](int c, int x) { return reinterpret_cast<const float4*>(s_o + c * kSegHeads * D)[x]; });
     write_empty<NB>(a);
 }
 

@@ -163,7 +163,6 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
 
     while (line.next(s)) {
         // ---- queries: rotated, scaled to integers, cut into digits ----
-        open();
         float qsc[kE];
         {
             constexpr int kAtOnce = HG * NB <= 32 ? HG : 4;   // heads
@@ -181,7 +180,8 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
                 for (int i = 0; i < kAtOnce; ++i)
 #pragma unroll
                     for (int b = 0; b < NB; ++b) v[i][b] = h0 + i < s.heads ? load_as_f32(a.q, a.q_dtype, q0 + (h0 + i) * D + b * 32) : 0.0f;
-                if (h0 == 0) {
+                if (h0 == 0) {   // (behind the queries' loads)
+                    open();
 #pragma unroll
                     for (int i = 0; i < kInFlight; ++i) fill(ring + i * G::kStage);
                 }
@@ -462,18 +462,17 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
         }
         __syncwarp();
         if (whole) {
+            const int quads = s.heads * (D / 4);
 #pragma unroll
-            for (int h = 0; h < HG; ++h) {
-                const float l = __shfl_sync(0xffffffffu, l_run[h % kE], h / kE);
-                if (h < s.heads) {
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) write_block<NB>(a, s.req, s.head0 + h, b, lane, to[h * D + b * 32 + lane], l);
-                }
+            for (int x0 = 0; x0 < HG * (D / 4); x0 += 32) {
+                const int x = x0 + lane, h = x / (D / 4);
+                const float l0 = __shfl_sync(0xffffffffu, l_run[0], h / kE), l1 = __shfl_sync(0xffffffffu, l_run[kE - 1], h / kE);
+                if (x0 < quads) write_quad<NB>(a, s, x, x < quads, reinterpret_cast<const float4*>(to)[x], (h % kE) ? l1 : l0);
             }
             __syncwarp();
         }
     }
-    finish<NB>(a, s_frag, [&](int c, int h, int d) { return fragment(c)[h * D + d]; });
+    finish<NB>(a, s_frag, [&](int c, int x) { return reinterpret_cast<const float4*>(fragment(c))[x]; });
     write_empty<NB>(a);
 }
 

@@ -59,8 +59,15 @@ struct Segment {
 };
 
 typedef unsigned long long Units;
-__device__ __forceinline__ Units divide(Units x, Units y) {   // (a 64-bit division is some 100 instructions in a row)
-    return ((x | y) >> 32) == 0 ? (unsigned)x / (unsigned)y : x / y;
+// x / y for quotients below 2^21: up to 2^31 the f32 quotient is off by less than 1/2, so one step mends it.  (Integer
+// divisions are 50 to 100 instructions one behind the other, and a run begins with seven of them.)
+__device__ __forceinline__ Units divide(Units x, Units y) {
+    if (((x | y) >> 31) != 0) return x / y;
+    const unsigned n = (unsigned)x, d = (unsigned)y;
+    unsigned q = (unsigned)__fdividef((float)n, (float)d);
+    const int r = (int)(n - q * d);
+    q += r < 0 ? -1 : r >= (int)d ? 1 : 0;
+    return q;
 }
 
 // A warp's run of the line.
@@ -138,7 +145,7 @@ struct WorkLine {
             const unsigned u0 = (unsigned)(cur - start), u1 = (unsigned)min((Units)units, u0 + (end - cur));
             const unsigned g0 = max(u0, (unsigned)kOpenCost) - kOpenCost, g1 = max(u1, (unsigned)kOpenCost) - kOpenCost;
             s.req = req;
-            s.kvh = (int)vh / a.splits;
+            s.kvh = a.splits == 1 ? (int)vh : (int)vh / a.splits;
             const int h0 = ((int)vh - s.kvh * a.splits) * kSegHeads;
             s.head0 = s.kvh * a.group + h0;
             s.heads = min(a.group - h0, kSegHeads);
@@ -195,12 +202,50 @@ __device__ __forceinline__ void store_as(void* p, int dtype, size_t i, float v) 
     else reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
-// Rotated output O of (query head `head`, block b), one lane a dim, over the softmax sum L, back through the rotation and out.
+__device__ __forceinline__ void store4(void* p, int dtype, size_t i, const float (&v)[4]) {   // i: a multiple of 4
+    if (dtype == TQB_F32) {
+        *reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
+    } else if (dtype == TQB_F16) {
+        const __half2 x = __floats2half2_rn(v[0], v[1]), y = __floats2half2_rn(v[2], v[3]);
+        *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(p) + i) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+    } else {
+        const __nv_bfloat162 x = __floats2bfloat162_rn(v[0], v[1]), y = __floats2bfloat162_rn(v[2], v[3]);
+        *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p) + i) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+    }
+}
+
+// Outputs leave four dims a lane: lane l of a warp has the quad `x` (x = l modulo 8) of a request's heads, head0 * D / 4 + x ..
+// Rotated output O over the softmax sum L, back through the rotation (stages 1, 2 in the lane, 4, 8, 16 between lanes).
+// All lanes of the warp take part.
 template <int NB>
-__device__ __forceinline__ void write_block(const PagedArgs& a, int req, int head, int b, int lane, float O, float L) {
-    const float r = wht32_across(O * block_sign(lane, a.sign_mag), lane) * (1.0f / sqrtf((float)kBlock));
-    // L is 0 where no page of the request can be read
-    store_as(a.out, a.out_dtype, ((size_t)req * a.hkv * a.group + head) * (NB * 32) + b * 32 + lane, L == 0.0f ? 0.0f : r / L);
+__device__ __forceinline__ void write_quad(const PagedArgs& a, const Segment& s, int x, bool live, float4 O, float L) {
+    const int lane = threadIdx.x & 31;
+    float v[4] = {O.x, O.y, O.z, O.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] *= ((0xB1A6D4B2u >> (4 * (lane & 7) + i)) & 1u) ? -a.sign_mag : a.sign_mag;   // src/cache/precomputed/rotation.rs:16-20
+    const float p = v[0] + v[1], q = v[0] - v[1], r = v[2] + v[3], t = v[2] - v[3];
+    v[0] = p + r;
+    v[1] = q + t;
+    v[2] = p - r;
+    v[3] = q - t;
+#pragma unroll
+    for (int m = 1; m <= 4; m <<= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float other = __shfl_xor_sync(0xffffffffu, v[i], m);
+            v[i] = (lane & m) ? (other - v[i]) : (v[i] + other);
+        }
+    const float inv = L == 0.0f ? 0.0f : (1.0f / sqrtf((float)kBlock)) / L;   // L is 0 where no page of the request can be read
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] *= inv;
+    if (live) store4(a.out, a.out_dtype, ((size_t)s.req * a.hkv * a.group + s.head0) * (NB * 32) + 4 * x, v);
+}
+
+__device__ __forceinline__ void add_scaled(float4& acc, float4 v, float w) {
+    acc.x = fmaf(v.x, w, acc.x);
+    acc.y = fmaf(v.y, w, acc.y);
+    acc.z = fmaf(v.z, w, acc.z);
+    acc.w = fmaf(v.w, w, acc.w);
 }
 
 // How many of a (request, head)'s parts are joined at a time: up to 16 at once, more of them in two rounds.  (A round is a
@@ -230,7 +275,7 @@ __device__ __forceinline__ size_t part_at(int cta0, int i) { return (size_t)((ct
 // of part i0.
 template <int NB>
 __device__ __forceinline__ void join_parts(const PagedArgs& a, const Segment& s, int i0, int stride, int count, bool to_out) {
-    constexpr int D = NB * 32, kUnits = 4;
+    constexpr int D = NB * 32, kAtOnce = 8;
     __shared__ float s_w[kSegHeads][kMaxRound], s_L[kSegHeads];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int hh = warp; hh < s.heads; hh += kWorkWarps) {
@@ -261,36 +306,22 @@ __device__ __forceinline__ void join_parts(const PagedArgs& a, const Segment& s,
         }
     }
     __syncthreads();
-    const int units = s.heads * NB;
-    for (int u0 = warp; u0 < units; u0 += kWorkWarps * kUnits) {   // four (head, block) units at a time: their loads are in flight together
-        float O[kUnits];
+    const int quads = s.heads * (D / 4);
+    for (int x0 = warp * 32; x0 < quads; x0 += kWorkThreads) {
+        const int x = min(x0 + lane, quads - 1), hh = x / (D / 4);
+        const bool live = x0 + lane < quads;
+        float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int i = 0; i < count; i += kAtOnce) {   // loads that are in flight together
+            float4 v[kAtOnce];
 #pragma unroll
-        for (int k = 0; k < kUnits; ++k) O[k] = 0.0f;
-        for (int i = 0; i < count; i += 4) {
-            float v[4][kUnits];
+            for (int k = 0; k < kAtOnce; ++k)
+                if (i + k < count) v[k] = __ldcg(reinterpret_cast<const float4*>(a.part_out + part_at(s.cta0, i0 + (i + k) * stride) * D) + x);
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-#pragma unroll
-                for (int k = 0; k < kUnits; ++k) {
-                    const int u = u0 + k * kWorkWarps;
-                    v[x][k] = i + x < count && u < units ? __ldcg(a.part_out + part_at(s.cta0, i0 + (i + x) * stride) * D + u * 32 + lane) : 0.0f;
-                }
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-#pragma unroll
-                for (int k = 0; k < kUnits; ++k) {
-                    const int u = u0 + k * kWorkWarps;
-                    if (i + x < count && u < units) O[k] = fmaf(v[x][k], s_w[u / NB][i + x], O[k]);
-                }
+            for (int k = 0; k < kAtOnce; ++k)
+                if (i + k < count) add_scaled(O, v[k], s_w[hh][i + k]);
         }
-#pragma unroll
-        for (int k = 0; k < kUnits; ++k) {
-            const int u = u0 + k * kWorkWarps;
-            if (u < units) {
-                if (to_out) write_block<NB>(a, s.req, s.head0 + u / NB, u % NB, lane, O[k], s_L[u / NB]);
-                else a.part_out[part_at(s.cta0, i0) * D + u * 32 + lane] = O[k];
-            }
-        }
+        if (to_out) write_quad<NB>(a, s, x, live, O, s_L[hh]);
+        else if (live) reinterpret_cast<float4*>(a.part_out + part_at(s.cta0, i0) * D)[x] = O;
     }
     __syncthreads();   // s_w is free again
 }
@@ -303,48 +334,47 @@ struct Fragments {
     int used[2 * kWorkWarps];
 };
 
-// The CTA's end, by all of its threads: value(slot, head, dim) is a fragment's un-normalised rotated output.
+// The CTA's end, by all of its threads: quad(slot, x) are four of a fragment's un-normalised rotated outputs.
 template <int NB, typename F>
-__device__ __forceinline__ void finish(const PagedArgs& a, const Fragments& f, F value) {
+__device__ __forceinline__ void finish(const PagedArgs& a, const Fragments& f, F quad) {
     constexpr int D = NB * 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     __syncthreads();
+    unsigned used = 0;
+#pragma unroll
+    for (int c = 0; c < 2 * kWorkWarps; ++c) used |= f.used[c] ? 1u << c : 0u;
     int crossing[2] = {-1, -1};   // a slot of the (request, head) that crosses the CTA's beginning | only its end
-    for (int c0 = 0; c0 < 2 * kWorkWarps;) {
-        if (!f.used[c0]) {
-            ++c0;
-            continue;
-        }
-        int c1 = c0 + 1;   // the fragments of one (request, head): up to the next odd slot
-        while (c1 < 2 * kWorkWarps && (!f.used[c1] || (c1 & 1) == 0)) ++c1;
-        int last = c0;
-        for (int c = c0 + 1; c < c1; ++c)
-            if (f.used[c]) last = c;
+    while (used != 0) {
+        const int c0 = __ffs(used) - 1;
+        // the fragments of one (request, head): up to the next odd slot
+        const unsigned odd = used & 0xaau & ~((2u << c0) - 1), mine = used & (odd != 0 ? (odd & (0u - odd)) - 1 : ~0u);
+        used &= ~mine;
+        const int last = 31 - __clz(mine);
         const Segment& s = f.seg[c0];
         const bool done = s.begins && f.seg[last].ends;
         const int side = s.begins ? 1 : 0;
         if (!done) crossing[side] = c0;
-        for (int u = warp; u < s.heads * NB; u += kWorkWarps) {
-            const int hh = u / NB, b = u - hh * NB;
+        const int quads = s.heads * (D / 4);
+        const size_t at = (size_t)(blockIdx.x * 2 + side) * kSegHeads;
+        for (int x0 = warp * 32; x0 < quads; x0 += kWorkThreads) {
+            const int x = min(x0 + lane, quads - 1), hh = x / (D / 4);
             float M = kNoScore;
-            for (int c = c0; c <= last; ++c)
-                if (f.used[c]) M = fmaxf(M, f.m[c][hh]);
-            float L = 0.0f, O = 0.0f;
-            for (int c = c0; c <= last; ++c)
-                if (f.used[c]) {
-                    const float e = exp2_fast(f.m[c][hh] - M);
-                    L = fmaf(f.l[c][hh], e, L);
-                    O = fmaf(value(c, hh, b * 32 + lane), e, O);
-                }
+            for (unsigned m = mine; m != 0; m &= m - 1) M = fmaxf(M, f.m[__ffs(m) - 1][hh]);
+            float L = 0.0f;
+            float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (unsigned m = mine; m != 0; m &= m - 1) {
+                const int c = __ffs(m) - 1;
+                const float e = exp2_fast(f.m[c][hh] - M);
+                L = fmaf(f.l[c][hh], e, L);
+                add_scaled(O, quad(c, x), e);
+            }
             if (done) {
-                write_block<NB>(a, s.req, s.head0 + hh, b, lane, O, L);
-            } else {
-                const size_t at = (size_t)(blockIdx.x * 2 + side) * kSegHeads + hh;
-                a.part_out[at * D + b * 32 + lane] = O;
-                if (b == 0 && lane == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(M, L);
+                write_quad<NB>(a, s, x, x0 + lane < quads, O, L);
+            } else if (x0 + lane < quads) {
+                reinterpret_cast<float4*>(a.part_out + at * D)[x] = O;
+                if (x % (D / 4) == 0) *reinterpret_cast<float2*>(a.part_ml + (at + hh) * 2) = make_float2(M, L);
             }
         }
-        c0 = c1;
     }
 #pragma unroll 1
     for (int side = 0; side < 2; ++side) {
