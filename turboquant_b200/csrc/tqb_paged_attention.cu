@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kWorkThreads) paged_simple_kernel(const __grid
             __syncwarp();
         }
     }
-    finish<NB>(a, s_frag, [&](int c, int x) { return reinterpret_cast<const float4*>(s_o + c * kSegHeads * D)[x]; });
+    finish<NB>(a, s_frag, s_o, [&](int c, int x) { return reinterpret_cast<const float4*>(s_o + c * kSegHeads * D)[x]; });
     write_empty<NB>(a);
 }
 

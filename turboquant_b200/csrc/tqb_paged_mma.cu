@@ -20,7 +20,7 @@
 //   is taken off by starting each accumulation at -7.5 sum P', itself an MMA with constant rows.  Accumulators live for
 //   32 tokens and are then added to the running output in rounded f32 additions; one long chain would add up the truncation
 //   of the MMA's adder relative to 7.5 sum P'.
-//   Products beyond f16 (|s_v| above 16) show as a non-finite output: the segment is then done again with smaller p.
+//   Where some |s_v| is above 32, so that a product could leave f16, the warp lowers kShift by as much.
 #include "tqb_common.cuh"
 #include "tqb_mma.cuh"
 #include "tqb_paged.cuh"
@@ -35,7 +35,8 @@ constexpr int kGroupTokens = 16;
 constexpr int kRing = 4;     // stages of a warp
 constexpr int kStepGroups = 2;
 constexpr int kInFlight = kRing - kStepGroups;
-constexpr float kShift = 8.0f, kLazy = 4.0f;
+constexpr float kShift = 6.0f, kLazy = 4.0f;
+constexpr uint32_t kScaleTop = 0x50005000u;   // 2^(15 - kShift - kLazy) = 32, twice
 constexpr float kQMax = 32639.0f;   // 127 * 256 + 127
 
 template <int BYTES>
@@ -73,10 +74,11 @@ struct Plan {
     static constexpr int kSets = HG == 4 ? 1 : 2;                 // MMAs of a block's scores
     static constexpr int kFragment = HG * NB * 32 * 4;            // outputs of a segment
     static constexpr int kDigits = kSets * NB * 32 * 8;           // the queries' MMA fragments
-    static constexpr int kWarpBytes = G::kWarpRing + kFragment + kDigits;   // [ring][fragment that began before][digits]
+    static constexpr int kQueries = HG * NB * 32 * 2;             // the next segment's queries as they are
+    static constexpr int kWarpBytes = G::kWarpRing + kFragment + kDigits + kQueries;   // [ring][fragment that began before][digits][queries]
     static constexpr int kBytes = kWorkWarps * kWarpBytes;
     // CTAs of an SM: by shared memory, and so that registers do not spill
-    static constexpr int kByShared = 227 * 1024 / (kBytes + 4096), kByRegs = NB == 8 ? (HG == 8 ? 2 : 3) : HG == 8 ? 4 : NB == 2 ? 5 : 4;
+    static constexpr int kByShared = 228 * 1024 / (kBytes + 1024 + 2560), kByRegs = NB == 8 ? (HG == 8 ? 2 : 3) : HG == 8 ? 4 : NB == 2 ? 5 : 4;
     static constexpr int kCtas = kByShared < kByRegs ? kByShared : kByRegs;
 };
 
@@ -88,6 +90,7 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
     constexpr int kO = HG == 4 ? 2 : 4;               // outputs that a lane holds of an MMA tile
     extern __shared__ __align__(128) unsigned char s_dyn[];
     __shared__ Fragments s_frag;
+    __shared__ Segment s_next[kWorkWarps];
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, j = lane & 3;
     const float step = 2.0f * a.cent[15] / 15.0f;
@@ -96,8 +99,10 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
     unsigned char* const s_digits = s_warp + G::kWarpRing + L::kFragment;
     const uint32_t digits = (uint32_t)__cvta_generic_to_shared(s_digits) + lane * 8;
     const uint32_t halves = 2 * ring + kInFlight * G::kStage;   // (one half's address) + (the other's)
+    unsigned char* const s_queries = s_digits + L::kDigits;
+    const uint32_t queries = (uint32_t)__cvta_generic_to_shared(s_queries);
     static_assert(kRing == 2 * kInFlight && kStepGroups == kInFlight, "the ring has two halves of a step each");
-    static_assert(L::kFragment <= G::kWarpRing, "a segment's outputs do not fit into the ring");
+    static_assert(L::kFragment <= kInFlight * G::kStage && kJoinSpace * 4 <= G::kWarpRing, "a segment's outputs do not fit into half a ring");
     // a fragment's outputs [HG][D]: that of the warp's last segment lies in its idle ring
     auto fragment = [&](int slot) { return reinterpret_cast<float*>(s_dyn + (slot >> 1) * L::kWarpBytes + ((slot & 1) ? 0 : G::kWarpRing)); };
     // ldmatrix: lane l gives the row address of token 8 ((l >> 3) & 1) + (l & 7), block 2 pair + (l >> 4)
@@ -112,35 +117,52 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
     if (threadIdx.x < 2 * kWorkWarps) s_frag.used[threadIdx.x] = 0;
     WorkLine line(a);   // (its barriers stand before the first use of what is set above)
 
-    // ---- copies of a segment's groups, one behind the other ----
+    // ---- copies: segment after segment without a break, a step ahead of the products ----
     Segment s{};
-    int to_copy;                              // first token of the group that is copied next
-    int page_now, page_next;                  // pages 32 k + lane of the segment, for this k and the next
-    bool some_bad = false;                    // some page does not exist (of those looked at so far)
-    const uint8_t *kp, *vp;
-    const uint16_t* sp;
-    auto page_at = [&](int i) {               // of the segment's i-th page
-        const int page = a.table[s.req * a.table_stride + min((s.t0 >> a.page_shift) + i, (s.t1 - 1) >> a.page_shift)];
+    bool more = line.next(s);
+    int to_copy = s.t0, copy_end = s.t1;      // of the segment whose copies are being made
+    int page_now = 0, page_next = 0, page0 = 0;   // pages page0 + 32 k + lane of it, for this k and the next
+    const int32_t* table = a.table;
+    uint32_t head = 0;
+    bool fresh = true;                        // its first group is still to come
+    bool bad_copy = false;                    // some page of it does not exist (of those looked at so far)
+    const uint8_t *kp = a.kb, *vp = a.vb;
+    const uint16_t* sp = a.ks;
+    auto page_at = [&](int i) {
+        const int page = table[min(page0 + i, (copy_end - 1) >> a.page_shift)];
         const bool bad = (unsigned)page >= (unsigned)a.num_pages;
-        some_bad |= __any_sync(0xffffffffu, bad) != 0;
+        bad_copy |= __any_sync(0xffffffffu, bad) != 0;
         return bad ? 0 : page;
     };
-    auto open = [&]() {
-        some_bad = false;
-        to_copy = s.t0;
+    auto open = [&](const Segment& x) {
+        to_copy = x.t0;
+        copy_end = x.t1;
+        page0 = x.t0 >> a.page_shift;
+        table = a.table + (size_t)x.req * a.table_stride;
+        head = (uint32_t)x.kvh << a.page_shift;
+        bad_copy = false;
+        fresh = true;
+        // the queries ride along with the first group
+        const uint8_t* q = reinterpret_cast<const uint8_t*>(a.q) + ((size_t)x.req * a.q_stride + (size_t)x.head0 * D) * 2;
+#pragma unroll
+        for (int i = 0; i < (L::kQueries / 16 + 31) / 32; ++i) {
+            const int piece = 32 * i + lane;
+            if (piece < x.heads * NB * 4) cp_async16(queries + piece * 16, q + piece * 16);
+        }
         page_now = page_at(lane);
-        page_next = (s.t1 - 1) >> a.page_shift >= (s.t0 >> a.page_shift) + 32 ? page_at(32 + lane) : 0;
+        page_next = (copy_end - 1) >> a.page_shift >= page0 + 32 ? page_at(32 + lane) : 0;
     };
     auto fill = [&](uint32_t st) {
-        if (to_copy < s.t1) {
-            if ((to_copy & mask) == 0 || to_copy == s.t0) {
-                const int i = (to_copy >> a.page_shift) - (s.t0 >> a.page_shift);
+        if (to_copy < copy_end) {
+            const int i = (to_copy >> a.page_shift) - page0;
+            if ((to_copy & mask) == 0 || fresh) {
+                fresh = false;
                 if (i > 0 && (i & 31) == 0) {
                     page_now = page_next;
                     page_next = page_at(i + 32 + lane);
                 }
                 const int page = __shfl_sync(0xffffffffu, page_now, i & 31);
-                const uint32_t row = (((uint32_t)page * a.hkv + s.kvh) << a.page_shift) + (to_copy & mask);
+                const uint32_t row = (((uint32_t)page * a.hkv) << a.page_shift) + head + (to_copy & mask);
                 kp = a.kb + (size_t)row * G::kRow + lane * 16;
                 vp = a.vb + (size_t)row * G::kRow + lane * 16;
                 sp = (lane < 16 ? a.ks : a.vs) + (size_t)(row + (lane & 15)) * NB;
@@ -161,67 +183,69 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
         to_copy += kGroupTokens;
     };
 
-    while (line.next(s)) {
+    if (more) {
+        open(s);
+#pragma unroll
+        for (int u = 0; u < kStepGroups; ++u) fill(ring + u * G::kStage);
+    }
+    uint32_t st = ring;
+    while (more) {
+        // ---- the next segment; copies go over to it by themselves ----
+        bool bad = bad_copy;                  // of this segment
+        Segment next{};
+        more = line.next(next);
+        __syncwarp();                         // (s_next has been read)
+        if (lane == 0) s_next[warp] = next;
+        bool ahead = false;                   // copies have gone over
+        cp_async_wait<kInFlight - 1>();       // the first group, and the queries
+        __syncwarp();
         // ---- queries: rotated, scaled to integers, cut into digits ----
         float qsc[kE];
         {
-            constexpr int kAtOnce = HG * NB <= 32 ? HG : 4;   // heads
             const float inv_sqrt = 1.0f / sqrtf((float)kBlock), sg = block_sign(lane, a.sign_mag);
-            const size_t q0 = (size_t)s.req * a.q_stride + (size_t)s.head0 * D + lane;
 #pragma unroll
             for (int e = 0; e < kE; ++e) qsc[e] = 0.0f;
             // Byte i of k-slots 4j' + i of fragment (b, 4n' + j') is dim 32 b + 8 j' + 2 i (first word) or one above it (second), of
             // column n': this lane's dim has j' = lane / 8, i = lane / 2 % 4, word lane % 2
             unsigned char* const at = s_digits + (lane >> 3) * 8 + (lane & 1) * 4 + ((lane >> 1) & 3);
 #pragma unroll
-            for (int h0 = 0; h0 < HG; h0 += kAtOnce) {
-                float v[kAtOnce][NB];
+            for (int h = 0; h < HG; ++h) {
+                float v[NB];
+                uint32_t top = 0;   // of the bits, so that NaN is above infinity
 #pragma unroll
-                for (int i = 0; i < kAtOnce; ++i)
+                for (int b = 0; b < NB; ++b) {
+                    v[b] = h < s.heads ? load_as_f32(s_queries, a.q_dtype, h * D + b * 32 + lane) : 0.0f;
+                    v[b] = wht32_across(v[b], lane) * inv_sqrt * sg;
+                    top = max(top, __float_as_uint(v[b]) & 0x7fffffffu);
+                }
+                float m = __uint_as_float(__reduce_max_sync(0xffffffffu, top));
+                if (!(m <= FLT_MAX)) m = __uint_as_float(0x7fc00000u);   // not finite: every score is NaN
+                const float inv = m > 0.0f ? kQMax / m : 0.0f;
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) v[i][b] = h0 + i < s.heads ? load_as_f32(a.q, a.q_dtype, q0 + (h0 + i) * D + b * 32) : 0.0f;
-                if (h0 == 0) {   // (behind the queries' loads)
-                    open();
-#pragma unroll
-                    for (int i = 0; i < kInFlight; ++i) fill(ring + i * G::kStage);
+                for (int b = 0; b < NB; ++b) {
+                    // (inv is infinite where the largest component is below 1e-34)
+                    const int x = inv <= FLT_MAX ? __float2int_rn(v[b] * inv) : 0;
+                    const int lo = (int)(signed char)(x & 0xff), hi = (x - lo) >> 8;
+                    if (HG == 4) {
+                        at[b * 256 + (2 * h) * 32] = (unsigned char)hi;
+                        at[b * 256 + (2 * h + 1) * 32] = (unsigned char)lo;
+                    } else {
+                        at[b * 256 + h * 32] = (unsigned char)hi;
+                        at[(NB + b) * 256 + h * 32] = (unsigned char)lo;
+                    }
                 }
 #pragma unroll
-                for (int i = 0; i < kAtOnce; ++i) {
-                    const int h = h0 + i;
-                    uint32_t top = 0;   // of the bits, so that NaN is above infinity
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        v[i][b] = wht32_across(v[i][b], lane) * inv_sqrt * sg;
-                        top = max(top, __float_as_uint(v[i][b]) & 0x7fffffffu);
-                    }
-                    float m = __uint_as_float(__reduce_max_sync(0xffffffffu, top));
-                    if (!(m <= FLT_MAX)) m = __uint_as_float(0x7fc00000u);   // not finite: every score is NaN
-                    const float inv = m > 0.0f ? kQMax / m : 0.0f;
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        // (inv is infinite where the largest component is below 1e-34)
-                        const int x = inv <= FLT_MAX ? __float2int_rn(v[i][b] * inv) : 0;
-                        const int lo = (int)(signed char)(x & 0xff), hi = (x - lo) >> 8;
-                        if (HG == 4) {
-                            at[b * 256 + (2 * h) * 32] = (unsigned char)hi;
-                            at[b * 256 + (2 * h + 1) * 32] = (unsigned char)lo;
-                        } else {
-                            at[b * 256 + h * 32] = (unsigned char)hi;
-                            at[(NB + b) * 256 + h * 32] = (unsigned char)lo;
-                        }
-                    }
-#pragma unroll
-                    for (int e = 0; e < kE; ++e)
-                        if (h == (HG == 4 ? j : 2 * j + e)) qsc[e] = m * (a.qk_const * step / (kQMax * 16.0f));
-                }
+                for (int e = 0; e < kE; ++e)
+                    if (h == (HG == 4 ? j : 2 * j + e)) qsc[e] = m * (a.qk_const * step / (kQMax * 16.0f));
             }
             __syncwarp();
         }
 
         float shift = kShift;
+        uint32_t sv_limit = kScaleTop;
         float m_ref[kE], l_run[kE];
         float o[NB][2][kO];
-        for (;;) {
+        {
 #pragma unroll
             for (int e = 0; e < kE; ++e) {
                 m_ref[e] = kNoScore;
@@ -233,9 +257,13 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
                 for (int m = 0; m < 2; ++m)
 #pragma unroll
                     for (int i = 0; i < kO; ++i) o[b][m][i] = 0.0f;
-            uint32_t st = ring;
             for (int t0 = s.t0; t0 < s.t1; t0 += kStepGroups * kGroupTokens) {
                 const uint32_t st_other = halves - st;
+                if (to_copy >= copy_end && more && !ahead) {   // this segment's copies are under way: the next one's
+                    bad |= bad_copy;
+                    ahead = true;
+                    open(s_next[warp]);
+                }
 #pragma unroll
                 for (int u = 0; u < kStepGroups; ++u) fill(st_other + u * G::kStage);
                 cp_async_wait<kInFlight>();
@@ -297,11 +325,12 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
                         out[u][t] = false;
                         sv_mask[u][t] = 0x7fff7fffu;
                     }
-                if (some_bad || t0 + kStepGroups * kGroupTokens > s.t1) {
+                if (!ahead) bad |= bad_copy;
+                if (bad || t0 + kStepGroups * kGroupTokens > s.t1) {
 #pragma unroll
                     for (int u = 0; u < kStepGroups; ++u) {
                         const int gs = t0 + u * kGroupTokens;
-                        const bool none = some_bad && (unsigned)a.table[s.req * a.table_stride + (min(gs, s.t1 - 1) >> a.page_shift)] >= (unsigned)a.num_pages;
+                        const bool none = bad && (unsigned)a.table[s.req * a.table_stride + (min(gs, s.t1 - 1) >> a.page_shift)] >= (unsigned)a.num_pages;
 #pragma unroll
                         for (int t = 0; t < 2; ++t)
                             if (none || gs + n + 8 * t >= s.t1) {
@@ -310,9 +339,22 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
                             }
                     }
                 }
+                // ---- scales of V, and the largest of them ----
+                uint32_t sv[kStepGroups][2][kPairs], sv_top = 0u;
+                static_for<0, kStepGroups>([&](auto u_) {
+                    constexpr int u = decltype(u_)::value;
+                    static_for<0, 2>([&](auto t_) {
+                        constexpr int t = decltype(t_)::value;
+                        static_for<0, kPairs>([&](auto p_) {
+                            constexpr int pr = decltype(p_)::value;
+                            sv[u][t][pr] = lds32_o<16 * G::kSc + 8 * t * G::kSc + 4 * pr>(st + u * G::kStage + off_s) & sv_mask[u][t];
+                            sv_top = h2_as_u32(__hmax2(u32_as_h2(sv_top), u32_as_h2(sv[u][t][pr])));
+                        });
+                    });
+                });
                 // ---- softmax ----
                 float x[kStepGroups][2][kE];
-                bool over = false;
+                bool over = ((sv_limit - sv_top) & 0x80008000u) != 0u;   // some half of sv_top is larger (a borrow is one itself)
 #pragma unroll
                 for (int e = 0; e < kE; ++e) {
                     float top = -INFINITY;
@@ -326,6 +368,14 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
                     over |= top > shift + kLazy;
                 }
                 if (__any_sync(0xffffffffu, over)) {
+                    const uint32_t largest = __reduce_max_sync(0xffffffffu, max(sv_top & 0xffffu, sv_top >> 16));
+                    float less = 0.0f;
+                    if (largest > (sv_limit & 0xffffu)) {   // (f16 bits, positive: they compare like numbers)
+                        const uint32_t above = min((largest - (sv_limit & 0xffffu) + 1023u) >> 10, (0x7c00u - (sv_limit & 0xffffu)) >> 10);
+                        less = (float)above;                // powers of two
+                        shift -= less;
+                        sv_limit += above * 0x04000400u;
+                    }
 #pragma unroll
                     for (int e = 0; e < kE; ++e) {
                         float mx = -INFINITY;
@@ -337,7 +387,7 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                        const float m_new = fmaxf(m_ref[e], mx - shift), keep = ex2(m_ref[e] - m_new);
+                        const float m_new = fmaxf(m_ref[e] + less, mx - shift), keep = ex2(m_ref[e] - m_new);
                         m_ref[e] = m_new;
                         l_run[e] *= keep;
 #pragma unroll
@@ -357,7 +407,6 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
                 uint32_t pq[kStepGroups][HG == 4 ? kPairs : NB][2];   // [octet]
                 static_for<0, kStepGroups>([&](auto u_) {
                     constexpr int u = decltype(u_)::value;
-                    const uint32_t stu = st + u * G::kStage;
                     static_for<0, 2>([&](auto t_) {
                         constexpr int t = decltype(t_)::value;
                         float p[kE];
@@ -369,12 +418,12 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
                         const uint32_t ph = h2_as_u32(__floats2half2_rn(p[0], p[kE - 1]));
                         static_for<0, kPairs>([&](auto p_) {
                             constexpr int pr = decltype(p_)::value;
-                            const uint32_t sv = lds32_o<16 * G::kSc + 8 * t * G::kSc + 4 * pr>(stu + off_s) & sv_mask[u][t];
+                            const uint32_t w = sv[u][t][pr];
                             if constexpr (HG == 4) {   // columns 2j, 2j + 1: head j with the scales of blocks 2 pr, 2 pr + 1
-                                pq[u][pr][t] = movmatrix_trans(product(ph, sv));
+                                pq[u][pr][t] = movmatrix_trans(product(ph, w));
                             } else {                   // columns 2j, 2j + 1: heads 2j, 2j + 1
-                                pq[u][2 * pr][t] = movmatrix_trans(product(ph, __byte_perm(sv, sv, 0x1010)));
-                                pq[u][2 * pr + 1][t] = movmatrix_trans(product(ph, __byte_perm(sv, sv, 0x3232)));
+                                pq[u][2 * pr][t] = movmatrix_trans(product(ph, __byte_perm(w, w, 0x1010)));
+                                pq[u][2 * pr + 1][t] = movmatrix_trans(product(ph, __byte_perm(w, w, 0x3232)));
                             }
                         });
                     });
@@ -416,26 +465,14 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
                 __syncwarp();   // the stages may be filled again
                 st = st_other;
             }
-            cp_async_wait<0>();
-            __syncwarp();
-            bool finite = true;
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int i = 0; i < kO; ++i) finite = finite && fabsf(o[b][m][i]) <= FLT_MAX;
-            if (__all_sync(0xffffffffu, finite) || shift < 0.0f) break;
-            shift -= 6.0f;   // 8, 2, -4: with the last, p |s_v| is at most 65504
-            open();
-#pragma unroll
-            for (int i = 0; i < kInFlight; ++i) fill(ring + i * G::kStage);
         }
 
         // ---- the segment's end ----
+        // A whole segment's outputs pass through the half of the ring that holds nothing yet: the copies in flight are in `st`.
         const bool whole = s.whole();
         const int slot = 2 * warp + (s.begins ? 1 : 0);
-        float* const to = fragment(slot);
+        float* const to = whole ? reinterpret_cast<float*>(s_warp + (halves - st - ring)) : fragment(slot);
+        if (!whole && s.begins) cp_async_wait<0>();   // the warp's last segment: its ring is idle
         const float even = step * 8388608.0f, odd = step * 524288.0f;   // 2^23, 2^19
 #pragma unroll
         for (int b = 0; b < NB; ++b)
@@ -471,8 +508,9 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
             }
             __syncwarp();
         }
+        s = s_next[warp];
     }
-    finish<NB>(a, s_frag, [&](int c, int x) { return reinterpret_cast<const float4*>(fragment(c))[x]; });
+    finish<NB>(a, s_frag, reinterpret_cast<float*>(s_dyn), [&](int c, int x) { return reinterpret_cast<const float4*>(fragment(c))[x]; });
     write_empty<NB>(a);
 }
 

@@ -253,30 +253,38 @@ __device__ __forceinline__ void add_scaled(float4& acc, float4 v, float w) {
 __device__ __forceinline__ int parts_per_round(int parts) { return parts <= 16 ? parts : parts <= 64 ? 8 : parts <= 256 ? 16 : kMaxRound; }
 static_assert(kMaxRound * kMaxRound >= kMaxCtas, "two rounds are enough");
 
-// One arrival at a ticket of `want`, after everything that the CTA's threads have written; true for the last one, whose
-// threads then see what the others have written.
-__device__ __forceinline__ bool last_arrival(unsigned* ticket, int want) {
-    __shared__ int s_last;
+// Arrivals at up to two tickets (nullptr: none) of `want` each, after everything that the CTA's threads have written; bit i:
+// this CTA is the last at ticket i, and its threads see what the others have written.
+__device__ __forceinline__ int arrive(unsigned* ticket0, int want0, unsigned* ticket1, int want1) {
+    __shared__ int s_last[2];
     __syncthreads();
-    if (threadIdx.x == 0) {
-        unsigned old;
-        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;\n" : "=r"(old) : "l"(ticket) : "memory");
-        s_last = old == (unsigned)(want - 1);
-        if (s_last) *ticket = 0u;   // ready for the next call
+    if ((threadIdx.x & 31) == 0 && threadIdx.x < 64) {   // a warp each: the fences and the round trips overlap
+        unsigned* ticket = threadIdx.x == 0 ? ticket0 : ticket1;
+        const int want = threadIdx.x == 0 ? want0 : want1;
+        int last = 0;
+        if (ticket != nullptr) {
+            unsigned old;
+            asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;\n" : "=r"(old) : "l"(ticket) : "memory");
+            last = old == (unsigned)(want - 1);
+            if (last) *ticket = 0u;   // ready for the next call
+        }
+        s_last[threadIdx.x >> 5] = last;
     }
     __syncthreads();
-    return s_last != 0;
+    return s_last[0] | (s_last[1] << 1);
 }
 
 // Where part i of a (request, head) lies: of the first CTA the second slot, of the others the first.
 __device__ __forceinline__ size_t part_at(int cta0, int i) { return (size_t)((cta0 + i) * 2 + (i == 0 ? 1 : 0)) * kSegHeads; }
 
 // Joins parts i0, i0 + stride, .. (`count` <= kMaxRound of them) of a (request, head): into the output, or into the place
-// of part i0.
+// of part i0.  space: kJoinSpace floats of shared memory.
+constexpr int kJoinSpace = kSegHeads * (kMaxRound + 1);
 template <int NB>
-__device__ __forceinline__ void join_parts(const PagedArgs& a, const Segment& s, int i0, int stride, int count, bool to_out) {
+__device__ __noinline__ void join_parts(const PagedArgs& a, const Segment& s, int i0, int stride, int count, bool to_out, float* space) {
     constexpr int D = NB * 32, kAtOnce = 8;
-    __shared__ float s_w[kSegHeads][kMaxRound], s_L[kSegHeads];
+    float (*s_w)[kMaxRound] = reinterpret_cast<float (*)[kMaxRound]>(space);   // [kSegHeads]
+    float* s_L = space + kSegHeads * kMaxRound;                                // [kSegHeads]
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int hh = warp; hh < s.heads; hh += kWorkWarps) {
         float2 ml[(kMaxRound + 31) / 32];
@@ -334,9 +342,10 @@ struct Fragments {
     int used[2 * kWorkWarps];
 };
 
-// The CTA's end, by all of its threads: quad(slot, x) are four of a fragment's un-normalised rotated outputs.
+// The CTA's end, by all of its threads: quad(slot, x) are four of a fragment's un-normalised rotated outputs.  join_space:
+// shared memory for join_parts, which may be that of the fragments.
 template <int NB, typename F>
-__device__ __forceinline__ void finish(const PagedArgs& a, const Fragments& f, F quad) {
+__device__ __forceinline__ void finish(const PagedArgs& a, const Fragments& f, float* join_space, F quad) {
     constexpr int D = NB * 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     __syncthreads();
@@ -376,19 +385,47 @@ __device__ __forceinline__ void finish(const PagedArgs& a, const Fragments& f, F
             }
         }
     }
-#pragma unroll 1
+    // what crosses the CTA's ends: a first round of parts, if there are many, and the last one
+    unsigned* ticket[2];
+    int want[2], first[2], per[2];
+#pragma unroll
     for (int side = 0; side < 2; ++side) {
-        if (crossing[side] < 0) continue;
-        const Segment& s = f.seg[crossing[side]];
-        const int per = parts_per_round(s.ctas);
-        int rounds = s.ctas;
-        if (per < s.ctas) {
-            const int mine = (int)blockIdx.x - s.cta0, i0 = mine / per * per, count = min(per, s.ctas - i0);
-            rounds = (s.ctas + per - 1) / per;
-            if (!last_arrival(a.tickets + kMaxCtas + (s.cta0 + i0) * 2 + (i0 == 0 ? 1 : 0), count)) continue;
-            join_parts<NB>(a, s, i0, 1, count, false);
+        ticket[side] = nullptr;
+        want[side] = first[side] = per[side] = 0;
+        if (crossing[side] >= 0) {
+            const Segment& s = f.seg[crossing[side]];
+            per[side] = parts_per_round(s.ctas);
+            if (per[side] < s.ctas) {
+                const int mine = (int)blockIdx.x - s.cta0;
+                first[side] = mine / per[side] * per[side];
+                want[side] = min(per[side], s.ctas - first[side]);
+                ticket[side] = a.tickets + kMaxCtas + (s.cta0 + first[side]) * 2 + (first[side] == 0 ? 1 : 0);
+            } else {
+                want[side] = s.ctas;
+                ticket[side] = a.tickets + s.cta0;
+            }
         }
-        if (last_arrival(a.tickets + s.cta0, rounds)) join_parts<NB>(a, s, 0, per < s.ctas ? per : 1, rounds, true);
+    }
+    if (crossing[0] < 0 && crossing[1] < 0) return;
+#pragma unroll 1
+    for (int round = 0; round < 2; ++round) {
+        const int won = arrive(ticket[0], want[0], ticket[1], want[1]);
+        bool again = false;
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            ticket[side] = nullptr;
+            if (!((won >> side) & 1)) continue;
+            const Segment& s = f.seg[crossing[side]];
+            const bool two = per[side] < s.ctas, last = !two || round == 1;
+            if (last) join_parts<NB>(a, s, 0, two ? per[side] : 1, two ? (s.ctas + per[side] - 1) / per[side] : s.ctas, true, join_space);
+            else {
+                join_parts<NB>(a, s, first[side], 1, want[side], false, join_space);
+                ticket[side] = a.tickets + s.cta0;
+                want[side] = (s.ctas + per[side] - 1) / per[side];
+                again = true;
+            }
+        }
+        if (!again) break;
     }
 }
 
