@@ -1388,6 +1388,24 @@ bool stream_captured(cudaStream_t s) {
 
 }  // namespace
 
+// The eight centroids of a 3-bit cache as values of f16 times kappa (see best_kappa), computed once for each codebook.
+bool pqo3_values(int norm_mode, bool all_outlier, float& kappa, float (&values)[8]) {
+    std::lock_guard<std::mutex> lock(g_lut_mutex);
+    LutCache& lc = g_lut_cache[norm_mode == TQB_L2NORM ? 1 : 0][all_outlier ? 1 : 0];
+    if (!lc.valid) {
+        Codebook cb;
+        if (!block_codebook(all_outlier ? 3 : 2, norm_mode, cb)) return false;
+        float c[8];
+        for (int i = 0; i < 8; ++i) c[i] = cb.c[i < cb.n ? i : cb.n - 1];   // codes past a 4-entry book clamp (quantize_tensor.rs:245)
+        lc.kappa = best_kappa(c, 8);
+        for (int i = 0; i < 8; ++i) lc.lut[i] = c[i] / lc.kappa;
+        lc.valid = true;
+    }
+    kappa = lc.kappa;
+    for (int i = 0; i < 8; ++i) values[i] = lc.lut[i];
+    return true;
+}
+
 // Returns TQB_ERR_UNSUPPORTED when the shape is outside what the tensor-core kernels cover;
 // the caller then uses the general kernel.
 // `counters` != nullptr fuses the merge into the kernel: [num_kv_heads] tickets, zeroed here unless the
@@ -1481,22 +1499,10 @@ int launch_decode_mma(const tqb_decode_params* p, int num_partitions, float* par
         a.v_const = grid_step;
         return launch<4>(a, g, p->q_dtype, allow_tma, app_cb, grid, early, s);
     }
-    {
-        std::lock_guard<std::mutex> lock(g_lut_mutex);
-        LutCache& lc = g_lut_cache[p->norm_mode == TQB_L2NORM ? 1 : 0][all_outlier ? 1 : 0];
-        if (!lc.valid) {
-            Codebook cb;
-            if (!block_codebook(all_outlier ? 3 : 2, p->norm_mode, cb)) return TQB_ERR_UNSUPPORTED;
-            float c[8];
-            for (int i = 0; i < 8; ++i) c[i] = cb.c[i < cb.n ? i : cb.n - 1];   // codes past a 4-entry book clamp (quantize_tensor.rs:245)
-            lc.kappa = best_kappa(c, 8);
-            for (int i = 0; i < 8; ++i) lc.lut[i] = c[i] / lc.kappa;
-            lc.valid = true;
-        }
-        a.qk_const = p->softmax_scale * log2e * lc.kappa;
-        a.v_const = lc.kappa;
-        for (int i = 0; i < 8; ++i) a.lut[i] = lc.lut[i];
-    }
+    float kappa;
+    if (!pqo3_values(p->norm_mode, all_outlier, kappa, a.lut)) return TQB_ERR_UNSUPPORTED;
+    a.qk_const = p->softmax_scale * log2e * kappa;
+    a.v_const = kappa;
     return launch<3>(a, g, p->q_dtype, allow_tma, app_cb, grid, early, s);
 }
 

@@ -36,6 +36,7 @@ int check_launch(cudaStream_t s);
 
 bool whole_codebook(int bits, int dim, Codebook& cb);              // core-crate tables
 bool block_codebook(int cb_bits, int norm_mode, Codebook& cb);     // cache-module tables
+bool pqo3_values(int norm_mode, bool all_outlier, float& kappa, float (&values)[8]);   // the 3-bit centroids as f16 values times kappa
 extern const float kBlockSigns[32];
 
 __device__ __forceinline__ float f16_bits_to_f32(uint16_t u) { return __half2float(__ushort_as_half(u)); }

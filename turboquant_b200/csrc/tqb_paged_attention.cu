@@ -174,7 +174,7 @@ int tqb_paged_attention(const tqb_paged_layer* layer, const tqb_paged_attention_
     a.sign_mag = block_sign_magnitude();
     for (int i = 0; i < 16; ++i) a.cent[i] = cb.c[i];
     cudaStream_t s = as_stream(stream);
-    if (layer->bits == 4 && p->q_dtype != TQB_F32 && layer->num_pages > 0) return launch_paged_mma(a, layer->head_dim, s);
+    if (p->q_dtype != TQB_F32 && layer->num_pages > 0) return launch_paged_mma(a, layer->head_dim, layer->bits, s);
     switch (layer->head_dim * 10 + layer->bits) {
         case 643: return launch_simple<2, 3>(a, s);
         case 644: return launch_simple<2, 4>(a, s);

@@ -52,40 +52,50 @@ __device__ __forceinline__ void codes_to_subnormals(uint32_t w, uint32_t (&x)[4]
     x[2] = w7 & 0x001e001eu;
     x[3] = w7 & 0x01e001e0u;
 }
+// Eight 3-bit codes (24 bits; what is above them does not matter) -> a nibble each, the top bit clear.
+__device__ __forceinline__ uint32_t nibbles_of_codes(uint32_t w) {
+    const uint32_t a = bit_select(w, w << 4, 0x00000fffu);
+    const uint32_t b = bit_select(a, a << 2, 0x003f003fu);
+    return bit_select(b, b << 1, 0x07070707u) & 0x77777777u;
+}
 constexpr uint32_t kCentreEven = 0x800f800fu;   // -7.5 2^-23 as a subnormal f16, twice
 constexpr uint32_t kCentreOdd = 0x80f080f0u;    // -7.5 2^-19
 
 __device__ __forceinline__ uint32_t product(uint32_t a, uint32_t b) { return h2_as_u32(__hmul2(u32_as_h2(a), u32_as_h2(b))); }
 
-template <int NB>
+template <int NB, int HG, int BITS>
 struct Shape {
-    static constexpr int kRow = 16 * NB;                // bytes of a token's codes
+    static constexpr int kRow = 4 * BITS * NB;          // bytes of a token's codes
     static constexpr int kIdx = kGroupTokens * kRow;    // of a stage's K (or V) codes
     static constexpr int kSc = 2 * NB;                  // of a token's scales
-    static constexpr int kStage = 2 * kIdx + 2 * kGroupTokens * kSc;   // [K codes][V codes][K scales][V scales]
+    static constexpr int kOut = HG * NB * 32 * 4;       // of a segment's outputs: they must fit into half a ring
+    static constexpr int kUsed = 2 * kIdx + 2 * kGroupTokens * kSc;   // [K codes][V codes][K scales][V scales]
+    static constexpr int kStage = kUsed > kOut / kInFlight ? kUsed : kOut / kInFlight;
     static constexpr int kWarpRing = kRing * kStage;      // of a warp
-    // 16-byte piece c of token row t lies at piece c ^ swizzle(t): the eight rows of an ldmatrix hit different banks
+    static constexpr int kCopies = (kIdx / 16 + 31) / 32;   // 16-byte pieces of K (or V) codes that a lane copies, at most
+    // 4-bit: 16-byte piece c of token row t lies at piece c ^ swizzle(t), so that the eight rows of an ldmatrix hit different
+    // banks.  3-bit rows lie densely: their 6, 12 or 24 words spread over the banks by themselves.
     __device__ static __forceinline__ int swizzle(int t) { return NB == 2 ? (t >> 2) & 1 : NB == 4 ? (t >> 1) & 3 : t & 7; }
 };
 
-template <int NB, int HG>
+template <int NB, int HG, int BITS>
 struct Plan {
-    using G = Shape<NB>;
-    static constexpr int kSets = HG == 4 ? 1 : 2;                 // MMAs of a block's scores
-    static constexpr int kFragment = HG * NB * 32 * 4;            // outputs of a segment
+    using G = Shape<NB, HG, BITS>;
+    static constexpr int kSets = HG == 4 && BITS == 4 ? 1 : 2;    // sets of digits (3-bit: see the scores)
+    static constexpr int kFragment = G::kOut;
     static constexpr int kDigits = kSets * NB * 32 * 8;           // the queries' MMA fragments
     static constexpr int kQueries = HG * NB * 32 * 2;             // the next segment's queries as they are
     static constexpr int kWarpBytes = G::kWarpRing + kFragment + kDigits + kQueries;   // [ring][fragment that began before][digits][queries]
     static constexpr int kBytes = kWorkWarps * kWarpBytes;
     // CTAs of an SM: by shared memory, and so that registers do not spill
-    static constexpr int kByShared = 228 * 1024 / (kBytes + 1024 + 2560), kByRegs = NB == 8 ? (HG == 8 ? 2 : 3) : HG == 8 ? 4 : NB == 2 ? 5 : 4;
+    static constexpr int kByShared = 228 * 1024 / (kBytes + 1024 + 2560 + (BITS == 3 ? 8192 : 0)), kByRegs = NB == 8 ? (HG == 8 ? 2 : 3) : HG == 8 ? 4 : NB == 2 ? 5 : 4;
     static constexpr int kCtas = kByShared < kByRegs ? kByShared : kByRegs;
 };
 
-template <int NB, int HG>
-__global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_kernel(const __grid_constant__ PagedArgs a) {
-    using G = Shape<NB>;
-    using L = Plan<NB, HG>;
+template <int NB, int HG, int BITS>
+__global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG, BITS>::kCtas) paged_mma_kernel(const __grid_constant__ PagedArgs a) {
+    using G = Shape<NB, HG, BITS>;
+    using L = Plan<NB, HG, BITS>;
     constexpr int D = NB * 32, kE = HG == 4 ? 1 : 2, kPairs = NB / 2;
     constexpr int kO = HG == 4 ? 2 : 4;               // outputs that a lane holds of an MMA tile
     extern __shared__ __align__(128) unsigned char s_dyn[];
@@ -93,7 +103,8 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
     __shared__ Segment s_next[kWorkWarps];
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, j = lane & 3;
-    const float step = 2.0f * a.cent[15] / 15.0f;
+    __shared__ uint32_t s_pairs[BITS == 3 ? 64 : 1][32];   // half2(value of code i & 7, value of code i >> 3), a copy for each bank
+    const float step = 2.0f * a.cent[15] / 15.0f;          // 4-bit: between centroids
     unsigned char* const s_warp = s_dyn + warp * L::kWarpBytes;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_warp);
     unsigned char* const s_digits = s_warp + G::kWarpRing + L::kFragment;
@@ -102,7 +113,7 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
     unsigned char* const s_queries = s_digits + L::kDigits;
     const uint32_t queries = (uint32_t)__cvta_generic_to_shared(s_queries);
     static_assert(kRing == 2 * kInFlight && kStepGroups == kInFlight, "the ring has two halves of a step each");
-    static_assert(L::kFragment <= kInFlight * G::kStage && kJoinSpace * 4 <= G::kWarpRing, "a segment's outputs do not fit into half a ring");
+    static_assert(L::kFragment <= kInFlight * G::kStage && kJoinSpace * 4 <= G::kWarpRing && G::kStage % 16 == 0, "what lies in the ring when it is idle does not fit");
     // a fragment's outputs [HG][D]: that of the warp's last segment lies in its idle ring
     auto fragment = [&](int slot) { return reinterpret_cast<float*>(s_dyn + (slot >> 1) * L::kWarpBytes + ((slot & 1) ? 0 : G::kWarpRing)); };
     // ldmatrix: lane l gives the row address of token 8 ((l >> 3) & 1) + (l & 7), block 2 pair + (l >> 4)
@@ -110,10 +121,19 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
     const uint32_t off_k = tok * G::kRow + (((lane >> 4) ^ G::swizzle(tok)) << 4);   // ^ 32 pair
     const uint32_t off_s = 2 * G::kIdx + n * G::kSc;
     const int piece_t = lane / NB, piece_c = lane % NB;
-    const uint32_t off_p = piece_t * G::kRow + ((piece_c ^ G::swizzle(piece_t)) << 4);
+    const uint32_t off_p = BITS == 4 ? piece_t * G::kRow + ((piece_c ^ G::swizzle(piece_t)) << 4) : lane * 16;
+    // 3-bit: K codes 8j .. 8j + 7 are the 24 bits at byte 3j of a block, V codes 4n .. 4n + 3 the 12 bits at bit 12 n
+    const uint32_t off_k3 = n * G::kRow + 4 * ((3 * j) >> 2), off_k3h = off_k3 + (j < 3 ? 4 : 0), sh_k3 = ((3 * j) & 3) * 8;
+    const uint32_t off_v3 = G::kIdx + 2 * j * G::kRow + 4 * ((12 * n) >> 5), sh_v3 = (12 * n) & 31, off_v3h = off_v3 + (sh_v3 > 20 ? 4 : 0);
     const uint32_t off_ps = 2 * G::kIdx + lane * G::kSc;   // K scales of tokens 0..15, V scales behind them
     const int mask = (1 << a.page_shift) - 1;
+    auto pair_of = [&](uint32_t at) {   // table entry, in bits 7 .. 12 of `at`
+        return *reinterpret_cast<const uint32_t*>(reinterpret_cast<const unsigned char*>(s_pairs) + ((at & 0x1f80u) | (lane * 4)));
+    };
 
+    if (BITS == 3)
+        for (int i = threadIdx.x; i < 64 * 32; i += kWorkThreads)
+            s_pairs[i >> 5][i & 31] = h2_as_u32(__floats2half2_rn(a.values[(i >> 5) & 7], a.values[i >> 8]));
     if (threadIdx.x < 2 * kWorkWarps) s_frag.used[threadIdx.x] = 0;
     WorkLine line(a);   // (its barriers stand before the first use of what is set above)
 
@@ -169,10 +189,12 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
             }
             // whole groups, also where the request ends inside: the page has the room
 #pragma unroll
-            for (int p = 0; p < G::kRow / 32; ++p) {
-                const uint32_t d = st + (NB == 8 && (p & 1) ? off_p ^ 64 : off_p) + p * 512;
-                cp_async16(d, kp + p * 512);
-                cp_async16(d + G::kIdx, vp + p * 512);
+            for (int p = 0; p < G::kCopies; ++p) {
+                const uint32_t d = st + (BITS == 4 && NB == 8 && (p & 1) ? off_p ^ 64 : off_p) + p * 512;
+                if (G::kIdx / 16 >= 32 * (p + 1) || lane + 32 * p < G::kIdx / 16) {
+                    cp_async16(d, kp + p * 512);
+                    cp_async16(d + G::kIdx, vp + p * 512);
+                }
             }
             cp_async_small<G::kSc>(st + off_ps, sp);
             kp += G::kIdx;
@@ -205,9 +227,9 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
             const float inv_sqrt = 1.0f / sqrtf((float)kBlock), sg = block_sign(lane, a.sign_mag);
 #pragma unroll
             for (int e = 0; e < kE; ++e) qsc[e] = 0.0f;
-            // Byte i of k-slots 4j' + i of fragment (b, 4n' + j') is dim 32 b + 8 j' + 2 i (first word) or one above it (second), of
-            // column n': this lane's dim has j' = lane / 8, i = lane / 2 % 4, word lane % 2
-            unsigned char* const at = s_digits + (lane >> 3) * 8 + (lane & 1) * 4 + ((lane >> 1) & 3);
+            // Fragment (b, 4n' + j') of column n' has eight dims from 32 b + 8 j' on, a byte each.  4-bit: the even ones (k-slots 4j' ..)
+            // in its first word, the odd ones (k-slots 16 + 4j' ..) in the second; 3-bit: the first four, the last four.
+            unsigned char* const at = s_digits + (lane >> 3) * 8 + (BITS == 4 ? (lane & 1) * 4 + ((lane >> 1) & 3) : lane & 7);
 #pragma unroll
             for (int h = 0; h < HG; ++h) {
                 float v[NB];
@@ -229,6 +251,10 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
                     if (HG == 4) {
                         at[b * 256 + (2 * h) * 32] = (unsigned char)hi;
                         at[b * 256 + (2 * h + 1) * 32] = (unsigned char)lo;
+                        if (BITS == 3) {
+                            at[(NB + b) * 256 + (2 * h) * 32] = 0;
+                            at[(NB + b) * 256 + (2 * h + 1) * 32] = (unsigned char)hi;
+                        }
                     } else {
                         at[b * 256 + h * 32] = (unsigned char)hi;
                         at[(NB + b) * 256 + h * 32] = (unsigned char)lo;
@@ -236,7 +262,7 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
                 }
 #pragma unroll
                 for (int e = 0; e < kE; ++e)
-                    if (h == (HG == 4 ? j : 2 * j + e)) qsc[e] = m * (a.qk_const * step / (kQMax * 16.0f));
+                    if (h == (HG == 4 ? j : 2 * j + e)) qsc[e] = m * (a.qk_const * (BITS == 4 ? step / (kQMax * 16.0f) : a.cent[7] * 256.0f / (kQMax * kQMax)));
             }
             __syncwarp();
         }
@@ -281,26 +307,49 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
                     static_for<0, kPairs>([&](auto p_) {
                         constexpr int p = decltype(p_)::value;
                         uint32_t kw[4];
-                        ldsm4_o<0>(stu + (off_k ^ (32 * p)), kw);
+                        if (BITS == 4) ldsm4_o<0>(stu + (off_k ^ (32 * p)), kw);
                         const uint32_t sa = lds32_o<4 * p>(stu + off_s) & 0x7fff7fffu, sb = lds32_o<4 * p + 8 * G::kSc>(stu + off_s) & 0x7fff7fffu;
                         static_for<0, 2>([&](auto i_) {
                             constexpr int i = decltype(i_)::value, b = 2 * p + i;
                             const float ka = i ? __high2float(u32_as_h2(sa)) : __low2float(u32_as_h2(sa));
                             const float kc = i ? __high2float(u32_as_h2(sb)) : __low2float(u32_as_h2(sb));
-                            // c ^ 8 is the two's complement of c - 8; at the top of a byte with bit 3 set below it: 16 (c - 7.5)
-                            const uint32_t u0 = kw[2 * i], u1 = kw[2 * i + 1];
-                            const uint32_t a0 = lop3_xor_select(u0 << 4, 0xF0F0F0F0u, 0x88888888u), a2 = lop3_xor_select(u0, 0xF0F0F0F0u, 0x88888888u);
-                            const uint32_t a1 = lop3_xor_select(u1 << 4, 0xF0F0F0F0u, 0x88888888u), a3 = lop3_xor_select(u1, 0xF0F0F0F0u, 0x88888888u);
                             const uint2 qa = lds64_o<b * 256>(digits);
-                            int hi[4];
-                            imma16832(hi, a0, a1, a2, a3, qa.x, qa.y);
+                            int hi[4], lo[4];
+                            if constexpr (BITS == 4) {
+                                // c ^ 8 is the two's complement of c - 8; at the top of a byte with bit 3 set below it: 16 (c - 7.5)
+                                const uint32_t u0 = kw[2 * i], u1 = kw[2 * i + 1];
+                                const uint32_t a0 = lop3_xor_select(u0 << 4, 0xF0F0F0F0u, 0x88888888u), a2 = lop3_xor_select(u0, 0xF0F0F0F0u, 0x88888888u);
+                                const uint32_t a1 = lop3_xor_select(u1 << 4, 0xF0F0F0F0u, 0x88888888u), a3 = lop3_xor_select(u1, 0xF0F0F0F0u, 0x88888888u);
+                                imma16832(hi, a0, a1, a2, a3, qa.x, qa.y);
+                                if (HG == 8) {
+                                    const uint2 qb = lds64_o<(HG == 8 ? NB + b : b) * 256>(digits);
+                                    imma16832(lo, a0, a1, a2, a3, qb.x, qb.y);
+                                }
+                            } else {
+                                // The centroid as two base-256 digits: its bytes come out of an eight-entry table by PRMT.  Two columns a
+                                // head: the second set of digits has D1 in D0's column, so that one accumulator gathers what counts 256.
+                                uint32_t x[2][4];   // [token n | n + 8]: first digits of codes 0..3, 4..7, second digits
+                                static_for<0, 2>([&](auto t_) {
+                                    constexpr int t = decltype(t_)::value;
+                                    const uint32_t c = nibbles_of_codes(__funnelshift_r(lds32_o<12 * b + 8 * t * G::kRow>(stu + off_k3), lds32_o<12 * b + 8 * t * G::kRow>(stu + off_k3h), sh_k3));
+                                    x[t][0] = __byte_perm(a.digits[0], a.digits[1], c);
+                                    x[t][1] = __byte_perm(a.digits[0], a.digits[1], c >> 16);
+                                    x[t][2] = __byte_perm(a.digits[2], a.digits[3], c);
+                                    x[t][3] = __byte_perm(a.digits[2], a.digits[3], c >> 16);
+                                });
+                                const uint2 qb = lds64_o<(NB + b) * 256>(digits);
+                                imma16832(hi, x[0][0], x[1][0], x[0][1], x[1][1], qa.x, qa.y);
+                                if (HG == 4) {
+                                    imma16832_acc(hi, x[0][2], x[1][2], x[0][3], x[1][3], qb.x, qb.y);
+                                } else {
+                                    imma16832(lo, x[0][0], x[1][0], x[0][1], x[1][1], qb.x, qb.y);
+                                    imma16832_acc(lo, x[0][2], x[1][2], x[0][3], x[1][3], qa.x, qa.y);
+                                }
+                            }
                             if constexpr (HG == 4) {
                                 acc[0][0] = fmaf(ka, (float)(hi[0] * 256 + hi[1]), acc[0][0]);
                                 acc[1][0] = fmaf(kc, (float)(hi[2] * 256 + hi[3]), acc[1][0]);
                             } else {
-                                const uint2 qb = lds64_o<(NB + b) * 256>(digits);
-                                int lo[4];
-                                imma16832(lo, a0, a1, a2, a3, qb.x, qb.y);
 #pragma unroll
                                 for (int e = 0; e < kE; ++e) {
                                     acc[0][e] = fmaf(ka, (float)(hi[e] * 256 + lo[e]), acc[0][e]);
@@ -434,28 +483,47 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
                     constexpr int pr = decltype(p_)::value;
                     uint32_t vw[kStepGroups][4];
 #pragma unroll
-                    for (int u = 0; u < kStepGroups; ++u) ldsm4t_o<G::kIdx>(st + u * G::kStage + (off_k ^ (32 * pr)), vw[u]);
+                    for (int u = 0; u < kStepGroups; ++u)
+                        if (BITS == 4) ldsm4t_o<G::kIdx>(st + u * G::kStage + (off_k ^ (32 * pr)), vw[u]);
                     float centre[4];
                     static_for<0, 2>([&](auto i_) {
                         constexpr int i = decltype(i_)::value, b = 2 * pr + i, f = HG == 4 ? pr : b;
-                        if (HG == 8 || i == 0) {
+                        if (BITS == 3) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) centre[k] = 0.0f;
+                        } else if (HG == 8 || i == 0) {
                             mma16816_from(centre, zero, kCentreEven, kCentreOdd, kCentreEven, kCentreOdd, pq[0][f][0], pq[0][f][1]);
 #pragma unroll
                             for (int u = 1; u < kStepGroups; ++u)
                                 mma16816(centre, kCentreEven, kCentreOdd, kCentreEven, kCentreOdd, pq[u][f][0], pq[u][f][1]);
                         }
                         float acc[2][4];
-#pragma unroll
-                        for (int u = 0; u < kStepGroups; ++u) {
+                        static_for<0, kStepGroups>([&](auto u_) {
+                            constexpr int u = decltype(u_)::value;
                             uint32_t xa[4], xb[4];   // tokens 2j, 2j + 1 and 2j + 8, 2j + 9: codes 4n .. 4n + 3 of the block
-                            codes_to_subnormals(vw[u][2 * i], xa);
-                            codes_to_subnormals(vw[u][2 * i + 1], xb);
+                            if constexpr (BITS == 4) {
+                                codes_to_subnormals(vw[u][2 * i], xa);
+                                codes_to_subnormals(vw[u][2 * i + 1], xb);
+                            } else {
+                                static_for<0, 2>([&](auto o_) {
+                                    constexpr int o8 = decltype(o_)::value, off = 12 * b + 8 * o8 * G::kRow + u * G::kStage;
+                                    const uint32_t ya = __funnelshift_r(lds32_o<off>(st + off_v3), lds32_o<off>(st + off_v3h), sh_v3);
+                                    const uint32_t yb = __funnelshift_r(lds32_o<off + G::kRow>(st + off_v3), lds32_o<off + G::kRow>(st + off_v3h), sh_v3);
+                                    // six-bit pairs (token 2j | token 2j + 1 << 3): codes 0 and 2, codes 1 and 3
+                                    const uint32_t z0 = bit_select(ya, yb << 3, 0x1c7u), z1 = bit_select(ya >> 3, yb, 0x1c7u);
+                                    uint32_t* x = o8 == 0 ? xa : xb;
+                                    x[0] = pair_of(z0 << 7);
+                                    x[1] = pair_of(z1 << 7);
+                                    x[2] = pair_of(z0 << 1);
+                                    x[3] = pair_of(z1 << 1);
+                                });
+                            }
 #pragma unroll
                             for (int m = 0; m < 2; ++m) {
                                 if (u == 0) mma16816_from(acc[m], centre, xa[2 * m], xa[2 * m + 1], xb[2 * m], xb[2 * m + 1], pq[u][f][0], pq[u][f][1]);
                                 else mma16816(acc[m], xa[2 * m], xa[2 * m + 1], xb[2 * m], xb[2 * m + 1], pq[u][f][0], pq[u][f][1]);
                             }
-                        }
+                        });
 #pragma unroll
                         for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -473,7 +541,7 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
         const int slot = 2 * warp + (s.begins ? 1 : 0);
         float* const to = whole ? reinterpret_cast<float*>(s_warp + (halves - st - ring)) : fragment(slot);
         if (!whole && s.begins) cp_async_wait<0>();   // the warp's last segment: its ring is idle
-        const float even = step * 8388608.0f, odd = step * 524288.0f;   // 2^23, 2^19
+        const float even = BITS == 4 ? step * 8388608.0f : a.kappa, odd = BITS == 4 ? step * 524288.0f : a.kappa;   // 2^23, 2^19
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -514,20 +582,35 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG>::kCtas) paged_mma_k
     write_empty<NB>(a);
 }
 
-template <int NB, int HG>
+template <int NB, int HG, int BITS>
 int launch(const PagedArgs& a, cudaStream_t s) {
-    if (int st = allow_shared<paged_mma_kernel<NB, HG>>(Plan<NB, HG>::kBytes)) return st;
-    paged_mma_kernel<NB, HG><<<148 * Plan<NB, HG>::kCtas, kWorkThreads, Plan<NB, HG>::kBytes, s>>>(a);
+    using L = Plan<NB, HG, BITS>;
+    if (int st = allow_shared<paged_mma_kernel<NB, HG, BITS>>(L::kBytes)) return st;
+    paged_mma_kernel<NB, HG, BITS><<<148 * L::kCtas, kWorkThreads, L::kBytes, s>>>(a);
     return check_launch(s);
+}
+
+template <int BITS>
+int launch_bits(const PagedArgs& a, int head_dim, cudaStream_t s) {
+    const bool narrow = a.group <= 4;
+    if (head_dim == 64) return narrow ? launch<2, 4, BITS>(a, s) : launch<2, 8, BITS>(a, s);
+    if (head_dim == 128) return narrow ? launch<4, 4, BITS>(a, s) : launch<4, 8, BITS>(a, s);
+    return narrow ? launch<8, 4, BITS>(a, s) : launch<8, 8, BITS>(a, s);
 }
 
 }  // namespace
 
-int launch_paged_mma(const PagedArgs& a, int head_dim, cudaStream_t s) {
-    const bool narrow = a.group <= 4;
-    if (head_dim == 64) return narrow ? launch<2, 4>(a, s) : launch<2, 8>(a, s);
-    if (head_dim == 128) return narrow ? launch<4, 4>(a, s) : launch<4, 8>(a, s);
-    return narrow ? launch<8, 4>(a, s) : launch<8, 8>(a, s);
+int launch_paged_mma(const PagedArgs& a, int head_dim, int bits, cudaStream_t s) {
+    if (bits == 4) return launch_bits<4>(a, head_dim, s);
+    PagedArgs b = a;
+    if (!pqo3_values(TQB_MAXNORM, true, b.kappa, b.values)) return TQB_ERR_UNSUPPORTED;
+    for (int i = 0; i < 4; ++i) b.digits[i] = 0;
+    for (int i = 0; i < 8; ++i) {
+        const int v = (int)lrintf(a.cent[i] / a.cent[7] * kQMax), lo = (int)(signed char)(v & 0xff), hi = (v - lo) >> 8;
+        b.digits[i >> 2] |= (uint32_t)(hi & 0xff) << (8 * (i & 3));
+        b.digits[2 + (i >> 2)] |= (uint32_t)(lo & 0xff) << (8 * (i & 3));
+    }
+    return launch_bits<3>(b, head_dim, s);
 }
 
 }  // namespace tqb

@@ -46,9 +46,12 @@ struct PagedArgs {
     float qk_const;      // softmax_scale * log2(e)
     float sign_mag;
     float cent[16];
+    // 3-bit, tensor-core kernel: centroid / kappa, and centroids / the largest * 32639 in two base-256 digits ([0..1] the high ones)
+    float kappa, values[8];
+    uint32_t digits[4];
 };
 
-int launch_paged_mma(const PagedArgs& a, int head_dim, cudaStream_t s);   // 4-bit, 16-bit queries, some page
+int launch_paged_mma(const PagedArgs& a, int head_dim, int bits, cudaStream_t s);   // 16-bit queries, some page
 
 struct Segment {
     int req, kvh, head0, heads;   // query heads head0 .. head0 + heads - 1 of the request
