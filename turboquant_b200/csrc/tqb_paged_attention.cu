@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kWorkThreads) paged_simple_kernel(const __grid
             __syncwarp();
         }
     }
-    finish<NB>(a, s_frag, s_o, [&](int c, int x) { return reinterpret_cast<const float4*>(s_o + c * kSegHeads * D)[x]; });
+    finish<NB>(a, s_frag, [&](int c, int x) { return reinterpret_cast<const float4*>(s_o + c * kSegHeads * D)[x]; });
     write_empty<NB>(a);
 }
 
@@ -109,7 +109,7 @@ int launch_simple(const PagedArgs& a, cudaStream_t s) {
     return check_launch(s);
 }
 
-size_t part_bytes(int head_dim) { return sizeof(float) * (size_t)kMaxCtas * 2 * kSegHeads * (2 + head_dim); }
+size_t part_bytes(int head_dim) { return sizeof(float) * (size_t)kMaxCtas * 2 * kSegHeads * (2 + 2 + head_dim); }
 
 }  // namespace
 }  // namespace tqb
@@ -155,7 +155,8 @@ int tqb_paged_attention(const tqb_paged_layer* layer, const tqb_paged_attention_
     a.lens = p->kv_lens;
     a.tickets = reinterpret_cast<unsigned*>(p->scratch);
     a.part_ml = reinterpret_cast<float*>(reinterpret_cast<char*>(p->scratch) + TQB_PAGED_TICKET_BYTES);
-    a.part_out = a.part_ml + (size_t)kMaxCtas * 2 * kSegHeads * 2;
+    a.round_ml = a.part_ml + (size_t)kMaxCtas * 2 * kSegHeads * 2;
+    a.part_out = a.round_ml + (size_t)kMaxCtas * 2 * kSegHeads * 2;
     a.q_stride = p->q_row_stride != 0 ? p->q_row_stride : (long long)p->num_q_heads * layer->head_dim;
     a.table_stride = p->table_stride;
     a.requests = p->num_requests;

@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG, BITS>::kCtas) paged
     unsigned char* const s_queries = s_digits + L::kDigits;
     const uint32_t queries = (uint32_t)__cvta_generic_to_shared(s_queries);
     static_assert(kRing == 2 * kInFlight && kStepGroups == kInFlight, "the ring has two halves of a step each");
-    static_assert(L::kFragment <= kInFlight * G::kStage && kJoinSpace * 4 <= G::kWarpRing && G::kStage % 16 == 0, "what lies in the ring when it is idle does not fit");
+    static_assert(L::kFragment <= kInFlight * G::kStage && G::kStage % 16 == 0, "what lies in the ring when it is idle does not fit");
     // a fragment's outputs [HG][D]: that of the warp's last segment lies in its idle ring
     auto fragment = [&](int slot) { return reinterpret_cast<float*>(s_dyn + (slot >> 1) * L::kWarpBytes + ((slot & 1) ? 0 : G::kWarpRing)); };
     // ldmatrix: lane l gives the row address of token 8 ((l >> 3) & 1) + (l & 7), block 2 pair + (l >> 4)
@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG, BITS>::kCtas) paged
         }
         s = s_next[warp];
     }
-    finish<NB>(a, s_frag, reinterpret_cast<float*>(s_dyn), [&](int c, int x) { return reinterpret_cast<const float4*>(fragment(c))[x]; });
+    finish<NB>(a, s_frag, [&](int c, int x) { return reinterpret_cast<const float4*>(fragment(c))[x]; });
     write_empty<NB>(a);
 }
 

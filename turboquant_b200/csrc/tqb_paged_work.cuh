@@ -19,7 +19,14 @@
 namespace tqb {
 
 constexpr int kRunTokens = 16;       // of a group
-constexpr int kOpenCost = 2;         // groups that beginning a segment is worth
+#ifndef OPENCOST
+#define OPENCOST 6
+#endif
+#ifndef MINRUN
+#define MINRUN 4
+#endif
+constexpr int kOpenCost = OPENCOST;  // groups that beginning a segment is worth
+constexpr int kMinRun = MINRUN;      // units of a run, at least
 constexpr int kSegHeads = 8;         // query heads of a segment, at most
 constexpr int kWorkWarps = 4;
 constexpr int kWorkThreads = 32 * kWorkWarps;
@@ -39,6 +46,7 @@ struct PagedArgs {
     const int32_t* lens;
     unsigned* tickets;
     float* part_ml;      // [kMaxCtas][2][kSegHeads][2]: maximum (log2 units), sum
+    float* round_ml;     // the same of joined parts, where two rounds are needed
     float* part_out;     // [kMaxCtas][2][kSegHeads][D], rotated domain
     long long q_stride, table_stride;
     int requests, max_blocks, max_len, page_shift, num_pages, hkv, group, vheads, splits;   // vheads = hkv * splits
@@ -115,7 +123,7 @@ struct WorkLine {
         total *= a.vheads;
         // as many runs as the longest run needs: it is no longer with them, and fewer parts are joined
         const unsigned most = gridDim.x * kWorkWarps, i = blockIdx.x * kWorkWarps + warp;
-        const Units longest = divide(total + most - 1, most), runs = longest > 0 ? divide(total + longest - 1, longest) : 0;
+        const Units longest = max(divide(total + most - 1, most), (Units)min(total, (Units)kMinRun)), runs = longest > 0 ? divide(total + longest - 1, longest) : 0;
         cur = end = base = 0;
         quot = rem = 0;
         req = len = 0;
@@ -244,16 +252,9 @@ __device__ __forceinline__ void write_quad(const PagedArgs& a, const Segment& s,
     if (live) store4(a.out, a.out_dtype, ((size_t)s.req * a.hkv * a.group + s.head0) * (NB * 32) + 4 * x, v);
 }
 
-__device__ __forceinline__ void add_scaled(float4& acc, float4 v, float w) {
-    acc.x = fmaf(v.x, w, acc.x);
-    acc.y = fmaf(v.y, w, acc.y);
-    acc.z = fmaf(v.z, w, acc.z);
-    acc.w = fmaf(v.w, w, acc.w);
-}
-
-// How many of a (request, head)'s parts are joined at a time: up to 16 at once, more of them in two rounds.  (A round is a
+// How many of a (request, head)'s parts are joined at a time: up to 24 at once, more of them in two rounds.  (A round is a
 // fence, a ticket and two dependent trips to L2, about 2.5 us; 93 parts in one round took a CTA 30 us.)
-__device__ __forceinline__ int parts_per_round(int parts) { return parts <= 16 ? parts : parts <= 64 ? 8 : parts <= 256 ? 16 : kMaxRound; }
+__device__ __forceinline__ int parts_per_round(int parts) { return parts <= 24 ? parts : parts <= 64 ? 8 : parts <= 256 ? 16 : kMaxRound; }
 static_assert(kMaxRound * kMaxRound >= kMaxCtas, "two rounds are enough");
 
 // Arrivals at up to two tickets (nullptr: none) of `want` each, after everything that the CTA's threads have written; bit i:
@@ -278,63 +279,71 @@ __device__ __forceinline__ int arrive(unsigned* ticket0, int want0, unsigned* ti
 }
 
 // Where part i of a (request, head) lies: of the first CTA the second slot, of the others the first.
-__device__ __forceinline__ size_t part_at(int cta0, int i) { return (size_t)((cta0 + i) * 2 + (i == 0 ? 1 : 0)) * kSegHeads; }
+__device__ __forceinline__ unsigned part_at(int cta0, int i) { return (unsigned)((cta0 + i) * 2 + (i == 0 ? 1 : 0)) * kSegHeads; }
 
-// Joins parts i0, i0 + stride, .. (`count` <= kMaxRound of them) of a (request, head): into the output, or into the place
-// of part i0.  space: kJoinSpace floats of shared memory.
-constexpr int kJoinSpace = kSegHeads * (kMaxRound + 1);
-template <int NB>
-__device__ __noinline__ void join_parts(const PagedArgs& a, const Segment& s, int i0, int stride, int count, bool to_out, float* space) {
+// A running (maximum, sum, output) of a softmax, four dims of a head.
+struct Running {
+    float M = kNoScore, L = 0.0f;
+    float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    __device__ __forceinline__ void raise(float m) {
+        const float to = fmaxf(M, m), keep = exp2_fast(M - to);
+        M = to;
+        L *= keep;
+        O.x *= keep;
+        O.y *= keep;
+        O.z *= keep;
+        O.w *= keep;
+    }
+    __device__ __forceinline__ void add(float m, float l, float4 o) {   // m is not above M
+        const float e = exp2_fast(m - M);
+        L = fmaf(l, e, L);
+        O.x = fmaf(o.x, e, O.x);
+        O.y = fmaf(o.y, e, O.y);
+        O.z = fmaf(o.z, e, O.z);
+        O.w = fmaf(o.w, e, O.w);
+    }
+};
+
+// Joins parts i0, i0 + stride, .. (`count` of them) of a (request, head): into the output, or (FIRST: the first of two rounds)
+// into the place of part i0, with maximum and sum in a place of their own, since other threads still read part i0's.
+// Every thread reads the maxima and sums of its head for itself, beside the outputs: one trip to L2 for eight parts, no
+// barrier.
+template <int NB, bool FIRST>
+__device__ __forceinline__ void join_parts(const PagedArgs& a, const Segment& s, int i0, int stride, int count) {
     constexpr int D = NB * 32, kAtOnce = 8;
-    float (*s_w)[kMaxRound] = reinterpret_cast<float (*)[kMaxRound]>(space);   // [kSegHeads]
-    float* s_L = space + kSegHeads * kMaxRound;                                // [kSegHeads]
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int hh = warp; hh < s.heads; hh += kWorkWarps) {
-        float2 ml[(kMaxRound + 31) / 32];
-        float M = kNoScore, L = 0.0f;
-#pragma unroll
-        for (int k = 0; k < (kMaxRound + 31) / 32; ++k) {
-            const int i = k * 32 + lane;
-            ml[k] = i < count ? __ldcg(reinterpret_cast<const float2*>(a.part_ml + (part_at(s.cta0, i0 + i * stride) + hh) * 2)) : make_float2(kNoScore, 0.0f);
-            M = fmaxf(M, ml[k].x);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-#pragma unroll
-        for (int k = 0; k < (kMaxRound + 31) / 32; ++k) {
-            const int i = k * 32 + lane;
-            const float w = exp2_fast(ml[k].x - M);
-            if (i < count) {
-                s_w[hh][i] = w;
-                L = fmaf(ml[k].y, w, L);
-            }
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-        if (lane == 0) {
-            s_L[hh] = L;
-            if (!to_out) *reinterpret_cast<float2*>(a.part_ml + (part_at(s.cta0, i0) + hh) * 2) = make_float2(M, L);
-        }
-    }
-    __syncthreads();
-    const int quads = s.heads * (D / 4);
-    for (int x0 = warp * 32; x0 < quads; x0 += kWorkThreads) {
+    const int lane = threadIdx.x & 31, quads = s.heads * (D / 4);
+    for (int x0 = (int)threadIdx.x - lane; x0 < quads; x0 += kWorkThreads) {
         const int x = min(x0 + lane, quads - 1), hh = x / (D / 4);
-        const bool live = x0 + lane < quads;
-        float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int i = 0; i < count; i += kAtOnce) {   // loads that are in flight together
+        const float2* ml_in = reinterpret_cast<const float2*>(!FIRST && stride > 1 ? a.round_ml : a.part_ml) + hh;
+        const float4* out_in = reinterpret_cast<const float4*>(a.part_out) + x;
+        Running r;
+        for (int i = 0; i < count; i += kAtOnce) {
             float4 v[kAtOnce];
+            float2 ml[kAtOnce];
 #pragma unroll
             for (int k = 0; k < kAtOnce; ++k)
-                if (i + k < count) v[k] = __ldcg(reinterpret_cast<const float4*>(a.part_out + part_at(s.cta0, i0 + (i + k) * stride) * D) + x);
+                if (i + k < count) {
+                    const unsigned at = part_at(s.cta0, i0 + (i + k) * stride);
+                    ml[k] = __ldcg(ml_in + at);
+                    v[k] = __ldcg(out_in + at * (D / 4));
+                }
+            float top = kNoScore;
 #pragma unroll
             for (int k = 0; k < kAtOnce; ++k)
-                if (i + k < count) add_scaled(O, v[k], s_w[hh][i + k]);
+                if (i + k < count) top = fmaxf(top, ml[k].x);
+            r.raise(top);
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k)
+                if (i + k < count) r.add(ml[k].x, ml[k].y, v[k]);
         }
-        if (to_out) write_quad<NB>(a, s, x, live, O, s_L[hh]);
-        else if (live) reinterpret_cast<float4*>(a.part_out + part_at(s.cta0, i0) * D)[x] = O;
+        if constexpr (!FIRST) {
+            write_quad<NB>(a, s, x, x0 + lane < quads, r.O, r.L);
+        } else if (x0 + lane < quads) {
+            const unsigned at = part_at(s.cta0, i0);
+            reinterpret_cast<float4*>(a.part_out)[at * (D / 4) + x] = r.O;
+            if (x % (D / 4) == 0) reinterpret_cast<float2*>(a.round_ml)[at + hh] = make_float2(r.M, r.L);
+        }
     }
-    __syncthreads();   // s_w is free again
 }
 
 // A CTA's segments that are not whole: of each warp the one that began before it (slot 2 w) and the one that goes on behind it
@@ -345,10 +354,9 @@ struct Fragments {
     int used[2 * kWorkWarps];
 };
 
-// The CTA's end, by all of its threads: quad(slot, x) are four of a fragment's un-normalised rotated outputs.  join_space:
-// shared memory for join_parts, which may be that of the fragments.
+// The CTA's end, by all of its threads: quad(slot, x) are four of a fragment's un-normalised rotated outputs.
 template <int NB, typename F>
-__device__ __forceinline__ void finish(const PagedArgs& a, const Fragments& f, float* join_space, F quad) {
+__device__ __forceinline__ void finish(const PagedArgs& a, const Fragments& f, F quad) {
     constexpr int D = NB * 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     __syncthreads();
@@ -370,21 +378,17 @@ __device__ __forceinline__ void finish(const PagedArgs& a, const Fragments& f, f
         const size_t at = (size_t)(blockIdx.x * 2 + side) * kSegHeads;
         for (int x0 = warp * 32; x0 < quads; x0 += kWorkThreads) {
             const int x = min(x0 + lane, quads - 1), hh = x / (D / 4);
-            float M = kNoScore;
-            for (unsigned m = mine; m != 0; m &= m - 1) M = fmaxf(M, f.m[__ffs(m) - 1][hh]);
-            float L = 0.0f;
-            float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            Running r;
+            for (unsigned m = mine; m != 0; m &= m - 1) r.M = fmaxf(r.M, f.m[__ffs(m) - 1][hh]);
             for (unsigned m = mine; m != 0; m &= m - 1) {
                 const int c = __ffs(m) - 1;
-                const float e = exp2_fast(f.m[c][hh] - M);
-                L = fmaf(f.l[c][hh], e, L);
-                add_scaled(O, quad(c, x), e);
+                r.add(f.m[c][hh], f.l[c][hh], quad(c, x));
             }
             if (done) {
-                write_quad<NB>(a, s, x, x0 + lane < quads, O, L);
+                write_quad<NB>(a, s, x, x0 + lane < quads, r.O, r.L);
             } else if (x0 + lane < quads) {
-                reinterpret_cast<float4*>(a.part_out + at * D)[x] = O;
-                if (x % (D / 4) == 0) *reinterpret_cast<float2*>(a.part_ml + (at + hh) * 2) = make_float2(M, L);
+                reinterpret_cast<float4*>(a.part_out + at * D)[x] = r.O;
+                if (x % (D / 4) == 0) reinterpret_cast<float2*>(a.part_ml)[at + hh] = make_float2(r.M, r.L);
             }
         }
     }
@@ -420,9 +424,9 @@ __device__ __forceinline__ void finish(const PagedArgs& a, const Fragments& f, f
             if (!((won >> side) & 1)) continue;
             const Segment& s = f.seg[crossing[side]];
             const bool two = per[side] < s.ctas, last = !two || round == 1;
-            if (last) join_parts<NB>(a, s, 0, two ? per[side] : 1, two ? (s.ctas + per[side] - 1) / per[side] : s.ctas, true, join_space);
+            if (last) join_parts<NB, false>(a, s, 0, two ? per[side] : 1, two ? (s.ctas + per[side] - 1) / per[side] : s.ctas);
             else {
-                join_parts<NB>(a, s, first[side], 1, want[side], false, join_space);
+                join_parts<NB, true>(a, s, first[side], 1, want[side]);
                 ticket[side] = a.tickets + s.cta0;
                 want[side] = (s.ctas + per[side] - 1) / per[side];
                 again = true;
