@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(kWorkThreads) paged_simple_kernel(const __grid
                 float L = l[0];
 #pragma unroll
                 for (int h = 1; h < kSegHeads; ++h) L = h == hh ? l[h] : L;
-                write_quad<NB>(a, s, x, x0 + lane < quads, reinterpret_cast<const float4*>(s_o + slot * kSegHeads * D)[x], L);
+                write_quad(a.out, a.out_dtype, quad_at<NB>(a, s, x), x0 + lane < quads, reinterpret_cast<const float4*>(s_o + slot * kSegHeads * D)[x], L, a.sign_mag);
             }
             __syncwarp();
         }

@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG, BITS>::kCtas) paged
 
     if (more) {
         open(s);
-#pragma unroll
+#pragma unroll 1
         for (int u = 0; u < kStepGroups; ++u) fill(ring + u * G::kStage);
     }
     uint32_t st = ring;
@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG, BITS>::kCtas) paged
             // Fragment (b, 4n' + j') of column n' has eight dims from 32 b + 8 j' on, a byte each.  4-bit: the even ones (k-slots 4j' ..)
             // in its first word, the odd ones (k-slots 16 + 4j' ..) in the second; 3-bit: the first four, the last four.
             unsigned char* const at = s_digits + (lane >> 3) * 8 + (BITS == 4 ? (lane & 1) * 4 + ((lane >> 1) & 3) : lane & 7);
-#pragma unroll
+#pragma unroll 1
             for (int h = 0; h < HG; ++h) {
                 float v[NB];
                 uint32_t top = 0;   // of the bits, so that NaN is above infinity
@@ -568,11 +568,11 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG, BITS>::kCtas) paged
         __syncwarp();
         if (whole) {
             const int quads = s.heads * (D / 4);
-#pragma unroll
-            for (int x0 = 0; x0 < HG * (D / 4); x0 += 32) {
+#pragma unroll 1
+            for (int x0 = 0; x0 < quads; x0 += 32) {
                 const int x = x0 + lane, h = x / (D / 4);
                 const float l0 = __shfl_sync(0xffffffffu, l_run[0], h / kE), l1 = __shfl_sync(0xffffffffu, l_run[kE - 1], h / kE);
-                if (x0 < quads) write_quad<NB>(a, s, x, x < quads, reinterpret_cast<const float4*>(to)[x], (h % kE) ? l1 : l0);
+                write_quad(a.out, a.out_dtype, quad_at<NB>(a, s, x), x < quads, reinterpret_cast<const float4*>(to)[x], (h % kE) ? l1 : l0, a.sign_mag);
             }
             __syncwarp();
         }

@@ -225,58 +225,40 @@ __device__ __forceinline__ void store4(void* p, int dtype, size_t i, const float
     }
 }
 
-// Outputs leave four dims a lane: lane l of a warp has the quad `x` (x = l modulo 8) of a request's heads, head0 * D / 4 + x ..
-// Rotated output O over the softmax sum L, back through the rotation (stages 1, 2 in the lane, 4, 8, 16 between lanes).
-// All lanes of the warp take part.
-template <int NB>
-__device__ __forceinline__ void write_quad(const PagedArgs& a, const Segment& s, int x, bool live, float4 O, float L) {
+// Outputs leave four dims a lane, lane l of a warp with dims 4 (l modulo 8) .. of a 32-block: the rotated output O over the
+// softmax sum L, back through the rotation (stages 1, 2 in the lane, 4, 8, 16 between lanes), to elements i .. i + 3.  All
+// lanes of the warp take part.  Not inlined, like what else runs once a segment: code that runs once waits for its
+// instructions more than for anything else (10 of 18 stalls an instruction in a call of one short request).
+static __device__ __noinline__ void write_quad(void* out, int dtype, size_t i, bool live, float4 O, float L, float sign_mag) {
     const int lane = threadIdx.x & 31;
-    float v[4] = {O.x, O.y, O.z, O.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] *= ((0xB1A6D4B2u >> (4 * (lane & 7) + i)) & 1u) ? -a.sign_mag : a.sign_mag;   // src/cache/precomputed/rotation.rs:16-20
+    const uint32_t neg = 0xB1A6D4B2u >> (4 * (lane & 7));   // src/cache/precomputed/rotation.rs:16-20
+    float v[4] = {(neg & 1u) ? -O.x : O.x, (neg & 2u) ? -O.y : O.y, (neg & 4u) ? -O.z : O.z, (neg & 8u) ? -O.w : O.w};
     const float p = v[0] + v[1], q = v[0] - v[1], r = v[2] + v[3], t = v[2] - v[3];
     v[0] = p + r;
     v[1] = q + t;
     v[2] = p - r;
     v[3] = q - t;
-#pragma unroll
+#pragma unroll 1
     for (int m = 1; m <= 4; m <<= 1)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float other = __shfl_xor_sync(0xffffffffu, v[i], m);
-            v[i] = (lane & m) ? (other - v[i]) : (v[i] + other);
+        for (int k = 0; k < 4; ++k) {
+            const float other = __shfl_xor_sync(0xffffffffu, v[k], m);
+            v[k] = (lane & m) ? (other - v[k]) : (v[k] + other);
         }
-    const float inv = L == 0.0f ? 0.0f : (1.0f / sqrtf((float)kBlock)) / L;   // L is 0 where no page of the request can be read
+    const float inv = L == 0.0f ? 0.0f : __fdividef(sign_mag * (1.0f / sqrtf((float)kBlock)), L);   // L is 0 where no page of the request can be read
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] *= inv;
-    if (live) store4(a.out, a.out_dtype, ((size_t)s.req * a.hkv * a.group + s.head0) * (NB * 32) + 4 * x, v);
+    for (int k = 0; k < 4; ++k) v[k] *= inv;
+    if (live) store4(out, dtype, i, v);
+}
+template <int NB>
+__device__ __forceinline__ size_t quad_at(const PagedArgs& a, const Segment& s, int x) {   // element 4 x of the segment's heads
+    return ((size_t)s.req * a.hkv * a.group + s.head0) * (NB * 32) + 4 * x;
 }
 
 // How many of a (request, head)'s parts are joined at a time: up to 24 at once, more of them in two rounds.  (A round is a
 // fence, a ticket and two dependent trips to L2, about 2.5 us; 93 parts in one round took a CTA 30 us.)
 __device__ __forceinline__ int parts_per_round(int parts) { return parts <= 24 ? parts : parts <= 64 ? 8 : parts <= 256 ? 16 : kMaxRound; }
 static_assert(kMaxRound * kMaxRound >= kMaxCtas, "two rounds are enough");
-
-// Arrivals at up to two tickets (nullptr: none) of `want` each, after everything that the CTA's threads have written; bit i:
-// this CTA is the last at ticket i, and its threads see what the others have written.
-__device__ __forceinline__ int arrive(unsigned* ticket0, int want0, unsigned* ticket1, int want1) {
-    __shared__ int s_last[2];
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0 && threadIdx.x < 64) {   // a warp each: the fences and the round trips overlap
-        unsigned* ticket = threadIdx.x == 0 ? ticket0 : ticket1;
-        const int want = threadIdx.x == 0 ? want0 : want1;
-        int last = 0;
-        if (ticket != nullptr) {
-            unsigned old;
-            asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;\n" : "=r"(old) : "l"(ticket) : "memory");
-            last = old == (unsigned)(want - 1);
-            if (last) *ticket = 0u;   // ready for the next call
-        }
-        s_last[threadIdx.x >> 5] = last;
-    }
-    __syncthreads();
-    return s_last[0] | (s_last[1] << 1);
-}
 
 // Where part i of a (request, head) lies: of the first CTA the second slot, of the others the first.
 __device__ __forceinline__ unsigned part_at(int cta0, int i) { return (unsigned)((cta0 + i) * 2 + (i == 0 ? 1 : 0)) * kSegHeads; }
@@ -304,42 +286,48 @@ struct Running {
     }
 };
 
-// Joins parts i0, i0 + stride, .. (`count` of them) of a (request, head): into the output, or (FIRST: the first of two rounds)
-// into the place of part i0, with maximum and sum in a place of their own, since other threads still read part i0's.
-// Every thread reads the maxima and sums of its head for itself, beside the outputs: one trip to L2 for eight parts, no
+// Parts i0, i0 + stride, .. (`count` of them) of a (request, head) that a CTA has to join: into the output, or (first: the first
+// of two rounds) into the place of part i0, with maximum and sum in a place of their own, since other threads still read
+// part i0's.
+struct Join {
+    int count, i0, stride, first;
+};
+
+// Every thread reads the maxima and sums of its head for itself, beside the outputs: one trip to L2 for kAtOnce parts, no
 // barrier.
-template <int NB, bool FIRST>
-__device__ __forceinline__ void join_parts(const PagedArgs& a, const Segment& s, int i0, int stride, int count) {
-    constexpr int D = NB * 32, kAtOnce = 8;
+template <int NB>
+__device__ __forceinline__ void join_parts(const PagedArgs& a, const Segment& s, const Join& j) {
+    constexpr int D = NB * 32, kAtOnce = 4;
     const int lane = threadIdx.x & 31, quads = s.heads * (D / 4);
+#pragma unroll 1
     for (int x0 = (int)threadIdx.x - lane; x0 < quads; x0 += kWorkThreads) {
         const int x = min(x0 + lane, quads - 1), hh = x / (D / 4);
-        const float2* ml_in = reinterpret_cast<const float2*>(!FIRST && stride > 1 ? a.round_ml : a.part_ml) + hh;
+        const float2* ml_in = reinterpret_cast<const float2*>(j.stride > 1 ? a.round_ml : a.part_ml) + hh;
         const float4* out_in = reinterpret_cast<const float4*>(a.part_out) + x;
         Running r;
-        for (int i = 0; i < count; i += kAtOnce) {
+#pragma unroll 1
+        for (int i = 0; i < j.count; i += kAtOnce) {
             float4 v[kAtOnce];
             float2 ml[kAtOnce];
 #pragma unroll
-            for (int k = 0; k < kAtOnce; ++k)
-                if (i + k < count) {
-                    const unsigned at = part_at(s.cta0, i0 + (i + k) * stride);
-                    ml[k] = __ldcg(ml_in + at);
-                    v[k] = __ldcg(out_in + at * (D / 4));
-                }
-            float top = kNoScore;
+            for (int k = 0; k < kAtOnce; ++k) {   // (past the end: the last part again, with weight 0)
+                const unsigned at = part_at(s.cta0, j.i0 + min(i + k, j.count - 1) * j.stride);
+                ml[k] = __ldcg(ml_in + at);
+                v[k] = __ldcg(out_in + at * (D / 4));
+            }
+            float top = ml[0].x;
 #pragma unroll
-            for (int k = 0; k < kAtOnce; ++k)
-                if (i + k < count) top = fmaxf(top, ml[k].x);
+            for (int k = 1; k < kAtOnce; ++k) top = fmaxf(top, ml[k].x);
             r.raise(top);
 #pragma unroll
             for (int k = 0; k < kAtOnce; ++k)
-                if (i + k < count) r.add(ml[k].x, ml[k].y, v[k]);
+                if (i + k < j.count) r.add(ml[k].x, ml[k].y, v[k]);
         }
-        if constexpr (!FIRST) {
-            write_quad<NB>(a, s, x, x0 + lane < quads, r.O, r.L);
-        } else if (x0 + lane < quads) {
-            const unsigned at = part_at(s.cta0, i0);
+        const bool live = x0 + lane < quads;
+        if (!j.first) {
+            write_quad(a.out, a.out_dtype, quad_at<NB>(a, s, x), live, r.O, r.L, a.sign_mag);
+        } else if (live) {
+            const unsigned at = part_at(s.cta0, j.i0);
             reinterpret_cast<float4*>(a.part_out)[at * (D / 4) + x] = r.O;
             if (x % (D / 4) == 0) reinterpret_cast<float2*>(a.round_ml)[at + hh] = make_float2(r.M, r.L);
         }
@@ -376,63 +364,65 @@ __device__ __forceinline__ void finish(const PagedArgs& a, const Fragments& f, F
         if (!done) crossing[side] = c0;
         const int quads = s.heads * (D / 4);
         const size_t at = (size_t)(blockIdx.x * 2 + side) * kSegHeads;
+#pragma unroll 1
         for (int x0 = warp * 32; x0 < quads; x0 += kWorkThreads) {
             const int x = min(x0 + lane, quads - 1), hh = x / (D / 4);
             Running r;
+#pragma unroll 1
             for (unsigned m = mine; m != 0; m &= m - 1) r.M = fmaxf(r.M, f.m[__ffs(m) - 1][hh]);
+#pragma unroll 1
             for (unsigned m = mine; m != 0; m &= m - 1) {
                 const int c = __ffs(m) - 1;
                 r.add(f.m[c][hh], f.l[c][hh], quad(c, x));
             }
             if (done) {
-                write_quad<NB>(a, s, x, x0 + lane < quads, r.O, r.L);
+                write_quad(a.out, a.out_dtype, quad_at<NB>(a, s, x), x0 + lane < quads, r.O, r.L, a.sign_mag);
             } else if (x0 + lane < quads) {
                 reinterpret_cast<float4*>(a.part_out + at * D)[x] = r.O;
                 if (x % (D / 4) == 0) reinterpret_cast<float2*>(a.part_ml)[at + hh] = make_float2(r.M, r.L);
             }
         }
     }
-    // what crosses the CTA's ends: a first round of parts, if there are many, and the last one
-    unsigned* ticket[2];
-    int want[2], first[2], per[2];
-#pragma unroll
-    for (int side = 0; side < 2; ++side) {
-        ticket[side] = nullptr;
-        want[side] = first[side] = per[side] = 0;
-        if (crossing[side] >= 0) {
-            const Segment& s = f.seg[crossing[side]];
-            per[side] = parts_per_round(s.ctas);
-            if (per[side] < s.ctas) {
-                const int mine = (int)blockIdx.x - s.cta0;
-                first[side] = mine / per[side] * per[side];
-                want[side] = min(per[side], s.ctas - first[side]);
-                ticket[side] = a.tickets + kMaxCtas + (s.cta0 + first[side]) * 2 + (first[side] == 0 ? 1 : 0);
-            } else {
-                want[side] = s.ctas;
-                ticket[side] = a.tickets + s.cta0;
-            }
-        }
-    }
     if (crossing[0] < 0 && crossing[1] < 0) return;
+    // What crosses the CTA's ends: a first round of parts, if there are many, and the last one.  Warp 0 arrives for what crosses
+    // the beginning, warp 1 for the rest, after everything that the CTA's threads have written; the last one to arrive sees
+    // what the others have written and joins.
+    __shared__ Join s_join[2];
 #pragma unroll 1
     for (int round = 0; round < 2; ++round) {
-        const int won = arrive(ticket[0], want[0], ticket[1], want[1]);
-        bool again = false;
-#pragma unroll
-        for (int side = 0; side < 2; ++side) {
-            ticket[side] = nullptr;
-            if (!((won >> side) & 1)) continue;
-            const Segment& s = f.seg[crossing[side]];
-            const bool two = per[side] < s.ctas, last = !two || round == 1;
-            if (last) join_parts<NB, false>(a, s, 0, two ? per[side] : 1, two ? (s.ctas + per[side] - 1) / per[side] : s.ctas);
-            else {
-                join_parts<NB, true>(a, s, first[side], 1, want[side]);
-                ticket[side] = a.tickets + s.cta0;
-                want[side] = (s.ctas + per[side] - 1) / per[side];
-                again = true;
+        __syncthreads();
+        if (lane == 0 && warp < 2) {
+            const int c = warp == 0 ? crossing[0] : crossing[1];
+            Join j{0, 0, 1, 0};
+            if (c >= 0 && (round == 0 || s_join[warp].first)) {
+                const int parts = f.seg[c].ctas, cta0 = f.seg[c].cta0, per = parts_per_round(parts);
+                unsigned* ticket = a.tickets + cta0;
+                int want = parts;
+                if (per < parts && round == 0) {
+                    j.i0 = ((int)blockIdx.x - cta0) / per * per;
+                    j.first = 1;
+                    want = min(per, parts - j.i0);
+                    ticket = a.tickets + kMaxCtas + (cta0 + j.i0) * 2 + (j.i0 == 0 ? 1 : 0);
+                } else if (per < parts) {
+                    j.stride = per;
+                    want = (parts + per - 1) / per;
+                }
+                unsigned old;
+                asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;\n" : "=r"(old) : "l"(ticket) : "memory");
+                if (old == (unsigned)(want - 1)) {
+                    j.count = want;
+                    *ticket = 0u;   // ready for the next call
+                } else {
+                    j.first = 0;
+                }
             }
+            s_join[warp] = j;
         }
-        if (!again) break;
+        __syncthreads();
+#pragma unroll 1
+        for (int side = 0; side < 2; ++side)
+            if (s_join[side].count > 0) join_parts<NB>(a, f.seg[side == 0 ? crossing[0] : crossing[1]], s_join[side]);
+        if (!s_join[0].first && !s_join[1].first) return;
     }
 }
 
