@@ -5,12 +5,12 @@ The reference's caches hold one sequence each; its rows (src/cache/storage.rs) a
 of tokens, bit for bit as `block_quantize` packs them.  All arithmetic runs in the CUDA library; calls are ordered on the
 current stream of the tensors' device.
 """
-import ctypes
+import struct
 from dataclasses import dataclass
 
 import torch
 
-from ._lib import TqbPagedAttentionParams, TqbPagedLayer, TqbRopeParams, lib
+from ._lib import lib
 from .api import ALL_BLOCKS, TQB_ERR_UNSUPPORTED, DecodeOutput, DimensionMismatch, QuantNormMode, TqbRuntimeError, check
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -18,6 +18,13 @@ _TICKET_BYTES = 16384   # TQB_PAGED_TICKET_BYTES
 _INTERLEAVED, _NO_NORM, _POSITIONS_64 = 1, 2, 4
 _PLAN_STATUS = {1: "not enough free pages", 2: "a request's length is negative or beyond its block table",
                 3: "more new tokens than the plan's capacity"}
+# The C structures (tqb200.h), packed in one go for each call: these calls are short, and so is their way to the launch.
+_LAYER = struct.Struct("@4P6i")                 # tqb_paged_layer
+_ROPE = struct.Struct("@4P8q4P7if")             # tqb_rope_params
+_ATTEND = struct.Struct("@5PN2q5if")            # tqb_paged_attention_params
+
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _code(dt):
@@ -27,56 +34,67 @@ def _code(dt):
     return code
 
 
-def _call(device, fn, *args):
+def _call(index, fn, *args):
     """fn(*args, stream) with the tensors' device current."""
-    index = device.index
-    if index == torch.cuda.current_device():
-        check(fn(*args, torch.cuda.current_stream(index).cuda_stream))
+    if index == _current_device():
+        status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            check(fn(*args, torch.cuda.current_stream(index).cuda_stream))
+            status = fn(*args, _raw_stream(index))
+    if status:
+        check(status)
 
 
-def _want(name, t, dtype, shape, device):
-    """A dense tensor of this dtype and shape (None: any extent) on `device`."""
-    if t.dtype != dtype:
+def _device(name, t):
+    index = t.get_device()
+    if index < 0:
+        raise ValueError(f"{name}: expected a CUDA tensor")
+    return index
+
+
+def _want(name, t, dtype, shape, index):
+    """The address of a dense tensor of this dtype and shape on the device."""
+    if t.dtype is not dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
-    if t.dim() != len(shape) or any(s is not None and s != n for s, n in zip(shape, t.shape)):
+    if t.shape != shape:
         raise DimensionMismatch(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-    if t.device != device:
-        raise ValueError(f"{name}: expected a tensor on {device}, got {t.device}")
+    if t.get_device() != index:
+        raise ValueError(f"{name}: expected a tensor on cuda:{index}, got {t.device}")
     if not t.is_contiguous():
         raise ValueError(f"{name}: expected a contiguous tensor")
+    return t.data_ptr()
 
 
-def _cuda(name, t):
-    if not t.is_cuda:
-        raise ValueError(f"{name}: expected a CUDA tensor")
-    return t.device
-
-
-def _rows(name, t, heads, dim, device):
-    """A tensor [tokens, heads, dim] whose rows the kernels can read where they lie, else a dense copy of it."""
-    if t.dim() != 3 or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
-        raise DimensionMismatch(f"{name}: expected shape (tokens, {heads or 'heads'}, {dim}), got {tuple(t.shape)}")
-    if t.device != device:
-        raise ValueError(f"{name}: expected a tensor on {device}, got {t.device}")
-    s0, s1, s2 = t.stride()
-    e = 16 // t.element_size()
-    if s2 != 1 or s0 % e or s1 % e or t.data_ptr() % 16:
+def _rows(name, t, shape, index):
+    """(tensor, address, token stride, head stride) of rows [tokens, heads, dim]: where they lie if the kernels can read them
+    there, else of a dense copy."""
+    if t.shape != shape:
+        raise DimensionMismatch(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.get_device() != index:
+        raise ValueError(f"{name}: expected a tensor on cuda:{index}, got {t.device}")
+    at, (s0, s1, s2), e = t.data_ptr(), t.stride(), 16 // t.element_size()
+    if s2 != 1 or s0 % e or s1 % e or at % 16:
         t = t.clone(memory_format=torch.contiguous_format)
-    return t
+        at, (s0, s1, s2) = t.data_ptr(), t.stride()
+    return t, at, s0, s1
 
 
-def _out_rows(name, t, like, device):
-    if t.dtype != like.dtype or t.shape != like.shape:
+def _out_rows(name, t, like, index):
+    """(address, token stride, head stride) of rows to be written."""
+    if t.dtype is not like.dtype or t.shape != like.shape:
         raise DimensionMismatch(f"{name}: expected {like.dtype} of shape {tuple(like.shape)}")
-    if t.device != device:
-        raise ValueError(f"{name}: expected a tensor on {device}, got {t.device}")
-    s0, s1, s2 = t.stride()
-    e, (n, h, d) = 16 // t.element_size(), t.shape
-    if s2 != 1 or s0 % e or s1 % e or t.data_ptr() % 16 or (h > 1 and s1 < d) or (n > 1 and s0 < (h - 1) * s1 + d):
+    if t.get_device() != index:
+        raise ValueError(f"{name}: expected a tensor on cuda:{index}, got {t.device}")
+    at, (s0, s1, s2), e, (n, h, d) = t.data_ptr(), t.stride(), 16 // t.element_size(), t.shape
+    if s2 != 1 or s0 % e or s1 % e or at % 16 or (h > 1 and s1 < d) or (n > 1 and s0 < (h - 1) * s1 + d):
         raise ValueError(f"{name}: rows must be dense, 16-byte aligned and apart from one another")
+    return at, s0, s1
+
+
+def _three(name, t):
+    if t.dim() != 3:
+        raise DimensionMismatch(f"{name}: expected [tokens, heads, dim], got {tuple(t.shape)}")
+    return t.shape
 
 
 # ---------------------------------------------------------------------------------------
@@ -101,14 +119,14 @@ class PagedStep:
             raise err
 
 
-def _plan_shapes(seq_lens, block_table, free_pages, state):
-    dev = _cuda("seq_lens", seq_lens)
-    n = seq_lens.shape[0] if seq_lens.dim() == 1 else -1
-    _want("seq_lens", seq_lens, torch.int32, (None,), dev)
-    _want("block_table", block_table, torch.int32, (n, None), dev)
-    _want("free_pages", free_pages, torch.int32, (None,), dev)
-    _want("state", state, torch.int32, (4,), dev)
-    return dev, n
+def _plan_args(seq_lens, block_table, free_pages, state):
+    index = _device("seq_lens", seq_lens)
+    if seq_lens.dim() != 1 or block_table.dim() != 2 or free_pages.dim() != 1:
+        raise DimensionMismatch("expected seq_lens [requests], block_table [requests, blocks] and free_pages [pages]")
+    n, blocks = seq_lens.shape[0], block_table.shape[1]
+    i32 = torch.int32
+    return (index, n, blocks, _want("seq_lens", seq_lens, i32, (n,), index), _want("block_table", block_table, i32, (n, blocks), index),
+            _want("free_pages", free_pages, i32, free_pages.shape, index), _want("state", state, i32, (4,), index))
 
 
 def paged_plan(seq_lens, new_tokens, block_table, free_pages, state, page_size, capacity, kv_lens=None, state_out=None):
@@ -117,37 +135,39 @@ def paged_plan(seq_lens, new_tokens, block_table, free_pages, state, page_size, 
     seq_lens, new_tokens [requests], block_table [requests, blocks] (new entries are written in place), free_pages and
     state int32; the first state[0] entries of free_pages are the free pages.  kv_lens and state_out are made new unless
     given; they may be seq_lens and state themselves.  Returns a PagedStep; `check()` on it says whether the step fitted."""
-    dev, n = _plan_shapes(seq_lens, block_table, free_pages, state)
-    _want("new_tokens", new_tokens, torch.int32, (n,), dev)
+    index, n, blocks, seq, table, free, st = _plan_args(seq_lens, block_table, free_pages, state)
+    new = _want("new_tokens", new_tokens, torch.int32, (n,), index)
     if capacity < 0:
         raise ValueError("capacity must not be negative")
-    slots = torch.empty(capacity, dtype=torch.int64, device=dev)
-    positions = torch.empty(capacity, dtype=torch.int32, device=dev)
-    cu = torch.empty(n + 1, dtype=torch.int32, device=dev)
+    slots = torch.empty(capacity, dtype=torch.int64, device=seq_lens.device)
+    made = seq_lens.new_empty(capacity + n + 1 + (n if kv_lens is None else 0) + (4 if state_out is None else 0))
+    parts = [capacity, n + 1]
     if kv_lens is None:
-        kv_lens = torch.empty(n, dtype=torch.int32, device=dev)
+        parts.append(n)
     else:
-        _want("kv_lens", kv_lens, torch.int32, (n,), dev)
+        _want("kv_lens", kv_lens, torch.int32, (n,), index)
     if state_out is None:
-        state_out = torch.empty(4, dtype=torch.int32, device=dev)
+        parts.append(4)
     else:
-        _want("state_out", state_out, torch.int32, (4,), dev)
-    blocks = block_table.shape[1]
-    _call(dev, lib.tqb_paged_plan, seq_lens.data_ptr(), new_tokens.data_ptr(), n, block_table.data_ptr(), blocks, blocks,
-          free_pages.data_ptr(), state.data_ptr(), page_size, slots.data_ptr(), positions.data_ptr(), capacity, cu.data_ptr(),
-          kv_lens.data_ptr(), state_out.data_ptr())
+        _want("state_out", state_out, torch.int32, (4,), index)
+    parts = list(made.split_with_sizes(parts))
+    positions, cu = parts[0], parts[1]
+    if state_out is None:
+        state_out = parts.pop()
+    if kv_lens is None:
+        kv_lens = parts.pop()
+    _call(index, lib.tqb_paged_plan, seq, new, n, table, blocks, blocks, free, st, page_size, slots.data_ptr(), positions.data_ptr(),
+          capacity, cu.data_ptr(), kv_lens.data_ptr(), state_out.data_ptr())
     return PagedStep(slots, positions, cu, kv_lens, state_out)
 
 
 def paged_release(mask, seq_lens, block_table, free_pages, state, page_size):
     """Gives the pages of the requests with mask[r] back to free_pages (tqb_paged_release): in place."""
-    dev, n = _plan_shapes(seq_lens, block_table, free_pages, state)
-    if mask.dtype == torch.bool:
+    index, n, blocks, seq, table, free, st = _plan_args(seq_lens, block_table, free_pages, state)
+    if mask.dtype is torch.bool:
         mask = mask.view(torch.uint8)
-    _want("mask", mask, torch.uint8, (n,), dev)
-    blocks = block_table.shape[1]
-    _call(dev, lib.tqb_paged_release, mask.data_ptr(), seq_lens.data_ptr(), n, block_table.data_ptr(), blocks, blocks,
-          free_pages.data_ptr(), free_pages.shape[0], state.data_ptr(), page_size)
+    _call(index, lib.tqb_paged_release, _want("mask", mask, torch.uint8, (n,), index), seq, n, table, blocks, blocks, free,
+          free_pages.shape[0], st, page_size)
 
 
 # ---------------------------------------------------------------------------------------
@@ -160,65 +180,54 @@ class QkNormRope:
     for ones; norm=False leaves the norms out; interleaved rotates neighbouring elements together instead of halves."""
 
     def __init__(self, inv_freq, q_weight=None, k_weight=None, eps=1e-6, norm=True, interleaved=False):
-        self.device = _cuda("inv_freq", inv_freq)
-        _want("inv_freq", inv_freq, torch.float32, (None,), self.device)
+        self.index = _device("inv_freq", inv_freq)
+        if inv_freq.dim() != 1:
+            raise DimensionMismatch("inv_freq: expected [rot_dim / 2]")
+        self._freq = _want("inv_freq", inv_freq, torch.float32, inv_freq.shape, self.index)
         for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
             if w is not None:
-                _want(name, w, w.dtype, (None,), self.device)
                 _code(w.dtype)
-                if w.data_ptr() % 16:
-                    raise ValueError(f"{name}: expected a 16-byte aligned tensor")
+                if w.dim() != 1 or _want(name, w, w.dtype, w.shape, self.index) % 16:
+                    raise ValueError(f"{name}: expected a 16-byte aligned vector")
         self.inv_freq, self.q_weight, self.k_weight = inv_freq, q_weight, k_weight
         self.eps, self.norm, self.interleaved = float(eps), bool(norm), bool(interleaved)
+        self._rot = 2 * inv_freq.shape[0]
+        self._flags = (_INTERLEAVED if self.interleaved else 0) | (0 if self.norm else _NO_NORM)
 
-    def _params(self, q, k, positions):
-        """The argument block for q, k (either may be None) without outputs."""
-        x = q if q is not None else k
-        n, d, dt = x.shape[0], x.shape[2], x.dtype
-        p = TqbRopeParams()
-        p.dtype, p.num_tokens, p.head_dim, p.eps = _code(dt), n, d, self.eps
-        p.rot_dim = 2 * self.inv_freq.shape[0]
-        flags = (_INTERLEAVED if self.interleaved else 0) | (0 if self.norm else _NO_NORM)
-        if p.rot_dim:
-            if positions.dtype == torch.int64:
+    def _weight(self, name, w, dt, d):
+        if w is None or not self.norm:
+            return None
+        if w.dtype is not dt or w.shape[0] != d:
+            raise DimensionMismatch(f"{name}: expected {dt} of length {d}, got {w.dtype} of length {w.shape[0]}")
+        return w.data_ptr()
+
+    def _params(self, q, q_out, k, k_out, n, hq, hkv, d, dt, positions):
+        """The argument block; q .. k_out are (address, token stride, head stride)."""
+        flags, at = self._flags, 0
+        if self._rot:
+            if positions.dtype is torch.int64:
                 flags |= _POSITIONS_64
-            elif positions.dtype != torch.int32:
+            elif positions.dtype is not torch.int32:
                 raise TypeError(f"positions: expected int32 or int64, got {positions.dtype}")
-            _want("positions", positions, positions.dtype, (n,), self.device)
-            p.positions, p.inv_freq = positions.data_ptr(), self.inv_freq.data_ptr()
-        p.flags = flags
-        for w, name in ((self.q_weight, "q_weight"), (self.k_weight, "k_weight")):
-            if w is not None and self.norm:
-                if w.dtype != dt or w.shape[0] != d:
-                    raise DimensionMismatch(f"{name}: expected {dt} of length {d}, got {w.dtype} of length {w.shape[0]}")
-                setattr(p, name, w.data_ptr())
-        if q is not None:
-            p.q, p.num_q_heads = q.data_ptr(), q.shape[1]
-            p.q_token_stride, p.q_head_stride, _ = q.stride()
-        if k is not None:
-            if k.dtype != dt or k.shape[0] != n:
-                raise DimensionMismatch(f"k: expected {dt} with {n} tokens, got {k.dtype} with {k.shape[0]}")
-            p.k, p.num_kv_heads = k.data_ptr(), k.shape[1]
-            p.k_token_stride, p.k_head_stride, _ = k.stride()
-        return p
+            at = _want("positions", positions, positions.dtype, (n,), self.index)
+        wq, wk = self._weight("q_weight", self.q_weight, dt, d), self._weight("k_weight", self.k_weight, dt, d)
+        return _ROPE.pack(q[0], q_out[0], k[0], k_out[0], q[1], q[2], q_out[1], q_out[2], k[1], k[2], k_out[1], k_out[2], wq or 0, wk or 0, at,
+                          self._freq, n, hq, hkv, d, self._rot, _code(dt), flags, self.eps)
 
     def __call__(self, q, k, positions, q_out=None, k_out=None):
         """q [tokens, query heads, dim], k [tokens, KV heads, dim] -> (q_out, k_out); the outputs may be q and k themselves."""
-        d = q.shape[-1]
-        qi, ki = _rows("q", q, None, d, self.device), _rows("k", k, None, d, self.device)
-        p = self._params(qi, ki, positions)
+        index, dt = self.index, q.dtype
+        n, hq, d = _three("q", q)
+        hkv = _three("k", k)[1]
+        if k.dtype is not dt:
+            raise DimensionMismatch(f"k: expected {dt}, got {k.dtype}")
+        qi, ki = _rows("q", q, q.shape, index), _rows("k", k, (n, hkv, d), index)
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-        else:
-            _out_rows("q_out", q_out, q, self.device)
+            q_out = q.new_empty((n, hq, d))
         if k_out is None:
-            k_out = torch.empty(k.shape, dtype=k.dtype, device=self.device)
-        else:
-            _out_rows("k_out", k_out, k, self.device)
-        p.q_out, p.k_out = q_out.data_ptr(), k_out.data_ptr()
-        p.q_out_token_stride, p.q_out_head_stride, _ = q_out.stride()
-        p.k_out_token_stride, p.k_out_head_stride, _ = k_out.stride()
-        _call(self.device, lib.tqb_qk_norm_rope, ctypes.byref(p))
+            k_out = q.new_empty((n, hkv, d))
+        _call(index, lib.tqb_qk_norm_rope, self._params(qi[1:], _out_rows("q_out", q_out, q, index), ki[1:], _out_rows("k_out", k_out, k, index),
+                                                        n, hq, hkv, d, dt, positions))
         return q_out, k_out
 
 
@@ -230,66 +239,58 @@ class PagedLayer:
     v_scales [pages, KV heads, page_size, head_dim / 32] int16 (f16 bits).  The tensors stay the caller's."""
 
     def __init__(self, k_indices, k_scales, v_indices, v_scales, bits):
-        dev = _cuda("k_indices", k_indices)
+        self.index = _device("k_indices", k_indices)
         if k_indices.dim() != 4 or k_scales.dim() != 4:
             raise DimensionMismatch("expected arrays [pages, KV heads, page_size, ...]")
         pages, heads, page, _ = k_indices.shape
         dim = 32 * k_scales.shape[3]
-        for name, t in (("k_indices", k_indices), ("v_indices", v_indices)):
-            _want(name, t, torch.uint8, (pages, heads, page, dim * bits // 8), dev)
-        for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
-            _want(name, t, torch.int16, (pages, heads, page, dim // 32), dev)
+        codes, blocks = (pages, heads, page, dim * bits // 8), (pages, heads, page, dim // 32)
+        self._c = _LAYER.pack(_want("k_indices", k_indices, torch.uint8, codes, self.index), _want("k_scales", k_scales, torch.int16, blocks, self.index),
+                              _want("v_indices", v_indices, torch.uint8, codes, self.index), _want("v_scales", v_scales, torch.int16, blocks, self.index),
+                              pages, heads, page, dim, bits, 0)
         self.tensors = (k_indices, k_scales, v_indices, v_scales)
-        self.device, self.bits, self.head_dim = dev, bits, dim
+        self.device, self.bits, self.head_dim = k_indices.device, bits, dim
         self.num_pages, self.num_kv_heads, self.page_size = pages, heads, page
-        self._c = TqbPagedLayer(k_indices.data_ptr(), k_scales.data_ptr(), v_indices.data_ptr(), v_scales.data_ptr(), pages, heads, page,
-                                dim, bits, 0)
-        self._ref = ctypes.byref(self._c)
-        check(lib.tqb_paged_dequantize(self._ref, None, 0, None, None, 0, None))   # checks the description, launches nothing
+        check(lib.tqb_paged_dequantize(self._c, None, 0, None, None, 0, None))   # checks the description, launches nothing
 
     def _slots(self, slots, n):
-        _want("slots", slots, torch.int64, (n,), self.device)
-        return slots.data_ptr()
+        return _want("slots", slots, torch.int64, (n,), self.index)
+
+    def _kv(self, k, v):
+        n = k.shape[0]
+        shape = (n, self.num_kv_heads, self.head_dim)
+        if v.dtype is not k.dtype:
+            raise DimensionMismatch(f"k and v differ in dtype: {k.dtype}, {v.dtype}")
+        return n, _rows("k", k, shape, self.index), _rows("v", v, shape, self.index)
 
     def append(self, k, v, slots):
         """Packs k, v [tokens, KV heads, dim] into their slots; a slot of -1 leaves a token out."""
-        k = _rows("k", k, self.num_kv_heads, self.head_dim, self.device)
-        v = _rows("v", v, self.num_kv_heads, self.head_dim, self.device)
-        if v.dtype != k.dtype or v.shape != k.shape:
-            raise DimensionMismatch("k and v differ in dtype or shape")
-        n = k.shape[0]
-        sk, sv = k.stride(), v.stride()
-        _call(self.device, lib.tqb_paged_append, self._ref, k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1], _code(k.dtype),
-              self._slots(slots, n), n)
+        n, k, v = self._kv(k, v)
+        _call(self.index, lib.tqb_paged_append, self._c, k[1], k[2], k[3], v[1], v[2], v[3], _code(k[0].dtype), self._slots(slots, n), n)
 
     def append_rope(self, rope, q, k, v, positions, slots, q_out=None):
         """Norms and rotation of q and k (`rope`: a QkNormRope), the keys and v packed into their slots, in one launch.
         Returns the rotated queries."""
-        q = _rows("q", q, None, self.head_dim, self.device)
-        k = _rows("k", k, self.num_kv_heads, self.head_dim, self.device)
-        v = _rows("v", v, self.num_kv_heads, self.head_dim, self.device)
-        if v.dtype != k.dtype or v.shape != k.shape:
-            raise DimensionMismatch("k and v differ in dtype or shape")
-        if rope.device != self.device:
-            raise ValueError(f"rope: expected tensors on {self.device}, got {rope.device}")
-        p = rope._params(q, k, positions)
+        n, k, v = self._kv(k, v)
+        hq, d, index = _three("q", q)[1], self.head_dim, self.index
+        qi = _rows("q", q, (n, hq, d), index)
+        if q.dtype is not k[0].dtype:
+            raise DimensionMismatch(f"q and k differ in dtype: {q.dtype}, {k[0].dtype}")
+        if rope.index != index:
+            raise ValueError(f"rope: expected tensors on cuda:{index}, got cuda:{rope.index}")
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-        else:
-            _out_rows("q_out", q_out, q, self.device)
-        p.q_out = q_out.data_ptr()
-        p.q_out_token_stride, p.q_out_head_stride, _ = q_out.stride()
-        sv = v.stride()
-        _call(self.device, lib.tqb_paged_append_rope, self._ref, ctypes.byref(p), v.data_ptr(), sv[0], sv[1],
-              self._slots(slots, k.shape[0]))
+            q_out = q.new_empty((n, hq, d))
+        p = rope._params(qi[1:], _out_rows("q_out", q_out, q, index), k[1:], (0, 0, 0), n, hq, self.num_kv_heads, d, q.dtype, positions)
+        _call(index, lib.tqb_paged_append_rope, self._c, p, v[1], v[2], v[3], self._slots(slots, n))
         return q_out
 
     def dequantize(self, slots, dtype=torch.float32):
         """The rows at `slots`: (k, v) [n, KV heads, dim]; rows of zeros where a slot lies outside the pages."""
         n = slots.shape[0]
+        at = self._slots(slots, n)
         k = torch.empty((n, self.num_kv_heads, self.head_dim), dtype=dtype, device=self.device)
         v = torch.empty_like(k)
-        _call(self.device, lib.tqb_paged_dequantize, self._ref, self._slots(slots, n), n, k.data_ptr(), v.data_ptr(), _code(dtype))
+        _call(self.index, lib.tqb_paged_dequantize, self._c, at, n, k.data_ptr(), v.data_ptr(), _code(dtype))
         return k, v
 
     def attend_scratch(self, num_q_heads):
@@ -302,25 +303,25 @@ class PagedLayer:
     def attend(self, q, block_table, kv_lens, softmax_scale, out=None, scratch=None):
         """Attention of one new token of each request over its pages: q [requests, query heads, dim] -> the same shape.
         block_table [requests, blocks] and kv_lens [requests] int32; a request without tokens gets zeros."""
-        n, hq, d = q.shape
-        q = _rows("q", q, None, self.head_dim, self.device)
-        if q.stride(1) != d or (n > 1 and q.stride(0) < hq * d):
-            q = q.contiguous()
-        _want("block_table", block_table, torch.int32, (n, None), self.device)
-        _want("kv_lens", kv_lens, torch.int32, (n,), self.device)
+        index, d = self.index, self.head_dim
+        n, hq, _ = _three("q", q)
+        qi, at, s0, s1 = _rows("q", q, (n, hq, d), index)
+        if s1 != d or (n > 1 and s0 < hq * d):   # heads one behind the other
+            qi = qi.contiguous() if not qi.is_contiguous() else qi.clone()
+            at, s0 = qi.data_ptr(), hq * d
+        if block_table.dim() != 2:
+            raise DimensionMismatch(f"block_table: expected [requests, blocks], got {tuple(block_table.shape)}")
+        blocks = block_table.shape[1]
+        table = _want("block_table", block_table, torch.int32, (n, blocks), index)
+        lens = _want("kv_lens", kv_lens, torch.int32, (n,), index)
         if out is None:
-            out = torch.empty((n, hq, d), dtype=q.dtype, device=self.device)
-        else:
-            _want("out", out, out.dtype, (n, hq, d), self.device)
+            out = q.new_empty((n, hq, d))
+        to = _want("out", out, out.dtype, (n, hq, d), index)
         if scratch is None:
             scratch = self.attend_scratch(hq)
-        else:
-            _want("scratch", scratch, torch.uint8, (None,), self.device)
-        blocks = block_table.shape[1]
-        p = TqbPagedAttentionParams(q.data_ptr(), out.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), scratch.data_ptr(),
-                                    scratch.shape[0], q.stride(0) if n > 1 else 0, blocks, blocks, n, hq, _code(q.dtype),
-                                    _code(out.dtype), softmax_scale)
-        _call(self.device, lib.tqb_paged_attention, self._ref, ctypes.byref(p))
+        work = _want("scratch", scratch, torch.uint8, scratch.shape, index)
+        _call(index, lib.tqb_paged_attention, self._c, _ATTEND.pack(at, to, table, lens, work, scratch.numel(), s0 if n > 1 else 0, blocks, blocks,
+                                                                    n, hq, _code(q.dtype), _code(out.dtype), softmax_scale))
         return out
 
 
