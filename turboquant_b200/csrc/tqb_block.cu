@@ -9,6 +9,7 @@
 // stream (src/packed/mod.rs:242-309), which makes packing a lane-local shift/or plus one
 // shuffle for the 3-bit width.
 #include "tqb_common.cuh"
+#include "tqb_pqo_dequant.cuh"
 #include "tqb_pqo_quant.cuh"
 
 namespace tqb {
@@ -461,23 +462,15 @@ block_dequantize_kernel(DequantArgs a, Codebook normal, Codebook outlier) {
 template <typename T, int BITS>
 __global__ void __launch_bounds__(kThreads)
 block_dequantize_lane_kernel(DequantArgs a, Codebook cb) {
-    constexpr int kCodes = 1 << BITS, kTabB = kCodes * 128;       // bytes of one sign's table
     constexpr int kPitch = 32 * (int)sizeof(T) + 16;              // a lane's staged row: 16-byte pieces of 8 lanes in 32 banks
-    __shared__ __align__(2048) unsigned char s_tab[2 * kTabB];
+    __shared__ __align__(2048) unsigned char s_tab[2 * DequantTable<BITS>::kBytes];
     __shared__ __align__(16) unsigned char s_stage[kThreads * kPitch];
     const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int k = 0; k < kCodes * 32 / kThreads; ++k) {
-        const int i = (int)threadIdx.x + k * kThreads, code = i >> 5;
-        const float v = cb.c[code < cb.n ? code : cb.n - 1] * a.sign_mag;
-        reinterpret_cast<float*>(s_tab)[i] = v;
-        reinterpret_cast<float*>(s_tab)[i + kCodes * 32] = -v;
-    }
+    build_dequant_table<BITS>(cb, a.sign_mag, s_tab, threadIdx.x, kThreads);
     __syncthreads();
     const uint32_t tab = (uint32_t)__cvta_generic_to_shared(s_tab) + lane * 4;
     unsigned char* stage = s_stage + (threadIdx.x >> 5) * 32 * kPitch;
     const unsigned total = (unsigned)(a.n_rows * a.nblk), nblk = (unsigned)a.nblk;
-    const F2 inv_sqrt = f2(1.0f / sqrtf((float)kBlock));
     for (unsigned blk0 = (blockIdx.x * kThreads + threadIdx.x) & ~31u; blk0 < total; blk0 += gridDim.x * kThreads) {
         const unsigned blk = min(blk0 + lane, total - 1);
         size_t sblk = blk;
@@ -495,25 +488,7 @@ block_dequantize_lane_kernel(DequantArgs a, Codebook cb) {
         }
         const F2 as = f2(fabsf(f16_bits_to_f32(__ldg(a.scales + sblk))));
         float v[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            // the code moved to bits 7.. (its row of 128 bytes), the lane's bank below it
-            const int k = (BITS * i) >> 5, sh = (BITS * i) & 31;
-            const uint32_t m = sh < 7 ? w[k] << (7 - sh) : (sh + BITS <= 32 ? w[k] >> (sh - 7) : __funnelshift_r(w[k], w[k < 3 ? k + 1 : 3], sh - 7));
-            const uint32_t addr = (m & ((kCodes - 1) << 7)) | tab;
-            if ((kSignMask >> i) & 1u) asm("ld.shared.f32 %0, [%1+%2];" : "=f"(v[i]) : "r"(addr), "n"(kTabB) : "memory");
-            else asm("ld.shared.f32 %0, [%1];" : "=f"(v[i]) : "r"(addr) : "memory");
-        }
-        F2 p[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) p[i] = f2(v[i], v[i + 16]);
-        butterfly32_pairs(p);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float2 t = halves(mul2(mul2(p[i], inv_sqrt), as));
-            v[i] = t.x;
-            v[i + 16] = t.y;
-        }
+        dequantize_values<BITS>(w, as, tab, v);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             float e[8];

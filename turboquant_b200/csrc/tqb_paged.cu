@@ -2,6 +2,7 @@
 // and the rows that come back from them.  The attention over the pages is in tqb_paged_attention.cu.
 #include "tqb_common.cuh"
 #include "tqb_paged.cuh"
+#include "tqb_pqo_dequant.cuh"
 #include "tqb_pqo_quant.cuh"
 
 namespace tqb {
@@ -192,11 +193,14 @@ __global__ void __launch_bounds__(kReleaseThreads) release_kernel(const uint8_t*
 }
 
 // ---- rows into pages, with norm and rotation ---------------------------------------------------------------------------
-// One warp pass takes 32 / (D / 8) heads of a token, eight consecutive elements a lane: every load and store of a warp is
-// dense, the norm's sum and the partner of a rotated pair are shuffles away, and the 32-point butterfly runs stages 1, 2, 4
-// in the lane and 8, 16 between lanes - the operand pairs of the scalar butterfly, so the codes are those of
-// tqb_block_quantize.  The angles of a token are computed once per CTA: position * inv_freq in f64, less whole turns, then
-// sincosf in f32 (an f32 product would be off by position * 2^-24, 0.06 rad at a million tokens).
+// A CTA takes kRowTokens tokens at a time (one, where there are few).
+// Angles: position * inv_freq in f64, less whole turns, then sincosf in f32 (an f32 product would be off by position * 2^-24,
+//   0.06 rad at a million tokens), once for a token.
+// Rows: one warp pass takes 32 / (D / 8) heads of a token, eight consecutive elements a lane: every load and store of a warp is
+//   dense, the norm's sum and the partner of a rotated pair are shuffles away.  The next pass's loads are in flight.  Queries
+//   leave for q_out; keys and values go to a tile of 32-blocks in shared memory, in their type.
+// Blocks: one thread packs one 32-block of the tile as tqb_block_quantize does (pqo_quantize_values), 16 or 12 bytes of codes.
+//   Four lanes a block with the butterfly's last stages as shuffles needs three times the instructions.
 constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32;
 
@@ -215,7 +219,7 @@ struct RowArgs {
     uint8_t* idx[2];        // K, V
     uint16_t* sc[2];
     long long num_slots;
-    int tokens, rot_dim, flags, kv_heads, page_shift;
+    int tokens, chunk, rot_dim, flags, kv_heads, page_shift;   // chunk: tokens that a CTA takes at a time
     float eps;
     float outer_centroid;
 };
@@ -289,119 +293,83 @@ struct Eight<__half> {
     __device__ __forceinline__ void store(__half* p) const { *reinterpret_cast<uint4*>(p) = r; }
 };
 
-// The block's 32 values, eight a lane in four neighbouring lanes (quarter: lane & 3) -> this lane's eight codes in the low
-// 8 * BITS bits; returns the scale.  Arithmetic and results of pqo_quantize_values.
-template <int BITS>
-__device__ __forceinline__ float quantize8(float (&v)[8], int quarter, const Codebook& cb, float outer_centroid, uint32_t& codes) {
+constexpr int kRowTokens = 4;
+
+template <typename T>
+struct Tile {
+    static constexpr int kPitch = 32 * (int)sizeof(T) + 16;   // of a 32-block: 16-byte pieces of eight lanes in 32 banks
+};
+template <typename T>
+__device__ __forceinline__ void load_tile(const unsigned char* p, float (&v)[32]) {
 #pragma unroll
-    for (int h = 1; h < 8; h <<= 1)
+    for (int k = 0; k < 4; ++k) {
+        Eight<T> e;
+        e.load(reinterpret_cast<const T*>(p) + 8 * k);
+        float x[8];
+        e.get(x);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if ((i & h) == 0) {
-                const float x = v[i], y = v[i + h];
-                v[i] = x + y;
-                v[i + h] = x - y;
-            }
-#pragma unroll
-    for (int m = 1; m <= 2; m <<= 1) {
-        const bool upper = (quarter & m) != 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float other = __shfl_xor_sync(0xffffffffu, v[i], m);
-            v[i] = upper ? (other - v[i]) : (v[i] + other);
-        }
+        for (int i = 0; i < 8; ++i) v[8 * k + i] = x[i];
     }
-    const float inv_sqrt = 1.0f / sqrtf((float)kBlock);
-    float amax = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[i]));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2)) * inv_sqrt;
-    const float raw = __fdiv_rn(amax, outer_centroid);
-    const float scale = raw > kMinNorm ? raw : kMinNorm;
-    const float r = __frcp_rn(scale);
-    const uint32_t neg = kSignMask >> (8 * quarter);
-    codes = 0u;
-    if (BITS == 4) {
-        const float inv_step = 15.0f / (2.0f * cb.c[15]);
-        const float cpos = (inv_sqrt * r) * inv_step;
-        const float kMagic = 12582912.0f;   // 1.5 * 2^23
-        float far = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float u = fmaf(v[i], ((neg >> i) & 1u) ? -cpos : cpos, 7.5f);
-            const float m = u + kMagic;
-            far = fmaxf(far, fabsf(u - (m - kMagic)));
-            codes |= (__float_as_uint(m) & 15u) << (4 * i);
-        }
-        if (far > 0.49998f) {   // rare: exact division and the f32 boundary table
-            codes = 0u;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float t = __fdiv_rn((v[i] * inv_sqrt) * (((neg >> i) & 1u) ? -1.0f : 1.0f), scale);
-                uint32_t c = 0;
-#pragma unroll
-                for (int k = 0; k < 15; ++k) c += (t > cb.b[k]) ? 1u : 0u;
-                codes |= c << (4 * i);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float rot = (v[i] * inv_sqrt) * (((neg >> i) & 1u) ? -1.0f : 1.0f);
-            // rot / scale, correctly rounded: the quotient corrected by its remainder (Markstein, IBM J. Res. Dev. 34, 1990)
-            const float q = rot * r;
-            const float t = fmaf(fmaf(q, -scale, rot), r, q);
-            uint32_t c = 0;
-#pragma unroll
-            for (int k = 0; k < 7; ++k) c += (t > cb.b[k]) ? 1u : 0u;
-            codes |= c << (3 * i);
-        }
-    }
-    return scale;
 }
 
 template <typename T, int LPH, int BITS>
-__global__ void __launch_bounds__(kRowThreads) rows_kernel(const __grid_constant__ RowArgs a, const __grid_constant__ Codebook cb) {
-    constexpr int D = LPH * 8, HPW = 32 / LPH;
-    __shared__ __align__(16) float2 s_cs[2][D / 2];
+__global__ void __launch_bounds__(kRowThreads, BITS == 0 ? 4 : 3) rows_kernel(const __grid_constant__ RowArgs a, const __grid_constant__ Codebook cb) {
+    constexpr int D = LPH * 8, HPW = 32 / LPH, NB = D / 32;
+    extern __shared__ __align__(16) unsigned char s_tile[];   // BITS != 0: [token][K, V][head][block]
+    __shared__ __align__(16) float2 s_cs[kRowTokens][D / 2];
+    __shared__ float2 s_cells[BITS == 3 ? kCells * 32 : 1];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int sub = lane / LPH, l = lane % LPH;
     const int half = a.rot_dim >> 1;
     const bool inter = (a.flags & TQB_ROPE_INTERLEAVED) != 0, norm = (a.flags & TQB_ROPE_NO_NORM) == 0;
-    const int heads = a.q.heads + a.k.heads + a.v.heads;
-    int par = 0;
-    for (int t = blockIdx.x; t < a.tokens; t += gridDim.x, par ^= 1) {
-        if (half > 0) {
-            if (tid < half) {
-                const double pos = (a.flags & TQB_ROPE_POSITIONS_64) ? (double)reinterpret_cast<const long long*>(a.positions)[t]
-                                                                    : (double)reinterpret_cast<const int*>(a.positions)[t];
-                const double ang = pos * (double)a.inv_freq[tid];
-                const double turns = rint(ang * 0.15915494309189535);
-                float si, co;
-                sincosf((float)fma(turns, -6.283185307179586, ang), &si, &co);
-                s_cs[par][tid] = make_float2(co, si);
-            }
-            __syncthreads();   // one barrier a token: the other half of s_cs is free again when the next but one writes it
-        }
-        long long slot = -1;
-        size_t page = 0;
-        int in_page = 0;
-        if (BITS != 0) {
-            slot = a.slots[t];
-            if (slot >= a.num_slots) slot = -1;
-            page = (size_t)(slot >> a.page_shift);
-            in_page = (int)(slot & ((1 << a.page_shift) - 1));
-        }
-        for (int g = warp; g * HPW < heads; g += kRowWarps) {
-            const bool live = g * HPW + sub < heads;
+    const int heads = a.q.heads + a.k.heads + a.v.heads, groups = (heads + HPW - 1) / HPW;
+    if (BITS == 3) build_cell_table(cb, cb.n - 1, s_cells, tid, kRowThreads);
+    for (int t0 = blockIdx.x * a.chunk; t0 < a.tokens; t0 += gridDim.x * a.chunk) {
+        const int nt = min(a.chunk, a.tokens - t0);
+        // the lane's row of pass (token tok, group g)
+        auto span_of = [&](int g, int& h) -> const RowSpan& {
             const int hd = min(g * HPW + sub, heads - 1);
             const int kind = hd < a.q.heads ? 0 : hd < a.q.heads + a.k.heads ? 1 : 2;
-            const RowSpan& s = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-            const int h = kind == 0 ? hd : kind == 1 ? hd - a.q.heads : hd - a.q.heads - a.k.heads;
+            h = kind == 0 ? hd : kind == 1 ? hd - a.q.heads : hd - a.q.heads - a.k.heads;
+            return kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+        };
+        auto fetch = [&](int tok, int g, Eight<T>& e) {
+            int h;
+            const RowSpan& s = span_of(g, h);
+            e.load(reinterpret_cast<const T*>(s.in) + (t0 + tok) * s.in_token + h * s.in_head + 8 * l);
+        };
+        auto advance = [&](int& tok, int& g) {
+            g += kRowWarps;
+            while (g >= groups) {
+                g -= groups;
+                ++tok;
+            }
+        };
+        int tok = 0, g = warp - kRowWarps;
+        advance(tok, g);
+        Eight<T> ahead;
+        if (tok < nt) fetch(tok, g, ahead);
+        for (int i = tid; i < nt * half; i += kRowThreads) {
+            const int t = i / half, f = i - t * half;
+            const double pos = (a.flags & TQB_ROPE_POSITIONS_64) ? (double)reinterpret_cast<const long long*>(a.positions)[t0 + t]
+                                                                : (double)reinterpret_cast<const int*>(a.positions)[t0 + t];
+            const double ang = pos * (double)a.inv_freq[f];
+            const double turns = rint(ang * 0.15915494309189535);
+            float si, co;
+            sincosf((float)fma(turns, -6.283185307179586, ang), &si, &co);
+            s_cs[t][f] = make_float2(co, si);
+        }
+        __syncthreads();
+        while (tok < nt) {
+            const int this_tok = tok, this_g = g;
+            Eight<T> e = ahead;
+            advance(tok, g);
+            if (tok < nt) fetch(tok, g, ahead);
+            int h;
+            const RowSpan& s = span_of(this_g, h);
+            const bool live = this_g * HPW + sub < heads;
+            const int hd = min(this_g * HPW + sub, heads - 1), kind = hd < a.q.heads ? 0 : hd < a.q.heads + a.k.heads ? 1 : 2;
             float v[8];
-            Eight<T> e;
-            e.load(reinterpret_cast<const T*>(s.in) + t * s.in_token + h * s.in_head + 8 * l);
             e.get(v);
             // the shuffles below are done by all lanes, whichever tensor their head is of
             if (norm) {
@@ -428,53 +396,70 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const __grid_constant
             if (half > 0) {
                 if (inter) {
                     if (kind != 2 && 8 * l < a.rot_dim) {
+                        const float4* cs = reinterpret_cast<const float4*>(&s_cs[this_tok][4 * l]);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float2 cs = s_cs[par][4 * l + i];
-                            const float x = v[2 * i], y = v[2 * i + 1];
-                            v[2 * i] = fmaf(x, cs.x, -(y * cs.y));
-                            v[2 * i + 1] = fmaf(y, cs.x, x * cs.y);
+                        for (int i = 0; i < 2; ++i) {
+                            const float4 c = cs[i];   // (cos, sin) twice
+                            const float x0 = v[4 * i], y0 = v[4 * i + 1], x1 = v[4 * i + 2], y1 = v[4 * i + 3];
+                            v[4 * i] = fmaf(x0, c.x, -(y0 * c.y));
+                            v[4 * i + 1] = fmaf(y0, c.x, x0 * c.y);
+                            v[4 * i + 2] = fmaf(x1, c.z, -(y1 * c.w));
+                            v[4 * i + 3] = fmaf(y1, c.z, x1 * c.w);
                         }
                     }
                 } else {
                     const int hl = half >> 3;   // lanes of half a rotated row
                     const bool first = l < hl, turns = l < 2 * hl;
                     const int from = lane + (!turns ? 0 : first ? hl : -hl);
+                    const float4* cs = reinterpret_cast<const float4*>(&s_cs[this_tok][turns ? 8 * (first ? l : l - hl) : 0]);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float other = __shfl_sync(0xffffffffu, v[i], from);
+                    for (int i = 0; i < 4; ++i) {
+                        const float4 c = cs[i];
+                        const float o0 = __shfl_sync(0xffffffffu, v[2 * i], from), o1 = __shfl_sync(0xffffffffu, v[2 * i + 1], from);
                         if (kind != 2 && turns) {
-                            const float2 cs = s_cs[par][8 * (first ? l : l - hl) + i];
-                            v[i] = fmaf(v[i], cs.x, first ? -(other * cs.y) : other * cs.y);
+                            v[2 * i] = fmaf(v[2 * i], c.x, first ? -(o0 * c.y) : o0 * c.y);
+                            v[2 * i + 1] = fmaf(v[2 * i + 1], c.z, first ? -(o1 * c.w) : o1 * c.w);
                         }
                     }
                 }
             }
-            e.set(v);
-            if (live && s.out != nullptr) e.store(reinterpret_cast<T*>(s.out) + t * s.out_token + h * s.out_head + 8 * l);
-            if (BITS != 0) {
-                e.get(v);   // keys as their type holds them
-                uint32_t codes;
-                const float scale = quantize8<BITS == 0 ? 4 : BITS>(v, lane & 3, cb, a.outer_centroid, codes);
-                const uint32_t next = BITS == 3 ? __shfl_down_sync(0xffffffffu, codes, 1) : 0u;
-                if (live && kind != 0 && slot >= 0) {
-                    const size_t row = ((page * a.kv_heads + h) << a.page_shift) + in_page;
-                    uint32_t* wp = reinterpret_cast<uint32_t*>(a.idx[kind - 1] + row * (D / 8 * BITS));
-                    if (BITS == 4) {
-                        wp[l] = codes;
-                    } else {
-                        const int q = l & 3;   // four lanes' 24 bits make three words
-                        if (q < 3) wp[(l >> 2) * 3 + q] = (codes >> (8 * q)) | (next << (24 - 8 * q));
-                    }
-                    if ((l & 3) == 0) a.sc[kind - 1][row * (D / 32) + (l >> 2)] = f32_to_f16_bits(-scale);   // outlier blocks store -scale
+            if (kind != 2) e.set(v);
+            if (live && s.out != nullptr) e.store(reinterpret_cast<T*>(s.out) + (t0 + this_tok) * s.out_token + h * s.out_head + 8 * l);
+            if (BITS != 0 && live && kind != 0)
+                e.store(reinterpret_cast<T*>(s_tile + (size_t)(((this_tok * 2 + kind - 1) * a.kv_heads + h) * NB + (l >> 2)) * Tile<T>::kPitch) + 8 * (l & 3));
+        }
+        if constexpr (BITS != 0) {
+            __syncthreads();
+            const unsigned kv = (unsigned)a.kv_heads;
+            for (int i = tid; i < nt * 2 * a.kv_heads * NB; i += kRowThreads) {
+                const unsigned row = (unsigned)i / NB, ts = row / kv, h = row - ts * kv, b = (unsigned)i % NB;
+                const long long slot = a.slots[t0 + (ts >> 1)];
+                if (slot < 0 || slot >= a.num_slots) continue;
+                float v[32];
+                load_tile<T>(s_tile + (size_t)i * Tile<T>::kPitch, v);
+                uint32_t w[4];
+                const float scale = pqo_quantize_values<BITS>(v, cb, a.outer_centroid, w, BITS == 3 ? s_cells + lane : nullptr);
+                const int side = ts & 1;
+                const size_t at = (((((size_t)(slot >> a.page_shift) * kv + h) << a.page_shift) + (slot & ((1 << a.page_shift) - 1)))) * NB + b;
+                uint8_t* to = a.idx[side] + at * (4 * BITS);
+                if (BITS == 4) {
+                    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+                } else {
+                    uint32_t* wp = reinterpret_cast<uint32_t*>(to);
+                    wp[0] = w[0];
+                    wp[1] = w[1];
+                    wp[2] = w[2];
                 }
+                a.sc[side][at] = f32_to_f16_bits(-scale);   // outlier blocks store -scale
             }
         }
+        __syncthreads();   // angles and tile are free again
     }
 }
 
 // ---- rows back from pages ----------------------------------------------------------------------------------------------
-// Eight codes a lane like above; the values and their roundings are those of tqb_block_dequantize.  Bound: HBM (stores).
+// One lane a 32-block as in tqb_block_dequantize, whose values these are; the warp's 32 blocks leave through shared memory as
+// dense 512-byte stores, and the next blocks' codes are in flight.  Bound: HBM, mostly the stores.
 struct BackArgs {
     const uint8_t* idx[2];
     const uint16_t* sc[2];
@@ -485,70 +470,62 @@ struct BackArgs {
     float sign_mag;
 };
 
-template <typename T, int LPH, int BITS>
+template <typename T, int NB, int BITS>
 __global__ void __launch_bounds__(kRowThreads) back_kernel(const __grid_constant__ BackArgs a, const __grid_constant__ Codebook cb) {
-    constexpr int D = LPH * 8, HPW = 32 / LPH, kCodes = 1 << BITS;
-    __shared__ float s_tab[kCodes][32];   // a copy of the codebook for each bank
-    const int tid = threadIdx.x, lane = tid & 31;
-    const int sub = lane / LPH, l = lane % LPH;
-    for (int i = tid; i < kCodes * 32; i += kRowThreads) s_tab[i >> 5][i & 31] = cb.c[i >> 5] * a.sign_mag;
+    constexpr int kPitch = Tile<T>::kPitch, kPieces = 2 * (int)sizeof(T);   // 16-byte pieces of a block
+    __shared__ __align__(2048) unsigned char s_tab[2 * DequantTable<BITS>::kBytes];
+    __shared__ __align__(16) unsigned char s_stage[kRowThreads * kPitch];
+    const int tid = threadIdx.x, lane = tid & 31, side = blockIdx.y;
+    build_dequant_table<BITS>(cb, a.sign_mag, s_tab, tid, kRowThreads);
     __syncthreads();
-    const float inv_sqrt = 1.0f / sqrtf((float)kBlock);
-    const uint32_t neg = kSignMask >> (8 * (lane & 3));
-    const int side = blockIdx.y;
+    const uint32_t tab = (uint32_t)__cvta_generic_to_shared(s_tab) + lane * 4;
+    unsigned char* stage = s_stage + (tid >> 5) * 32 * kPitch;
     const unsigned kv = (unsigned)a.kv_heads;
-    const long long rows = a.n * kv, step = (long long)gridDim.x * kRowWarps * HPW;
-    for (long long r0 = ((long long)blockIdx.x * kRowWarps + (tid >> 5)) * HPW; r0 < rows; r0 += step) {
-        const long long r = min(r0 + sub, rows - 1), tok = r / kv;
-        const int h = (int)(r - tok * kv);
+    const long long total = a.n * kv * NB, step = (long long)gridDim.x * kRowThreads;
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+    float scale = 0.0f;
+    bool in = false;
+    auto fetch = [&](long long blk0) {
+        const long long blk = min(blk0 + lane, total - 1), row = blk / NB, tok = row / kv;
         const long long slot = a.slots[tok];
-        const bool in = slot >= 0 && slot < a.num_slots;
-        float v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-        float as = 0.0f;
-        if (in) {
-            const size_t row = (((size_t)(slot >> a.page_shift) * kv + h) << a.page_shift) + (slot & ((1 << a.page_shift) - 1));
-            const uint32_t* wp = reinterpret_cast<const uint32_t*>(a.idx[side] + row * (D / 8 * BITS));
-            uint32_t w;
-            if (BITS == 4) {
-                w = __ldg(wp + l);
-            } else {
-                const int k = (3 * l) >> 2;
-                w = __funnelshift_r(__ldg(wp + k), __ldg(wp + min(k + 1, D * BITS / 32 - 1)), (24 * l) & 31);
-            }
-            as = fabsf(f16_bits_to_f32(__ldg(a.sc[side] + row * (D / 32) + (l >> 2))));
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float c = s_tab[(w >> (BITS * i)) & (kCodes - 1)][lane];
-                v[i] = ((neg >> i) & 1u) ? -c : c;
-            }
+        in = slot >= 0 && slot < a.num_slots;
+        if (!in) return;
+        const size_t at = (((((size_t)(slot >> a.page_shift) * kv + (size_t)(row - tok * kv)) << a.page_shift) + (slot & ((1 << a.page_shift) - 1)))) * NB + blk % NB;
+        const uint8_t* p = a.idx[side] + at * (4 * BITS);
+        if (BITS == 4) {
+            const uint4 r = __ldg(reinterpret_cast<const uint4*>(p));
+            w[0] = r.x; w[1] = r.y; w[2] = r.z; w[3] = r.w;
+        } else {
+            const uint32_t* q = reinterpret_cast<const uint32_t*>(p);
+            w[0] = __ldg(q); w[1] = __ldg(q + 1); w[2] = __ldg(q + 2);
         }
+        scale = fabsf(f16_bits_to_f32(__ldg(a.sc[side] + at)));
+    };
+    long long blk0 = ((long long)blockIdx.x * kRowThreads + tid) & ~31ll;
+    if (blk0 < total) fetch(blk0);
+    for (; blk0 < total; blk0 += step) {
+        float v[32];
+        dequantize_values<BITS>(w, f2(scale), tab, v);
+        const bool live = in;
+        if (blk0 + step < total) fetch(blk0 + step);
 #pragma unroll
-        for (int hh = 1; hh < 8; hh <<= 1)
+        for (int k = 0; k < 4; ++k) {
+            float e[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if ((i & hh) == 0) {
-                    const float x = v[i], y = v[i + hh];
-                    v[i] = x + y;
-                    v[i + hh] = x - y;
-                }
-#pragma unroll
-        for (int m = 1; m <= 2; m <<= 1) {
-            const bool upper = (lane & m) != 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float other = __shfl_xor_sync(0xffffffffu, v[i], m);
-                v[i] = upper ? (other - v[i]) : (v[i] + other);
-            }
+            for (int i = 0; i < 8; ++i) e[i] = live ? v[8 * k + i] : 0.0f;
+            Eight<T> x;
+            x.set(e);
+            x.store(reinterpret_cast<T*>(stage + lane * kPitch) + 8 * k);
         }
+        __syncwarp();
+        unsigned char* out = reinterpret_cast<unsigned char*>(a.out[side]) + (size_t)blk0 * (32 * sizeof(T));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = in ? (v[i] * inv_sqrt) * as : 0.0f;
-        if (r0 + sub < rows) {
-            Eight<T> e;
-            e.set(v);
-            e.store(reinterpret_cast<T*>(a.out[side]) + r * D + 8 * l);
+        for (int i = 0; i < kPieces; ++i) {
+            const int q = 32 * i + lane;
+            const uint4 r = *reinterpret_cast<const uint4*>(stage + (q / kPieces) * kPitch + (q % kPieces) * 16);
+            if (blk0 + q / kPieces < total) *reinterpret_cast<uint4*>(out + q * 16) = r;
         }
+        __syncwarp();
     }
 }
 
@@ -570,18 +547,26 @@ int check_rows(const void* p, long long token, long long head, size_t elem) {
     return TQB_OK;
 }
 
-template <typename T, int LPH>
-int launch_rows_bits(int bits, const RowArgs& a, const Codebook& cb, cudaStream_t s) {
-    const int grid = a.tokens < 148 * 8 ? a.tokens : 148 * 8;
-    switch (bits) {
-        case 0: rows_kernel<T, LPH, 0><<<grid, kRowThreads, 0, s>>>(a, cb); break;
-        case 3: rows_kernel<T, LPH, 3><<<grid, kRowThreads, 0, s>>>(a, cb); break;
-        default: rows_kernel<T, LPH, 4><<<grid, kRowThreads, 0, s>>>(a, cb); break;
-    }
+template <typename T, int LPH, int BITS>
+int launch_rows_one(RowArgs& a, const Codebook& cb, cudaStream_t s) {
+    // One token a CTA while that leaves SMs idle, and while more would not fit.
+    const size_t token = BITS == 0 ? 0 : (size_t)2 * a.kv_heads * (LPH / 4) * Tile<T>::kPitch;
+    a.chunk = a.tokens < 148 * kRowTokens ? 1 : kRowTokens;
+    while (a.chunk > 1 && token * a.chunk > 64 * 1024) a.chunk >>= 1;
+    if (token > 160 * 1024) return TQB_ERR_UNSUPPORTED;   // KV heads x head_dim beyond 64 x 256 (16-bit)
+    const int bytes = (int)(token * a.chunk);
+    if (int st = allow_shared<rows_kernel<T, LPH, BITS>>(bytes, 160 * 1024)) return st;
+    const int want = (a.tokens + a.chunk - 1) / a.chunk, most = 148 * (BITS == 0 ? 4 : 3) * 2;
+    rows_kernel<T, LPH, BITS><<<want < most ? want : most, kRowThreads, bytes, s>>>(a, cb);
     return check_launch(s);
 }
+template <typename T, int LPH>
+int launch_rows_bits(int bits, RowArgs& a, const Codebook& cb, cudaStream_t s) {
+    if (bits == 0) return launch_rows_one<T, LPH, 0>(a, cb, s);
+    return bits == 3 ? launch_rows_one<T, LPH, 3>(a, cb, s) : launch_rows_one<T, LPH, 4>(a, cb, s);
+}
 template <typename T>
-int launch_rows_dim(int dim, int bits, const RowArgs& a, const Codebook& cb, cudaStream_t s) {
+int launch_rows_dim(int dim, int bits, RowArgs& a, const Codebook& cb, cudaStream_t s) {
     if (dim == 64) return launch_rows_bits<T, 8>(bits, a, cb, s);
     if (dim == 128) return launch_rows_bits<T, 16>(bits, a, cb, s);
     return launch_rows_bits<T, 32>(bits, a, cb, s);
@@ -771,20 +756,20 @@ int tqb_paged_dequantize(const tqb_paged_layer* layer, const int64_t* slots, int
                (long long)layer->num_pages * layer->page_size, layer->num_kv_heads, log2_of(layer->page_size), block_sign_magnitude()};
     Codebook cb{};
     if (!block_codebook(layer->bits, TQB_MAXNORM, cb)) return TQB_ERR_UNSUPPORTED_BITS;
-    const int lph = layer->head_dim / 8;
-    const long long warps = (n * layer->num_kv_heads * lph + 31) / 32, want = (warps + kRowWarps - 1) / kRowWarps;
+    const int nb = layer->head_dim / kBlock;
+    const long long want = (n * layer->num_kv_heads * nb + kRowThreads - 1) / kRowThreads;
     const dim3 grid((unsigned)(want < 148 * 8 ? want : 148 * 8), 2);
     cudaStream_t s = as_stream(stream);
-#define TQB_BACK(T, LPH)                                                               \
-    do {                                                                               \
-        if (layer->bits == 3) back_kernel<T, LPH, 3><<<grid, kRowThreads, 0, s>>>(a, cb); \
-        else back_kernel<T, LPH, 4><<<grid, kRowThreads, 0, s>>>(a, cb);               \
+#define TQB_BACK(T, NB)                                                                   \
+    do {                                                                                  \
+        if (layer->bits == 3) back_kernel<T, NB, 3><<<grid, kRowThreads, 0, s>>>(a, cb);  \
+        else back_kernel<T, NB, 4><<<grid, kRowThreads, 0, s>>>(a, cb);                   \
     } while (0)
-#define TQB_BACK_DIM(T)                 \
-    do {                                \
-        if (lph == 8) TQB_BACK(T, 8);   \
-        else if (lph == 16) TQB_BACK(T, 16); \
-        else TQB_BACK(T, 32);           \
+#define TQB_BACK_DIM(T)             \
+    do {                            \
+        if (nb == 2) TQB_BACK(T, 2); \
+        else if (nb == 4) TQB_BACK(T, 4); \
+        else TQB_BACK(T, 8);        \
     } while (0)
     if (out_dtype == TQB_F32) TQB_BACK_DIM(float);
     else if (out_dtype == TQB_F16) TQB_BACK_DIM(__half);

@@ -18,15 +18,16 @@ inline float block_sign_magnitude() {
     return inv * s;
 }
 
-// More than 48 KB of shared memory, the static part included, is a property of the kernel on a device: set once for each.
+// More than 48 KB of shared memory, the static part included, is a property of the kernel on a device: set once for each, to
+// `most` bytes (0: `bytes`, which is then the same in every call).
 template <auto* KERNEL>
-int allow_shared(int bytes) {
+int allow_shared(int bytes, int most = 0) {
     static std::atomic<unsigned long long> configured{0};
     if (bytes <= 32 * 1024) return TQB_OK;
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = -1;
     if (dev >= 0 && ((configured.load(std::memory_order_acquire) >> dev) & 1ull)) return TQB_OK;
-    const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, most > bytes ? most : bytes);
     if (e != cudaSuccess) {
         set_cuda_error(e);
         return TQB_ERR_CUDA;

@@ -91,6 +91,14 @@ def _out_rows(name, t, like, index):
     return at, s0, s1
 
 
+def _made(out, name, like, n, heads, dim, index):
+    """(tensor, its rows as _out_rows gives them) of an output, made here unless given."""
+    if out is not None:
+        return out, _out_rows(name, out, like, index)
+    out = like.new_empty((n, heads, dim))
+    return out, (out.data_ptr(), heads * dim, dim)
+
+
 def _three(name, t):
     if t.dim() != 3:
         raise DimensionMismatch(f"{name}: expected [tokens, heads, dim], got {tuple(t.shape)}")
@@ -222,12 +230,9 @@ class QkNormRope:
         if k.dtype is not dt:
             raise DimensionMismatch(f"k: expected {dt}, got {k.dtype}")
         qi, ki = _rows("q", q, q.shape, index), _rows("k", k, (n, hkv, d), index)
-        if q_out is None:
-            q_out = q.new_empty((n, hq, d))
-        if k_out is None:
-            k_out = q.new_empty((n, hkv, d))
-        _call(index, lib.tqb_qk_norm_rope, self._params(qi[1:], _out_rows("q_out", q_out, q, index), ki[1:], _out_rows("k_out", k_out, k, index),
-                                                        n, hq, hkv, d, dt, positions))
+        q_out, qo = _made(q_out, "q_out", q, n, hq, d, index)
+        k_out, ko = _made(k_out, "k_out", k, n, hkv, d, index)
+        _call(index, lib.tqb_qk_norm_rope, self._params(qi[1:], qo, ki[1:], ko, n, hq, hkv, d, dt, positions))
         return q_out, k_out
 
 
@@ -278,9 +283,8 @@ class PagedLayer:
             raise DimensionMismatch(f"q and k differ in dtype: {q.dtype}, {k[0].dtype}")
         if rope.index != index:
             raise ValueError(f"rope: expected tensors on cuda:{index}, got cuda:{rope.index}")
-        if q_out is None:
-            q_out = q.new_empty((n, hq, d))
-        p = rope._params(qi[1:], _out_rows("q_out", q_out, q, index), k[1:], (0, 0, 0), n, hq, self.num_kv_heads, d, q.dtype, positions)
+        q_out, qo = _made(q_out, "q_out", q, n, hq, d, index)
+        p = rope._params(qi[1:], qo, k[1:], (0, 0, 0), n, hq, self.num_kv_heads, d, q.dtype, positions)
         _call(index, lib.tqb_paged_append_rope, self._c, p, v[1], v[2], v[3], self._slots(slots, n))
         return q_out
 
@@ -316,7 +320,9 @@ class PagedLayer:
         lens = _want("kv_lens", kv_lens, torch.int32, (n,), index)
         if out is None:
             out = q.new_empty((n, hq, d))
-        to = _want("out", out, out.dtype, (n, hq, d), index)
+            to = out.data_ptr()
+        else:
+            to = _want("out", out, out.dtype, (n, hq, d), index)
         if scratch is None:
             scratch = self.attend_scratch(hq)
         work = _want("scratch", scratch, torch.uint8, scratch.shape, index)
