@@ -204,12 +204,25 @@ __global__ void __launch_bounds__(kReleaseThreads) release_kernel(const uint8_t*
 constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32;
 
+// x / d for x below 2^31 by a multiplication: m = floor(2^(31 + s) / d) + 1 with 2^(s - 1) < d <= 2^s errs by less than 1 / d
+// (Granlund and Montgomery, PLDI 1994).
+struct Divisor {
+    unsigned d, m, s;
+    explicit Divisor(unsigned div) : d(div), m(0), s(0) {
+        while ((1ull << s) < d) ++s;
+        m = (unsigned)(((1ull << (31 + s)) / d) + 1);
+    }
+    Divisor() : d(1), m(0), s(0) {}
+    __device__ __forceinline__ unsigned of(unsigned x) const { return (unsigned)(((unsigned long long)x * m) >> (31 + s)); }
+};
+
 struct RowSpan {            // one tensor of rows [tokens, heads, head_dim]
     const void* in;
     void* out;
     long long in_token, in_head, out_token, out_head;   // strides in elements
     const void* weight;
     int heads;
+    Divisor by_heads;
 };
 struct RowArgs {
     RowSpan q, k, v;
@@ -220,6 +233,7 @@ struct RowArgs {
     uint16_t* sc[2];
     long long num_slots;
     int tokens, chunk, rot_dim, flags, kv_heads, page_shift;   // chunk: tokens that a CTA takes at a time
+    Divisor by_kv, by_half;
     float eps;
     float outer_centroid;
 };
@@ -293,7 +307,8 @@ struct Eight<__half> {
     __device__ __forceinline__ void store(__half* p) const { *reinterpret_cast<uint4*>(p) = r; }
 };
 
-constexpr int kRowTokens = 4;
+constexpr int kRowBlocks = 512;   // 32-blocks that a CTA packs at a time, about
+constexpr int kRowTokens = 4;     // tokens at a time where nothing is packed
 
 template <typename T>
 struct Tile {
@@ -312,127 +327,141 @@ __device__ __forceinline__ void load_tile(const unsigned char* p, float (&v)[32]
     }
 }
 
+// Rows of one tensor of a chunk: KIND 0 queries, 1 keys, 2 values.  s_cos, s_sin [token][D]: element e of a rotated row is
+// v_e cos_e + v_partner sin_e, the sign of the first element's sine with it.
+template <int KIND, typename T, int LPH, bool STORE>
+__device__ __forceinline__ void do_rows(const RowArgs& a, const RowSpan& s, int t0, int nt, const float* s_cos, const float* s_sin, unsigned char* s_tile) {
+    constexpr int D = LPH * 8, HPW = 32 / LPH, NB = D / 32;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LPH, l = lane % LPH;
+    const int rows = nt * s.heads, half = a.rot_dim >> 1;
+    const bool norm = KIND != 2 && (a.flags & TQB_ROPE_NO_NORM) == 0, inter = (a.flags & TQB_ROPE_INTERLEAVED) != 0;
+    const T* const in = reinterpret_cast<const T*>(s.in) + t0 * s.in_token + 8 * l;
+    T* const out = s.out == nullptr ? nullptr : reinterpret_cast<T*>(s.out) + t0 * s.out_token + 8 * l;
+    F2 w[4];
+    if (norm) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = 1.0f;
+        if (s.weight != nullptr) {
+            Eight<T> e;
+            e.load(reinterpret_cast<const T*>(s.weight) + 8 * l);
+            e.get(x);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = f2(x[2 * i], x[2 * i + 1]);
+    }
+    const int hl = half >> 3;   // lanes of half a rotated row
+    const bool turns = 8 * l < a.rot_dim;
+    const int from = lane + (!turns ? 0 : l < hl ? hl : -hl);
+    int r = warp * HPW + sub;
+    Eight<T> ahead;
+    auto fetch = [&](int row) {
+        const int at = min(row, rows - 1), tok = (int)s.by_heads.of(at);
+        ahead.load(in + tok * s.in_token + (at - tok * s.heads) * s.in_head);
+    };
+    if (warp * HPW < rows) fetch(r);
+    for (; r - sub < rows; r += kRowWarps * HPW) {   // (the same for the whole warp)
+        const bool live = r < rows;
+        const int at = min(r, rows - 1), tok = (int)s.by_heads.of(at), h = at - tok * s.heads;
+        Eight<T> e = ahead;
+        if (r - sub + kRowWarps * HPW < rows) fetch(r + kRowWarps * HPW);
+        if (KIND != 2 && (norm || half > 0)) {
+            float x[8];
+            e.get(x);
+            F2 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = f2(x[2 * i], x[2 * i + 1]);
+            if (norm) {
+                F2 ss = mul2(v[0], v[0]);
+#pragma unroll
+                for (int i = 1; i < 4; ++i) ss = fma2(v[i], v[i], ss);
+                const float2 t = halves(ss);
+                float sum = t.x + t.y;
+#pragma unroll
+                for (int o = LPH / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                const F2 inv = f2(1.0f / sqrtf(sum * (1.0f / D) + a.eps));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = mul2(mul2(v[i], inv), w[i]);
+            }
+            if (half > 0) {
+                F2 p[4];
+                if (inter) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 t = halves(v[i]);
+                        p[i] = f2(t.y, t.x);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 t = halves(v[i]);
+                        const float p0 = __shfl_sync(0xffffffffu, t.x, from), p1 = __shfl_sync(0xffffffffu, t.y, from);
+                        p[i] = f2(p0, p1);
+                    }
+                }
+                if (turns) {
+                    const float4* c = reinterpret_cast<const float4*>(s_cos + tok * D + 8 * l);
+                    const float4* n = reinterpret_cast<const float4*>(s_sin + tok * D + 8 * l);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float4 ci = c[i], si = n[i];
+                        v[2 * i] = fma2(v[2 * i], f2(ci.x, ci.y), mul2(p[2 * i], f2(si.x, si.y)));
+                        v[2 * i + 1] = fma2(v[2 * i + 1], f2(ci.z, ci.w), mul2(p[2 * i + 1], f2(si.z, si.w)));
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 t = halves(v[i]);
+                x[2 * i] = t.x;
+                x[2 * i + 1] = t.y;
+            }
+            e.set(x);
+        }
+        if (live) {
+            if (out != nullptr) e.store(out + tok * s.out_token + h * s.out_head);
+            if (STORE && KIND != 0)
+                e.store(reinterpret_cast<T*>(s_tile + (size_t)(((tok * 2 + KIND - 1) * a.kv_heads + h) * NB + (l >> 2)) * Tile<T>::kPitch) + 8 * (l & 3));
+        }
+    }
+}
+
 template <typename T, int LPH, int BITS>
 __global__ void __launch_bounds__(kRowThreads, BITS == 0 ? 4 : 3) rows_kernel(const __grid_constant__ RowArgs a, const __grid_constant__ Codebook cb) {
-    constexpr int D = LPH * 8, HPW = 32 / LPH, NB = D / 32;
-    extern __shared__ __align__(16) unsigned char s_tile[];   // BITS != 0: [token][K, V][head][block]
-    __shared__ __align__(16) float2 s_cs[kRowTokens][D / 2];
-    __shared__ float2 s_cells[BITS == 3 ? kCells * 32 : 1];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int sub = lane / LPH, l = lane % LPH;
+    constexpr int D = LPH * 8, NB = D / 32;
+    extern __shared__ __align__(16) unsigned char s_dyn[];
     const int half = a.rot_dim >> 1;
-    const bool inter = (a.flags & TQB_ROPE_INTERLEAVED) != 0, norm = (a.flags & TQB_ROPE_NO_NORM) == 0;
-    const int heads = a.q.heads + a.k.heads + a.v.heads, groups = (heads + HPW - 1) / HPW;
+    float* const s_cos = reinterpret_cast<float*>(s_dyn);                       // rot_dim != 0: [token][D]
+    float* const s_sin = s_cos + (half > 0 ? a.chunk * D : 0);
+    unsigned char* const s_tile = reinterpret_cast<unsigned char*>(s_sin + (half > 0 ? a.chunk * D : 0));   // BITS != 0: [token][K, V][head][block]
+    __shared__ float2 s_cells[BITS == 3 ? kCells * 32 : 1];
+    const int tid = threadIdx.x, lane = tid & 31;
     if (BITS == 3) build_cell_table(cb, cb.n - 1, s_cells, tid, kRowThreads);
     for (int t0 = blockIdx.x * a.chunk; t0 < a.tokens; t0 += gridDim.x * a.chunk) {
         const int nt = min(a.chunk, a.tokens - t0);
-        // the lane's row of pass (token tok, group g)
-        auto span_of = [&](int g, int& h) -> const RowSpan& {
-            const int hd = min(g * HPW + sub, heads - 1);
-            const int kind = hd < a.q.heads ? 0 : hd < a.q.heads + a.k.heads ? 1 : 2;
-            h = kind == 0 ? hd : kind == 1 ? hd - a.q.heads : hd - a.q.heads - a.k.heads;
-            return kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-        };
-        auto fetch = [&](int tok, int g, Eight<T>& e) {
-            int h;
-            const RowSpan& s = span_of(g, h);
-            e.load(reinterpret_cast<const T*>(s.in) + (t0 + tok) * s.in_token + h * s.in_head + 8 * l);
-        };
-        auto advance = [&](int& tok, int& g) {
-            g += kRowWarps;
-            while (g >= groups) {
-                g -= groups;
-                ++tok;
-            }
-        };
-        int tok = 0, g = warp - kRowWarps;
-        advance(tok, g);
-        Eight<T> ahead;
-        if (tok < nt) fetch(tok, g, ahead);
         for (int i = tid; i < nt * half; i += kRowThreads) {
-            const int t = i / half, f = i - t * half;
+            const int t = (int)a.by_half.of(i), f = i - t * half;
             const double pos = (a.flags & TQB_ROPE_POSITIONS_64) ? (double)reinterpret_cast<const long long*>(a.positions)[t0 + t]
                                                                 : (double)reinterpret_cast<const int*>(a.positions)[t0 + t];
             const double ang = pos * (double)a.inv_freq[f];
             const double turns = rint(ang * 0.15915494309189535);
             float si, co;
             sincosf((float)fma(turns, -6.283185307179586, ang), &si, &co);
-            s_cs[t][f] = make_float2(co, si);
+            const bool inter = (a.flags & TQB_ROPE_INTERLEAVED) != 0;
+            const int first = t * D + (inter ? 2 * f : f), second = first + (inter ? 1 : half);
+            s_cos[first] = s_cos[second] = co;
+            s_sin[first] = -si;
+            s_sin[second] = si;
         }
         __syncthreads();
-        while (tok < nt) {
-            const int this_tok = tok, this_g = g;
-            Eight<T> e = ahead;
-            advance(tok, g);
-            if (tok < nt) fetch(tok, g, ahead);
-            int h;
-            const RowSpan& s = span_of(this_g, h);
-            const bool live = this_g * HPW + sub < heads;
-            const int hd = min(this_g * HPW + sub, heads - 1), kind = hd < a.q.heads ? 0 : hd < a.q.heads + a.k.heads ? 1 : 2;
-            float v[8];
-            e.get(v);
-            // the shuffles below are done by all lanes, whichever tensor their head is of
-            if (norm) {
-                float ss = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
-#pragma unroll
-                for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                if (kind != 2) {
-                    const float r = 1.0f / sqrtf(ss * (1.0f / D) + a.eps);
-                    float w[8];
-                    if (s.weight != nullptr) {
-                        Eight<T> we;
-                        we.load(reinterpret_cast<const T*>(s.weight) + 8 * l);
-                        we.get(w);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) w[i] = 1.0f;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = (v[i] * r) * w[i];
-                }
-            }
-            if (half > 0) {
-                if (inter) {
-                    if (kind != 2 && 8 * l < a.rot_dim) {
-                        const float4* cs = reinterpret_cast<const float4*>(&s_cs[this_tok][4 * l]);
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const float4 c = cs[i];   // (cos, sin) twice
-                            const float x0 = v[4 * i], y0 = v[4 * i + 1], x1 = v[4 * i + 2], y1 = v[4 * i + 3];
-                            v[4 * i] = fmaf(x0, c.x, -(y0 * c.y));
-                            v[4 * i + 1] = fmaf(y0, c.x, x0 * c.y);
-                            v[4 * i + 2] = fmaf(x1, c.z, -(y1 * c.w));
-                            v[4 * i + 3] = fmaf(y1, c.z, x1 * c.w);
-                        }
-                    }
-                } else {
-                    const int hl = half >> 3;   // lanes of half a rotated row
-                    const bool first = l < hl, turns = l < 2 * hl;
-                    const int from = lane + (!turns ? 0 : first ? hl : -hl);
-                    const float4* cs = reinterpret_cast<const float4*>(&s_cs[this_tok][turns ? 8 * (first ? l : l - hl) : 0]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float4 c = cs[i];
-                        const float o0 = __shfl_sync(0xffffffffu, v[2 * i], from), o1 = __shfl_sync(0xffffffffu, v[2 * i + 1], from);
-                        if (kind != 2 && turns) {
-                            v[2 * i] = fmaf(v[2 * i], c.x, first ? -(o0 * c.y) : o0 * c.y);
-                            v[2 * i + 1] = fmaf(v[2 * i + 1], c.z, first ? -(o1 * c.w) : o1 * c.w);
-                        }
-                    }
-                }
-            }
-            if (kind != 2) e.set(v);
-            if (live && s.out != nullptr) e.store(reinterpret_cast<T*>(s.out) + (t0 + this_tok) * s.out_token + h * s.out_head + 8 * l);
-            if (BITS != 0 && live && kind != 0)
-                e.store(reinterpret_cast<T*>(s_tile + (size_t)(((this_tok * 2 + kind - 1) * a.kv_heads + h) * NB + (l >> 2)) * Tile<T>::kPitch) + 8 * (l & 3));
-        }
+        if (a.q.heads > 0) do_rows<0, T, LPH, false>(a, a.q, t0, nt, s_cos, s_sin, s_tile);
+        if (a.k.heads > 0) do_rows<1, T, LPH, BITS != 0>(a, a.k, t0, nt, s_cos, s_sin, s_tile);
         if constexpr (BITS != 0) {
+            do_rows<2, T, LPH, true>(a, a.v, t0, nt, s_cos, s_sin, s_tile);
             __syncthreads();
             const unsigned kv = (unsigned)a.kv_heads;
             for (int i = tid; i < nt * 2 * a.kv_heads * NB; i += kRowThreads) {
-                const unsigned row = (unsigned)i / NB, ts = row / kv, h = row - ts * kv, b = (unsigned)i % NB;
+                const unsigned row = (unsigned)i / NB, ts = a.by_kv.of(row), h = row - ts * kv, b = (unsigned)i % NB;
                 const long long slot = a.slots[t0 + (ts >> 1)];
                 if (slot < 0 || slot >= a.num_slots) continue;
                 float v[32];
@@ -440,7 +469,8 @@ __global__ void __launch_bounds__(kRowThreads, BITS == 0 ? 4 : 3) rows_kernel(co
                 uint32_t w[4];
                 const float scale = pqo_quantize_values<BITS>(v, cb, a.outer_centroid, w, BITS == 3 ? s_cells + lane : nullptr);
                 const int side = ts & 1;
-                const size_t at = (((((size_t)(slot >> a.page_shift) * kv + h) << a.page_shift) + (slot & ((1 << a.page_shift) - 1)))) * NB + b;
+                const unsigned page = (unsigned)(slot >> a.page_shift), off = (unsigned)slot & ((1u << a.page_shift) - 1);   // (rows fit in 32 bits)
+                const size_t at = (size_t)(((page * kv + h) << a.page_shift) + off) * NB + b;
                 uint8_t* to = a.idx[side] + at * (4 * BITS);
                 if (BITS == 4) {
                     *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -465,13 +495,15 @@ struct BackArgs {
     const uint16_t* sc[2];
     void* out[2];
     const int64_t* slots;
-    long long n, num_slots;
-    int kv_heads, page_shift;
+    unsigned total;         // blocks of a side, below 2^31 - 2^20
+    long long num_slots;
+    Divisor kv_heads;
+    int page_shift;
     float sign_mag;
 };
 
 template <typename T, int NB, int BITS>
-__global__ void __launch_bounds__(kRowThreads) back_kernel(const __grid_constant__ BackArgs a, const __grid_constant__ Codebook cb) {
+__global__ void __launch_bounds__(kRowThreads, 4) back_kernel(const __grid_constant__ BackArgs a, const __grid_constant__ Codebook cb) {
     constexpr int kPitch = Tile<T>::kPitch, kPieces = 2 * (int)sizeof(T);   // 16-byte pieces of a block
     __shared__ __align__(2048) unsigned char s_tab[2 * DequantTable<BITS>::kBytes];
     __shared__ __align__(16) unsigned char s_stage[kRowThreads * kPitch];
@@ -480,17 +512,17 @@ __global__ void __launch_bounds__(kRowThreads) back_kernel(const __grid_constant
     __syncthreads();
     const uint32_t tab = (uint32_t)__cvta_generic_to_shared(s_tab) + lane * 4;
     unsigned char* stage = s_stage + (tid >> 5) * 32 * kPitch;
-    const unsigned kv = (unsigned)a.kv_heads;
-    const long long total = a.n * kv * NB, step = (long long)gridDim.x * kRowThreads;
+    const unsigned total = a.total, step = gridDim.x * kRowThreads;
     uint32_t w[4] = {0u, 0u, 0u, 0u};
     float scale = 0.0f;
     bool in = false;
-    auto fetch = [&](long long blk0) {
-        const long long blk = min(blk0 + lane, total - 1), row = blk / NB, tok = row / kv;
-        const long long slot = a.slots[tok];
+    auto slot_of = [&](unsigned blk0) { return a.slots[a.kv_heads.of(min(blk0 + lane, total - 1) / NB)]; };
+    auto fetch = [&](unsigned blk0, long long slot) {
+        const unsigned blk = min(blk0 + lane, total - 1), row = blk / NB, tok = a.kv_heads.of(row);
         in = slot >= 0 && slot < a.num_slots;
         if (!in) return;
-        const size_t at = (((((size_t)(slot >> a.page_shift) * kv + (size_t)(row - tok * kv)) << a.page_shift) + (slot & ((1 << a.page_shift) - 1)))) * NB + blk % NB;
+        const unsigned page = (unsigned)(slot >> a.page_shift), off = (unsigned)slot & ((1u << a.page_shift) - 1);   // (rows fit in 32 bits)
+        const size_t at = (size_t)(((page * a.kv_heads.d + (row - tok * a.kv_heads.d)) << a.page_shift) + off) * NB + blk % NB;
         const uint8_t* p = a.idx[side] + at * (4 * BITS);
         if (BITS == 4) {
             const uint4 r = __ldg(reinterpret_cast<const uint4*>(p));
@@ -501,13 +533,18 @@ __global__ void __launch_bounds__(kRowThreads) back_kernel(const __grid_constant
         }
         scale = fabsf(f16_bits_to_f32(__ldg(a.sc[side] + at)));
     };
-    long long blk0 = ((long long)blockIdx.x * kRowThreads + tid) & ~31ll;
-    if (blk0 < total) fetch(blk0);
+    unsigned blk0 = (blockIdx.x * kRowThreads + tid) & ~31u;
+    long long slot = 0;   // of the blocks after the next
+    if (blk0 < total) fetch(blk0, slot_of(blk0));
+    if (blk0 + step < total) slot = slot_of(blk0 + step);
     for (; blk0 < total; blk0 += step) {
         float v[32];
         dequantize_values<BITS>(w, f2(scale), tab, v);
         const bool live = in;
-        if (blk0 + step < total) fetch(blk0 + step);
+        if (blk0 + step < total) {
+            fetch(blk0 + step, slot);
+            if (blk0 + 2 * step < total) slot = slot_of(blk0 + 2 * step);
+        }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             float e[8];
@@ -549,14 +586,17 @@ int check_rows(const void* p, long long token, long long head, size_t elem) {
 
 template <typename T, int LPH, int BITS>
 int launch_rows_one(RowArgs& a, const Codebook& cb, cudaStream_t s) {
-    // One token a CTA while that leaves SMs idle, and while more would not fit.
-    const size_t token = BITS == 0 ? 0 : (size_t)2 * a.kv_heads * (LPH / 4) * Tile<T>::kPitch;
-    a.chunk = a.tokens < 148 * kRowTokens ? 1 : kRowTokens;
-    while (a.chunk > 1 && token * a.chunk > 64 * 1024) a.chunk >>= 1;
-    if (token > 160 * 1024) return TQB_ERR_UNSUPPORTED;   // KV heads x head_dim beyond 64 x 256 (16-bit)
+    // As many tokens at a time as make kRowBlocks blocks; fewer while that leaves SMs idle.
+    const int blocks = BITS == 0 ? 0 : 2 * a.kv_heads * (LPH / 4);
+    const size_t token = (size_t)blocks * Tile<T>::kPitch + (a.rot_dim > 0 ? (size_t)LPH * 8 * 2 * sizeof(float) : 0);
+    if (token > 160 * 1024) return TQB_ERR_UNSUPPORTED;
+    a.by_kv = Divisor((unsigned)(a.kv_heads > 0 ? a.kv_heads : 1));
+    a.by_half = Divisor((unsigned)(a.rot_dim > 0 ? a.rot_dim / 2 : 1));
+    a.chunk = BITS == 0 ? kRowTokens : (kRowBlocks + blocks - 1) / blocks;
+    while (a.chunk > 1 && (a.tokens < 148 * a.chunk || token * a.chunk > 64 * 1024)) a.chunk >>= 1;
     const int bytes = (int)(token * a.chunk);
     if (int st = allow_shared<rows_kernel<T, LPH, BITS>>(bytes, 160 * 1024)) return st;
-    const int want = (a.tokens + a.chunk - 1) / a.chunk, most = 148 * (BITS == 0 ? 4 : 3) * 2;
+    const int want = (a.tokens + a.chunk - 1) / a.chunk, most = 148 * (BITS == 0 ? 4 : 3);
     rows_kernel<T, LPH, BITS><<<want < most ? want : most, kRowThreads, bytes, s>>>(a, cb);
     return check_launch(s);
 }
@@ -603,13 +643,13 @@ int rope_args(const tqb_rope_params* p, bool keys_out, RowArgs& a) {
         if ((st = check_rows(p->q, p->q_token_stride, p->q_head_stride, elem)) != TQB_OK) return st;
         if ((st = check_rows(p->q_out, p->q_out_token_stride, p->q_out_head_stride, elem)) != TQB_OK) return st;
         if (!aligned16(p->q_weight)) return TQB_ERR_MISALIGNED;
-        a.q = RowSpan{p->q, p->q_out, p->q_token_stride, p->q_head_stride, p->q_out_token_stride, p->q_out_head_stride, p->q_weight, p->num_q_heads};
+        a.q = RowSpan{p->q, p->q_out, p->q_token_stride, p->q_head_stride, p->q_out_token_stride, p->q_out_head_stride, p->q_weight, p->num_q_heads, Divisor((unsigned)(p->num_q_heads > 0 ? p->num_q_heads : 1))};
     }
     if (p->k) {
         if ((st = check_rows(p->k, p->k_token_stride, p->k_head_stride, elem)) != TQB_OK) return st;
         if (p->k_out && (st = check_rows(p->k_out, p->k_out_token_stride, p->k_out_head_stride, elem)) != TQB_OK) return st;
         if (!aligned16(p->k_weight)) return TQB_ERR_MISALIGNED;
-        a.k = RowSpan{p->k, p->k_out, p->k_token_stride, p->k_head_stride, p->k_out_token_stride, p->k_out_head_stride, p->k_weight, p->num_kv_heads};
+        a.k = RowSpan{p->k, p->k_out, p->k_token_stride, p->k_head_stride, p->k_out_token_stride, p->k_out_head_stride, p->k_weight, p->num_kv_heads, Divisor((unsigned)(p->num_kv_heads > 0 ? p->num_kv_heads : 1))};
     }
     a.positions = p->positions;
     a.inv_freq = p->inv_freq;
@@ -720,8 +760,8 @@ int tqb_paged_append(const tqb_paged_layer* layer, const void* k, int64_t k_toke
     if ((st = check_rows(v, v_token_stride, v_head_stride, elem)) != TQB_OK) return st;
     RowArgs a{};
     if ((st = layer_args(layer, slots, a)) != TQB_OK) return st;
-    a.k = RowSpan{k, nullptr, k_token_stride, k_head_stride, 0, 0, nullptr, layer->num_kv_heads};
-    a.v = RowSpan{v, nullptr, v_token_stride, v_head_stride, 0, 0, nullptr, layer->num_kv_heads};
+    a.k = RowSpan{k, nullptr, k_token_stride, k_head_stride, 0, 0, nullptr, layer->num_kv_heads, Divisor((unsigned)layer->num_kv_heads)};
+    a.v = RowSpan{v, nullptr, v_token_stride, v_head_stride, 0, 0, nullptr, layer->num_kv_heads, Divisor((unsigned)layer->num_kv_heads)};
     a.tokens = num_tokens;
     a.flags = TQB_ROPE_NO_NORM;
     return launch_rows(dtype, layer->head_dim, layer->bits, a, as_stream(stream));
@@ -739,7 +779,7 @@ int tqb_paged_append_rope(const tqb_paged_layer* layer, const tqb_rope_params* p
     if (!p->k || !v) return TQB_ERR_NULL_POINTER;
     if ((st = check_rows(v, v_token_stride, v_head_stride, size_of(p->dtype))) != TQB_OK) return st;
     if ((st = layer_args(layer, slots, a)) != TQB_OK) return st;
-    a.v = RowSpan{v, nullptr, v_token_stride, v_head_stride, 0, 0, nullptr, layer->num_kv_heads};
+    a.v = RowSpan{v, nullptr, v_token_stride, v_head_stride, 0, 0, nullptr, layer->num_kv_heads, Divisor((unsigned)layer->num_kv_heads)};
     return launch_rows(p->dtype, p->head_dim, layer->bits, a, as_stream(stream));
 }
 
@@ -752,14 +792,21 @@ int tqb_paged_dequantize(const tqb_paged_layer* layer, const int64_t* slots, int
     if (n == 0) return TQB_OK;
     if (!slots || !k_out || !v_out) return TQB_ERR_NULL_POINTER;
     if ((uintptr_t)slots % 8 != 0 || !aligned16(k_out) || !aligned16(v_out)) return TQB_ERR_MISALIGNED;
-    BackArgs a{{layer->k_indices, layer->v_indices}, {layer->k_scales, layer->v_scales}, {k_out, v_out}, slots, n,
-               (long long)layer->num_pages * layer->page_size, layer->num_kv_heads, log2_of(layer->page_size), block_sign_magnitude()};
     Codebook cb{};
     if (!block_codebook(layer->bits, TQB_MAXNORM, cb)) return TQB_ERR_UNSUPPORTED_BITS;
     const int nb = layer->head_dim / kBlock;
-    const long long want = (n * layer->num_kv_heads * nb + kRowThreads - 1) / kRowThreads;
-    const dim3 grid((unsigned)(want < 148 * 8 ? want : 148 * 8), 2);
+    const int64_t token = (int64_t)layer->num_kv_heads * nb, most = ((1ll << 31) - (1 << 20)) / token;   // blocks of a token; tokens a launch
+    if (most < 1) return TQB_ERR_TOO_LARGE;
     cudaStream_t s = as_stream(stream);
+    for (int64_t done = 0; done < n; done += most) {
+        const int64_t now = n - done < most ? n - done : most;
+        const size_t skip = (size_t)done * token * kBlock * size_of(out_dtype);
+        const BackArgs a{{layer->k_indices, layer->v_indices}, {layer->k_scales, layer->v_scales},
+                         {reinterpret_cast<char*>(k_out) + skip, reinterpret_cast<char*>(v_out) + skip}, slots + done, (unsigned)(now * token),
+                         (long long)layer->num_pages * layer->page_size, Divisor((unsigned)layer->num_kv_heads), log2_of(layer->page_size),
+                         block_sign_magnitude()};
+        const long long want = (now * token + kRowThreads - 1) / kRowThreads;
+        const dim3 grid((unsigned)(want < 148 * 4 ? want : 148 * 4), 2);
 #define TQB_BACK(T, NB)                                                                   \
     do {                                                                                  \
         if (layer->bits == 3) back_kernel<T, NB, 3><<<grid, kRowThreads, 0, s>>>(a, cb);  \
@@ -771,12 +818,14 @@ int tqb_paged_dequantize(const tqb_paged_layer* layer, const int64_t* slots, int
         else if (nb == 4) TQB_BACK(T, 4); \
         else TQB_BACK(T, 8);        \
     } while (0)
-    if (out_dtype == TQB_F32) TQB_BACK_DIM(float);
-    else if (out_dtype == TQB_F16) TQB_BACK_DIM(__half);
-    else TQB_BACK_DIM(__nv_bfloat16);
+        if (out_dtype == TQB_F32) TQB_BACK_DIM(float);
+        else if (out_dtype == TQB_F16) TQB_BACK_DIM(__half);
+        else TQB_BACK_DIM(__nv_bfloat16);
+        if (int e = check_launch(s)) return e;
+    }
 #undef TQB_BACK_DIM
 #undef TQB_BACK
-    return check_launch(s);
+    return TQB_OK;
 }
 
 }  // extern "C"
