@@ -193,13 +193,14 @@ __global__ void __launch_bounds__(kReleaseThreads) release_kernel(const uint8_t*
 }
 
 // ---- rows into pages, with norm and rotation ---------------------------------------------------------------------------
-// A CTA takes kRowTokens tokens at a time (one, where there are few).
+// A warp takes a token (a CTA, where there are few): its angles, its rows, its blocks.
 // Angles: position * inv_freq in f64, less whole turns, then sincosf in f32 (an f32 product would be off by position * 2^-24,
 //   0.06 rad at a million tokens), once for a token.
 // Rows: one warp pass takes 32 / (D / 8) heads of a token, eight consecutive elements a lane: every load and store of a warp is
-//   dense, the norm's sum and the partner of a rotated pair are shuffles away.  The next pass's loads are in flight.  Queries
-//   leave for q_out; keys and values go to a tile of 32-blocks in shared memory, in their type.
-// Blocks: one thread packs one 32-block of the tile as tqb_block_quantize does (pqo_quantize_values), 16 or 12 bytes of codes.
+//   dense, the norm's sum and the partner of a rotated pair are shuffles away.  The next pass's load is in flight.  Queries
+//   leave for q_out; keys go to a tile of 32-blocks in shared memory, in their type.
+// Blocks: one thread packs one 32-block of the tile, or of the values where they lie, as tqb_block_quantize does
+//   (pqo_quantize_values), 16 or 12 bytes of codes.
 //   Four lanes a block with the butterfly's last stages as shuffles needs three times the instructions.
 constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32;
@@ -222,7 +223,6 @@ struct RowSpan {            // one tensor of rows [tokens, heads, head_dim]
     long long in_token, in_head, out_token, out_head;   // strides in elements
     const void* weight;
     int heads;
-    Divisor by_heads;
 };
 struct RowArgs {
     RowSpan q, k, v;
@@ -232,8 +232,10 @@ struct RowArgs {
     uint8_t* idx[2];        // K, V
     uint16_t* sc[2];
     long long num_slots;
-    int tokens, chunk, rot_dim, flags, kv_heads, page_shift;   // chunk: tokens that a CTA takes at a time
-    Divisor by_kv, by_half;
+    int tokens, rot_dim, flags, kv_heads, page_shift;
+    int shared_token, token_bytes;   // rows_kernel: a CTA for each token; shared memory for a token
+    unsigned total;         // append_kernel: blocks of K (or V), below 2^31 - 2^20
+    Divisor by_kv;
     float eps;
     float outer_centroid;
 };
@@ -307,9 +309,6 @@ struct Eight<__half> {
     __device__ __forceinline__ void store(__half* p) const { *reinterpret_cast<uint4*>(p) = r; }
 };
 
-constexpr int kRowBlocks = 512;   // 32-blocks that a CTA packs at a time, about
-constexpr int kRowTokens = 4;     // tokens at a time where nothing is packed
-
 template <typename T>
 struct Tile {
     static constexpr int kPitch = 32 * (int)sizeof(T) + 16;   // of a 32-block: 16-byte pieces of eight lanes in 32 banks
@@ -327,16 +326,62 @@ __device__ __forceinline__ void load_tile(const unsigned char* p, float (&v)[32]
     }
 }
 
-// Rows of one tensor of a chunk: KIND 0 queries, 1 keys, 2 values.  s_cos, s_sin [token][D]: element e of a rotated row is
-// v_e cos_e + v_partner sin_e, the sign of the first element's sine with it.
-template <int KIND, typename T, int LPH, bool STORE>
-__device__ __forceinline__ void do_rows(const RowArgs& a, const RowSpan& s, int t0, int nt, const float* s_cos, const float* s_sin, unsigned char* s_tile) {
+// Block b of row (token t, head h) of K or V into its slot: from the tile, or (tile == nullptr) from where the row lies.
+template <typename T, int BITS, int NB>
+__device__ __forceinline__ void pack_block(const RowArgs& a, const Codebook& cb, int side, long long t, unsigned h, unsigned b, const unsigned char* tile,
+                                           const float2* cells) {
+    const long long slot = a.slots[t];
+    if (slot < 0 || slot >= a.num_slots) return;
+    float v[32];
+    if (tile != nullptr) {
+        load_tile<T>(tile, v);
+    } else {
+        const RowSpan& s = side == 0 ? a.k : a.v;
+        load32<T>(reinterpret_cast<const T*>(s.in) + t * s.in_token + h * s.in_head + 32 * b, v);
+    }
+    uint32_t w[4];
+    const float scale = pqo_quantize_values<BITS>(v, cb, a.outer_centroid, w, cells);
+    const unsigned page = (unsigned)(slot >> a.page_shift), off = (unsigned)slot & ((1u << a.page_shift) - 1);   // (rows fit in 32 bits)
+    const size_t at = (size_t)(((page * (unsigned)a.kv_heads + h) << a.page_shift) + off) * NB + b;
+    uint8_t* to = a.idx[side] + at * (4 * BITS);
+    if (BITS == 4) {
+        *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+        uint32_t* wp = reinterpret_cast<uint32_t*>(to);
+        wp[0] = w[0];
+        wp[1] = w[1];
+        wp[2] = w[2];
+    }
+    a.sc[side][at] = f32_to_f16_bits(-scale);   // outlier blocks store -scale
+}
+
+// Rows that go into their slots as they are: a block a thread, from where it lies.
+template <typename T, int BITS, int NB>
+__global__ void __launch_bounds__(kRowThreads) append_kernel(const __grid_constant__ RowArgs a, const __grid_constant__ Codebook cb) {
+    __shared__ float2 s_cells[BITS == 3 ? kCells * 32 : 1];
+    if (BITS == 3) {
+        build_cell_table(cb, cb.n - 1, s_cells, threadIdx.x, kRowThreads);
+        __syncthreads();
+    }
+    const unsigned total = a.total;   // of a side
+    for (unsigned i = blockIdx.x * kRowThreads + threadIdx.x; i < total; i += gridDim.x * kRowThreads) {
+        const unsigned row = i / NB, tok = a.by_kv.of(row);
+        pack_block<T, BITS, NB>(a, cb, blockIdx.y, tok, row - tok * a.kv_heads, i % NB, nullptr, BITS == 3 ? s_cells + (threadIdx.x & 31) : nullptr);
+    }
+}
+
+// The heads of queries or keys of a token, passes `part`, part + parts, ..; STORE: into the tile too.  Element e of a rotated row is v_e cos_e + v_partner sin_e, the sign of the first element's sine with it.
+template <typename T, int LPH, bool STORE>
+__device__ __forceinline__ void do_rows(const RowArgs& a, const RowSpan& s, long long t, int part, int parts, const F2 (&co)[4], const F2 (&si)[4],
+                                        unsigned char* s_tile) {
     constexpr int D = LPH * 8, HPW = 32 / LPH, NB = D / 32;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LPH, l = lane % LPH;
-    const int rows = nt * s.heads, half = a.rot_dim >> 1;
-    const bool norm = KIND != 2 && (a.flags & TQB_ROPE_NO_NORM) == 0, inter = (a.flags & TQB_ROPE_INTERLEAVED) != 0;
-    const T* const in = reinterpret_cast<const T*>(s.in) + t0 * s.in_token + 8 * l;
-    T* const out = s.out == nullptr ? nullptr : reinterpret_cast<T*>(s.out) + t0 * s.out_token + 8 * l;
+    const int lane = threadIdx.x & 31, sub = lane / LPH, l = lane % LPH;
+    const bool norm = (a.flags & TQB_ROPE_NO_NORM) == 0, turn = a.rot_dim > 0, inter = (a.flags & TQB_ROPE_INTERLEAVED) != 0;
+    const int hl = a.rot_dim >> 4;   // lanes of half a rotated row
+    const bool turns = 8 * l < a.rot_dim;
+    const int from = lane + (!turns ? 0 : l < hl ? hl : -hl);
+    int h = part * HPW + sub;
+    if (h - sub >= s.heads) return;
     F2 w[4];
     if (norm) {
         float x[8];
@@ -350,140 +395,138 @@ __device__ __forceinline__ void do_rows(const RowArgs& a, const RowSpan& s, int 
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = f2(x[2 * i], x[2 * i + 1]);
     }
-    const int hl = half >> 3;   // lanes of half a rotated row
-    const bool turns = 8 * l < a.rot_dim;
-    const int from = lane + (!turns ? 0 : l < hl ? hl : -hl);
-    int r = warp * HPW + sub;
-    Eight<T> ahead;
-    auto fetch = [&](int row) {
-        const int at = min(row, rows - 1), tok = (int)s.by_heads.of(at);
-        ahead.load(in + tok * s.in_token + (at - tok * s.heads) * s.in_head);
+    const T* in = reinterpret_cast<const T*>(s.in) + t * s.in_token + min(h, s.heads - 1) * s.in_head + 8 * l;
+    T* out = reinterpret_cast<T*>(s.out) + t * s.out_token + h * s.out_head + 8 * l;
+    const int step = parts * HPW;
+    const long long in_step = step * s.in_head, out_step = step * s.out_head;
+    constexpr int kAhead = 1;   // passes in flight
+    Eight<T> ahead[kAhead];
+    auto fetch = [&](int k, int row) {   // (a lane without a head keeps to its last one)
+        if (row - sub >= s.heads) return;
+        ahead[k].load(in);
+        if (row + step < s.heads) in += in_step;
     };
-    if (warp * HPW < rows) fetch(r);
-    for (; r - sub < rows; r += kRowWarps * HPW) {   // (the same for the whole warp)
-        const bool live = r < rows;
-        const int at = min(r, rows - 1), tok = (int)s.by_heads.of(at), h = at - tok * s.heads;
-        Eight<T> e = ahead;
-        if (r - sub + kRowWarps * HPW < rows) fetch(r + kRowWarps * HPW);
-        if (KIND != 2 && (norm || half > 0)) {
-            float x[8];
-            e.get(x);
-            F2 v[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = f2(x[2 * i], x[2 * i + 1]);
-            if (norm) {
-                F2 ss = mul2(v[0], v[0]);
+    for (int k = 0; k < kAhead; ++k) fetch(k, h + k * step);
+    while (h - sub < s.heads) {   // (the same for the whole warp)
 #pragma unroll
-                for (int i = 1; i < 4; ++i) ss = fma2(v[i], v[i], ss);
-                const float2 t = halves(ss);
-                float sum = t.x + t.y;
+        for (int k = 0; k < kAhead; ++k) {
+            if (h - sub >= s.heads) break;
+            Eight<T> e = ahead[k];
+            fetch(k, h + kAhead * step);
+            if (norm || turn) {
+                float x[8];
+                e.get(x);
+                F2 v[4];
 #pragma unroll
-                for (int o = LPH / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                const F2 inv = f2(1.0f / sqrtf(sum * (1.0f / D) + a.eps));
+                for (int i = 0; i < 4; ++i) v[i] = f2(x[2 * i], x[2 * i + 1]);
+                if (norm) {
+                    F2 ss = mul2(v[0], v[0]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = mul2(mul2(v[i], inv), w[i]);
-            }
-            if (half > 0) {
-                F2 p[4];
-                if (inter) {
+                    for (int i = 1; i < 4; ++i) ss = fma2(v[i], v[i], ss);
+                    const float2 u = halves(ss);
+                    float sum = u.x + u.y;
+#pragma unroll
+                    for (int o = LPH / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    const F2 inv = f2(rsqrtf(sum * (1.0f / D) + a.eps));   // (two steps of 2^-24)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = mul2(mul2(v[i], inv), w[i]);
+                }
+                if (turn) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float2 t = halves(v[i]);
-                        p[i] = f2(t.y, t.x);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float2 t = halves(v[i]);
-                        const float p0 = __shfl_sync(0xffffffffu, t.x, from), p1 = __shfl_sync(0xffffffffu, t.y, from);
-                        p[i] = f2(p0, p1);
-                    }
-                }
-                if (turns) {
-                    const float4* c = reinterpret_cast<const float4*>(s_cos + tok * D + 8 * l);
-                    const float4* n = reinterpret_cast<const float4*>(s_sin + tok * D + 8 * l);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float4 ci = c[i], si = n[i];
-                        v[2 * i] = fma2(v[2 * i], f2(ci.x, ci.y), mul2(p[2 * i], f2(si.x, si.y)));
-                        v[2 * i + 1] = fma2(v[2 * i + 1], f2(ci.z, ci.w), mul2(p[2 * i + 1], f2(si.z, si.w)));
+                        const float2 u = halves(v[i]);
+                        F2 p;
+                        if (inter) {
+                            p = f2(u.y, u.x);
+                        } else {
+                            const float p0 = __shfl_sync(0xffffffffu, u.x, from), p1 = __shfl_sync(0xffffffffu, u.y, from);
+                            p = f2(p0, p1);
+                        }
+                        if (turns) v[i] = fma2(v[i], co[i], mul2(p, si[i]));
                     }
                 }
-            }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 t = halves(v[i]);
-                x[2 * i] = t.x;
-                x[2 * i + 1] = t.y;
+                for (int i = 0; i < 4; ++i) {
+                    const float2 u = halves(v[i]);
+                    x[2 * i] = u.x;
+                    x[2 * i + 1] = u.y;
+                }
+                e.set(x);
             }
-            e.set(x);
-        }
-        if (live) {
-            if (out != nullptr) e.store(out + tok * s.out_token + h * s.out_head);
-            if (STORE && KIND != 0)
-                e.store(reinterpret_cast<T*>(s_tile + (size_t)(((tok * 2 + KIND - 1) * a.kv_heads + h) * NB + (l >> 2)) * Tile<T>::kPitch) + 8 * (l & 3));
+            if (h < s.heads) {
+                if (s.out != nullptr) e.store(out);
+                if (STORE) e.store(reinterpret_cast<T*>(s_tile + (size_t)(h * NB + (l >> 2)) * Tile<T>::kPitch) + 8 * (l & 3));
+            }
+            out += out_step;
+            h += step;
         }
     }
 }
 
+// A token a warp; where there are few tokens (`shared_token`), a token a CTA.
 template <typename T, int LPH, int BITS>
 __global__ void __launch_bounds__(kRowThreads, BITS == 0 ? 4 : 3) rows_kernel(const __grid_constant__ RowArgs a, const __grid_constant__ Codebook cb) {
     constexpr int D = LPH * 8, NB = D / 32;
     extern __shared__ __align__(16) unsigned char s_dyn[];
-    const int half = a.rot_dim >> 1;
-    float* const s_cos = reinterpret_cast<float*>(s_dyn);                       // rot_dim != 0: [token][D]
-    float* const s_sin = s_cos + (half > 0 ? a.chunk * D : 0);
-    unsigned char* const s_tile = reinterpret_cast<unsigned char*>(s_sin + (half > 0 ? a.chunk * D : 0));   // BITS != 0: [token][K, V][head][block]
     __shared__ float2 s_cells[BITS == 3 ? kCells * 32 : 1];
-    const int tid = threadIdx.x, lane = tid & 31;
-    if (BITS == 3) build_cell_table(cb, cb.n - 1, s_cells, tid, kRowThreads);
-    for (int t0 = blockIdx.x * a.chunk; t0 < a.tokens; t0 += gridDim.x * a.chunk) {
-        const int nt = min(a.chunk, a.tokens - t0);
-        for (int i = tid; i < nt * half; i += kRowThreads) {
-            const int t = (int)a.by_half.of(i), f = i - t * half;
-            const double pos = (a.flags & TQB_ROPE_POSITIONS_64) ? (double)reinterpret_cast<const long long*>(a.positions)[t0 + t]
-                                                                : (double)reinterpret_cast<const int*>(a.positions)[t0 + t];
-            const double ang = pos * (double)a.inv_freq[f];
-            const double turns = rint(ang * 0.15915494309189535);
-            float si, co;
-            sincosf((float)fma(turns, -6.283185307179586, ang), &si, &co);
-            const bool inter = (a.flags & TQB_ROPE_INTERLEAVED) != 0;
-            const int first = t * D + (inter ? 2 * f : f), second = first + (inter ? 1 : half);
-            s_cos[first] = s_cos[second] = co;
-            s_sin[first] = -si;
-            s_sin[second] = si;
-        }
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, l = lane % LPH;
+    const int half = a.rot_dim >> 1, part = a.shared_token ? warp : 0, parts = a.shared_token ? kRowWarps : 1;
+    const int me = a.shared_token ? tid : lane, all = a.shared_token ? kRowThreads : 32;
+    unsigned char* const mine = s_dyn + (a.shared_token ? 0 : (size_t)warp * a.token_bytes);   // [cosines][sines][keys' blocks]
+    float* const s_cos = reinterpret_cast<float*>(mine);
+    float* const s_sin = s_cos + D;
+    unsigned char* const s_tile = mine + (half > 0 ? 2 * D * sizeof(float) : 0);
+    auto sync = [&]() {
+        if (a.shared_token) __syncthreads();
+        else __syncwarp();
+    };
+    if (BITS == 3) {
+        build_cell_table(cb, cb.n - 1, s_cells, tid, kRowThreads);
         __syncthreads();
-        if (a.q.heads > 0) do_rows<0, T, LPH, false>(a, a.q, t0, nt, s_cos, s_sin, s_tile);
-        if (a.k.heads > 0) do_rows<1, T, LPH, BITS != 0>(a, a.k, t0, nt, s_cos, s_sin, s_tile);
-        if constexpr (BITS != 0) {
-            do_rows<2, T, LPH, true>(a, a.v, t0, nt, s_cos, s_sin, s_tile);
-            __syncthreads();
-            const unsigned kv = (unsigned)a.kv_heads;
-            for (int i = tid; i < nt * 2 * a.kv_heads * NB; i += kRowThreads) {
-                const unsigned row = (unsigned)i / NB, ts = a.by_kv.of(row), h = row - ts * kv, b = (unsigned)i % NB;
-                const long long slot = a.slots[t0 + (ts >> 1)];
-                if (slot < 0 || slot >= a.num_slots) continue;
-                float v[32];
-                load_tile<T>(s_tile + (size_t)i * Tile<T>::kPitch, v);
-                uint32_t w[4];
-                const float scale = pqo_quantize_values<BITS>(v, cb, a.outer_centroid, w, BITS == 3 ? s_cells + lane : nullptr);
-                const int side = ts & 1;
-                const unsigned page = (unsigned)(slot >> a.page_shift), off = (unsigned)slot & ((1u << a.page_shift) - 1);   // (rows fit in 32 bits)
-                const size_t at = (size_t)(((page * kv + h) << a.page_shift) + off) * NB + b;
-                uint8_t* to = a.idx[side] + at * (4 * BITS);
-                if (BITS == 4) {
-                    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-                } else {
-                    uint32_t* wp = reinterpret_cast<uint32_t*>(to);
-                    wp[0] = w[0];
-                    wp[1] = w[1];
-                    wp[2] = w[2];
-                }
-                a.sc[side][at] = f32_to_f16_bits(-scale);   // outlier blocks store -scale
+    }
+    const int per_cta = a.shared_token ? 1 : kRowWarps;
+    for (int t = blockIdx.x * per_cta + (a.shared_token ? 0 : warp); t < a.tokens; t += gridDim.x * per_cta) {
+        if (half > 0) {
+            const double pos = (a.flags & TQB_ROPE_POSITIONS_64) ? (double)reinterpret_cast<const long long*>(a.positions)[t]
+                                                                : (double)reinterpret_cast<const int*>(a.positions)[t];
+            const bool inter = (a.flags & TQB_ROPE_INTERLEAVED) != 0;
+            for (int f = me; f < half; f += all) {
+                const double ang = pos * (double)a.inv_freq[f];
+                const double turns = rint(ang * 0.15915494309189535);
+                float si, co;
+                sincosf((float)fma(turns, -6.283185307179586, ang), &si, &co);
+                const int first = inter ? 2 * f : f, second = first + (inter ? 1 : half);
+                s_cos[first] = s_cos[second] = co;
+                s_sin[first] = -si;
+                s_sin[second] = si;
+            }
+            sync();
+        }
+        F2 co[4], si[4];
+        if (half > 0) {
+            const float4* c = reinterpret_cast<const float4*>(s_cos + 8 * l);
+            const float4* n = reinterpret_cast<const float4*>(s_sin + 8 * l);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                co[2 * i] = f2(c[i].x, c[i].y);
+                co[2 * i + 1] = f2(c[i].z, c[i].w);
+                si[2 * i] = f2(n[i].x, n[i].y);
+                si[2 * i + 1] = f2(n[i].z, n[i].w);
             }
         }
-        __syncthreads();   // angles and tile are free again
+        if (a.q.heads > 0) do_rows<T, LPH, false>(a, a.q, t, part, parts, co, si, s_tile);
+        if (a.k.heads > 0) do_rows<T, LPH, BITS != 0>(a, a.k, t, part, parts, co, si, s_tile);
+        if constexpr (BITS != 0) {
+            sync();
+            const int per_side = a.kv_heads * NB;
+            for (int i = me; i < 2 * per_side; i += all) {   // [K, V][head][block]
+                const int side = i >= per_side ? 1 : 0, at = i - side * per_side;
+                pack_block<T, BITS, NB>(a, cb, side, t, (unsigned)at / NB, (unsigned)at % NB, side == 0 ? s_tile + (size_t)at * Tile<T>::kPitch : nullptr,
+                                        BITS == 3 ? s_cells + lane : nullptr);
+            }
+        }
+        sync();   // angles and tile are free again
     }
 }
 
@@ -549,18 +592,22 @@ __global__ void __launch_bounds__(kRowThreads, 4) back_kernel(const __grid_const
         for (int k = 0; k < 4; ++k) {
             float e[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = live ? v[8 * k + i] : 0.0f;
+            for (int i = 0; i < 8; ++i) e[i] = v[8 * k + i];
             Eight<T> x;
             x.set(e);
             x.store(reinterpret_cast<T*>(stage + lane * kPitch) + 8 * k);
         }
+        if (!live) {   // a slot outside the pages
+            for (int i = 0; i < kPieces; ++i) *reinterpret_cast<uint4*>(stage + lane * kPitch + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
         __syncwarp();
-        unsigned char* out = reinterpret_cast<unsigned char*>(a.out[side]) + (size_t)blk0 * (32 * sizeof(T));
+        unsigned char* out = reinterpret_cast<unsigned char*>(a.out[side]) + (size_t)blk0 * (32 * sizeof(T)) + lane * 16;
+        const bool full = blk0 + 32 <= total;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
             const int q = 32 * i + lane;
             const uint4 r = *reinterpret_cast<const uint4*>(stage + (q / kPieces) * kPitch + (q % kPieces) * 16);
-            if (blk0 + q / kPieces < total) *reinterpret_cast<uint4*>(out + q * 16) = r;
+            if (full || blk0 + q / kPieces < total) *reinterpret_cast<uint4*>(out + i * 512) = r;
         }
         __syncwarp();
     }
@@ -586,18 +633,36 @@ int check_rows(const void* p, long long token, long long head, size_t elem) {
 
 template <typename T, int LPH, int BITS>
 int launch_rows_one(RowArgs& a, const Codebook& cb, cudaStream_t s) {
-    // As many tokens at a time as make kRowBlocks blocks; fewer while that leaves SMs idle.
-    const int blocks = BITS == 0 ? 0 : 2 * a.kv_heads * (LPH / 4);
-    const size_t token = (size_t)blocks * Tile<T>::kPitch + (a.rot_dim > 0 ? (size_t)LPH * 8 * 2 * sizeof(float) : 0);
-    if (token > 160 * 1024) return TQB_ERR_UNSUPPORTED;
     a.by_kv = Divisor((unsigned)(a.kv_heads > 0 ? a.kv_heads : 1));
-    a.by_half = Divisor((unsigned)(a.rot_dim > 0 ? a.rot_dim / 2 : 1));
-    a.chunk = BITS == 0 ? kRowTokens : (kRowBlocks + blocks - 1) / blocks;
-    while (a.chunk > 1 && (a.tokens < 148 * a.chunk || token * a.chunk > 64 * 1024)) a.chunk >>= 1;
-    const int bytes = (int)(token * a.chunk);
-    if (int st = allow_shared<rows_kernel<T, LPH, BITS>>(bytes, 160 * 1024)) return st;
-    const int want = (a.tokens + a.chunk - 1) / a.chunk, most = 148 * (BITS == 0 ? 4 : 3);
-    rows_kernel<T, LPH, BITS><<<want < most ? want : most, kRowThreads, bytes, s>>>(a, cb);
+    const long long blocks_of_token = (long long)a.kv_heads * (LPH / 4);
+    if constexpr (BITS != 0) {
+        if (a.q.heads == 0 && a.k.out == nullptr && (a.flags & TQB_ROPE_NO_NORM) != 0 && a.rot_dim == 0) {
+            const long long most = ((1ll << 31) - (1 << 20)) / blocks_of_token;   // tokens of a launch
+            if (most < 1) return TQB_ERR_TOO_LARGE;
+            RowArgs b = a;
+            for (long long done = 0; done < a.tokens; done += most) {
+                const long long now = a.tokens - done < most ? a.tokens - done : most;
+                b.k.in = reinterpret_cast<const T*>(a.k.in) + done * a.k.in_token;
+                b.v.in = reinterpret_cast<const T*>(a.v.in) + done * a.v.in_token;
+                b.slots = a.slots + done;
+                b.total = (unsigned)(now * blocks_of_token);
+                const long long want = (b.total + kRowThreads - 1) / kRowThreads;
+                append_kernel<T, BITS, LPH / 4><<<dim3((unsigned)(want < 148 * 16 ? want : 148 * 16), 2), kRowThreads, 0, s>>>(b, cb);
+                if (int e = check_launch(s)) return e;
+            }
+            return TQB_OK;
+        }
+    }
+    const size_t token = (BITS == 0 ? 0 : (size_t)blocks_of_token * Tile<T>::kPitch) + (a.rot_dim > 0 ? (size_t)LPH * 8 * 2 * sizeof(float) : 0);
+    if (token > 128 * 1024) return TQB_ERR_UNSUPPORTED;
+    a.token_bytes = (int)token;
+    // A warp has some 20 passes a token: below as many tokens as two warps an SM scheduler want, and where eight tokens take too
+    // much room, a CTA shares them.
+    a.shared_token = a.tokens < 148 * 8 || token * kRowWarps > 72 * 1024 ? 1 : 0;
+    const int bytes = (int)(token * (a.shared_token ? 1 : kRowWarps));
+    if (int st = allow_shared<rows_kernel<T, LPH, BITS>>(bytes, 128 * 1024)) return st;
+    const long long want = a.shared_token ? a.tokens : (a.tokens + kRowWarps - 1) / kRowWarps;
+    rows_kernel<T, LPH, BITS><<<(unsigned)(want < 148 * 32 ? want : 148 * 32), kRowThreads, bytes, s>>>(a, cb);
     return check_launch(s);
 }
 template <typename T, int LPH>
@@ -643,13 +708,13 @@ int rope_args(const tqb_rope_params* p, bool keys_out, RowArgs& a) {
         if ((st = check_rows(p->q, p->q_token_stride, p->q_head_stride, elem)) != TQB_OK) return st;
         if ((st = check_rows(p->q_out, p->q_out_token_stride, p->q_out_head_stride, elem)) != TQB_OK) return st;
         if (!aligned16(p->q_weight)) return TQB_ERR_MISALIGNED;
-        a.q = RowSpan{p->q, p->q_out, p->q_token_stride, p->q_head_stride, p->q_out_token_stride, p->q_out_head_stride, p->q_weight, p->num_q_heads, Divisor((unsigned)(p->num_q_heads > 0 ? p->num_q_heads : 1))};
+        a.q = RowSpan{p->q, p->q_out, p->q_token_stride, p->q_head_stride, p->q_out_token_stride, p->q_out_head_stride, p->q_weight, p->num_q_heads};
     }
     if (p->k) {
         if ((st = check_rows(p->k, p->k_token_stride, p->k_head_stride, elem)) != TQB_OK) return st;
         if (p->k_out && (st = check_rows(p->k_out, p->k_out_token_stride, p->k_out_head_stride, elem)) != TQB_OK) return st;
         if (!aligned16(p->k_weight)) return TQB_ERR_MISALIGNED;
-        a.k = RowSpan{p->k, p->k_out, p->k_token_stride, p->k_head_stride, p->k_out_token_stride, p->k_out_head_stride, p->k_weight, p->num_kv_heads, Divisor((unsigned)(p->num_kv_heads > 0 ? p->num_kv_heads : 1))};
+        a.k = RowSpan{p->k, p->k_out, p->k_token_stride, p->k_head_stride, p->k_out_token_stride, p->k_out_head_stride, p->k_weight, p->num_kv_heads};
     }
     a.positions = p->positions;
     a.inv_freq = p->inv_freq;
@@ -760,8 +825,8 @@ int tqb_paged_append(const tqb_paged_layer* layer, const void* k, int64_t k_toke
     if ((st = check_rows(v, v_token_stride, v_head_stride, elem)) != TQB_OK) return st;
     RowArgs a{};
     if ((st = layer_args(layer, slots, a)) != TQB_OK) return st;
-    a.k = RowSpan{k, nullptr, k_token_stride, k_head_stride, 0, 0, nullptr, layer->num_kv_heads, Divisor((unsigned)layer->num_kv_heads)};
-    a.v = RowSpan{v, nullptr, v_token_stride, v_head_stride, 0, 0, nullptr, layer->num_kv_heads, Divisor((unsigned)layer->num_kv_heads)};
+    a.k = RowSpan{k, nullptr, k_token_stride, k_head_stride, 0, 0, nullptr, layer->num_kv_heads};
+    a.v = RowSpan{v, nullptr, v_token_stride, v_head_stride, 0, 0, nullptr, layer->num_kv_heads};
     a.tokens = num_tokens;
     a.flags = TQB_ROPE_NO_NORM;
     return launch_rows(dtype, layer->head_dim, layer->bits, a, as_stream(stream));
@@ -779,7 +844,7 @@ int tqb_paged_append_rope(const tqb_paged_layer* layer, const tqb_rope_params* p
     if (!p->k || !v) return TQB_ERR_NULL_POINTER;
     if ((st = check_rows(v, v_token_stride, v_head_stride, size_of(p->dtype))) != TQB_OK) return st;
     if ((st = layer_args(layer, slots, a)) != TQB_OK) return st;
-    a.v = RowSpan{v, nullptr, v_token_stride, v_head_stride, 0, 0, nullptr, layer->num_kv_heads, Divisor((unsigned)layer->num_kv_heads)};
+    a.v = RowSpan{v, nullptr, v_token_stride, v_head_stride, 0, 0, nullptr, layer->num_kv_heads};
     return launch_rows(p->dtype, p->head_dim, layer->bits, a, as_stream(stream));
 }
 
