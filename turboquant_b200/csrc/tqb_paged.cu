@@ -1,6 +1,7 @@
 // Paged cache: block tables and slot maps from lengths, the rows that go into pages (norm, rotation and packing in one pass)
 // and the rows that come back from them.  The attention over the pages is in tqb_paged_attention.cu.
 #include "tqb_common.cuh"
+#include "tqb_mma.cuh"
 #include "tqb_paged.cuh"
 #include "tqb_pqo_dequant.cuh"
 #include "tqb_pqo_quant.cuh"
@@ -194,8 +195,8 @@ __global__ void __launch_bounds__(kReleaseThreads) release_kernel(const uint8_t*
 
 // ---- rows into pages, with norm and rotation ---------------------------------------------------------------------------
 // A warp takes a token (a CTA, where there are few): its angles, its rows, its blocks.
-// Angles: position * inv_freq in f64, less whole turns, then sincosf in f32 (an f32 product would be off by position * 2^-24,
-//   0.06 rad at a million tokens), once for a token.
+// Angles: turns = position * inv_freq / 2 pi in f64, less whole ones, then sine and cosine in f32 (an f32 product would be off by
+//   position * 2^-24, 0.06 rad at a million tokens), once for a token.
 // Rows: one warp pass takes 32 / (D / 8) heads of a token, eight consecutive elements a lane: every load and store of a warp is
 //   dense, the norm's sum and the partner of a rotated pair are shuffles away.  The next pass's load is in flight.  Queries
 //   leave for q_out; keys go to a tile of 32-blocks in shared memory, in their type.
@@ -370,10 +371,11 @@ __global__ void __launch_bounds__(kRowThreads) append_kernel(const __grid_consta
     }
 }
 
-// The heads of queries or keys of a token, passes `part`, part + parts, ..; STORE: into the tile too.  Element e of a rotated row is v_e cos_e + v_partner sin_e, the sign of the first element's sine with it.
+// The heads of queries or keys of a token, passes `part`, part + parts, .., where only the first rot_dim elements turn; STORE:
+// into the tile too.  Eight elements a lane; the partner of a pair may be in another lane.  s_cos, s_sin [rot_dim / 2].
 template <typename T, int LPH, bool STORE>
-__device__ __forceinline__ void do_rows(const RowArgs& a, const RowSpan& s, long long t, int part, int parts, const F2 (&co)[4], const F2 (&si)[4],
-                                        unsigned char* s_tile) {
+__device__ __forceinline__ void do_rows_part(const RowArgs& a, const RowSpan& s, long long t, int part, int parts, const float* s_cos, const float* s_sin,
+                                             unsigned char* s_tile) {
     constexpr int D = LPH * 8, HPW = 32 / LPH, NB = D / 32;
     const int lane = threadIdx.x & 31, sub = lane / LPH, l = lane % LPH;
     const bool norm = (a.flags & TQB_ROPE_NO_NORM) == 0, turn = a.rot_dim > 0, inter = (a.flags & TQB_ROPE_INTERLEAVED) != 0;
@@ -382,6 +384,16 @@ __device__ __forceinline__ void do_rows(const RowArgs& a, const RowSpan& s, long
     const int from = lane + (!turns ? 0 : l < hl ? hl : -hl);
     int h = part * HPW + sub;
     if (h - sub >= s.heads) return;
+    // element e of a rotated row is v_e cos_e + v_partner sin_e, the sign of the first element's sine with it
+    F2 co[4], si[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int f = inter ? 4 * l + i : 8 * (l < hl ? l : l - hl) + 2 * i;
+        const int f0 = turns ? f : 0, f1 = turns && !inter ? f + 1 : f0;
+        const float s0 = s_sin[f0], s1 = s_sin[f1];
+        co[i] = f2(s_cos[f0], s_cos[f1]);
+        si[i] = inter ? f2(-s0, s0) : l < hl ? f2(-s0, -s1) : f2(s0, s1);
+    }
     F2 w[4];
     if (norm) {
         float x[8];
@@ -464,19 +476,221 @@ __device__ __forceinline__ void do_rows(const RowArgs& a, const RowSpan& s, long
     }
 }
 
-// A token a warp; where there are few tokens (`shared_token`), a token a CTA.
-template <typename T, int LPH, int BITS>
-__global__ void __launch_bounds__(kRowThreads, BITS == 0 ? 4 : 3) rows_kernel(const __grid_constant__ RowArgs a, const __grid_constant__ Codebook cb) {
+// The same where whole rows turn, or nothing does: a lane has eight elements of the first half of a row and the eight half a
+// row behind them, so that both elements of a pair are its own, and a pass takes 32 / (D / 16) heads.  Half the
+// instructions a row of do_rows_part, which is what bounds this kernel: 8,191 tokens of 32 + 8 heads 45 us with it.
+// A pass is 32 / (D / 16) heads of queries, or of keys, of a token; passes are numbered token after token, queries before keys.
+// They are copied to a ring in shared memory, kDepth of them ahead; a lane reads what it has copied itself.
+template <typename T, int LPH, bool STORE>
+struct Rows {
+    static constexpr int D = LPH * 8, LPR = LPH / 2, HPW = 32 / LPR, NB = D / 32;
+    static constexpr int kDepth = 8 / (int)sizeof(T), kLane = 16 * (int)sizeof(T), kSlot = 32 * kLane;   // passes in flight, bytes a lane and a pass
+    const RowArgs& a;
+    const int sub, l, passes_q, passes, part, parts;   // of a token's passes the warp takes part, part + parts, ..
+    int token, pass, left, token_step;                 // what is copied next, and how many passes still
+    uint32_t to, ring;                                 // shared addresses of the lane's next slot and of its first
+    const unsigned char *from, *s_ring;                // the lane's slot that is read next, and its first
+
+    static __host__ __device__ __forceinline__ int passes_of(int heads) { return (heads + HPW - 1) / HPW; }
+
+    __device__ __forceinline__ Rows(const RowArgs& args, int token_, int pass_, int left_, int part_, int parts_, int step, unsigned char* space)
+        : a(args), sub((threadIdx.x & 31) / LPR), l((threadIdx.x & 31) % LPR), passes_q(passes_of(args.q.heads)),
+          passes(passes_q + passes_of(args.k.heads)), part(part_), parts(parts_), token(token_), pass(pass_), left(left_), token_step(step) {
+        s_ring = from = space + (threadIdx.x & 31) * kLane;
+        to = ring = (uint32_t)__cvta_generic_to_shared(s_ring);
+#pragma unroll 1
+        for (int k = 0; k < kDepth; ++k) fetch();
+    }
+    __device__ __forceinline__ void fetch() {
+        if (left > 0) {
+            --left;
+            const RowSpan& s = pass < passes_q ? a.q : a.k;
+            const int h = min((pass < passes_q ? pass : pass - passes_q) * HPW + sub, s.heads - 1);   // (a lane without a head reads the last one)
+            const T* in = reinterpret_cast<const T*>(s.in) + token * s.in_token + h * s.in_head + 8 * l;
+#pragma unroll
+            for (int k = 0; k < (int)sizeof(T) / 2; ++k) {
+                cp_async16(to + 32 * k, reinterpret_cast<const unsigned char*>(in) + 16 * k);
+                cp_async16(to + 32 * k + 16, reinterpret_cast<const unsigned char*>(in + D / 2) + 16 * k);
+            }
+            pass += parts;
+            if (pass >= passes) {
+                pass = part;
+                token += token_step;
+            }
+        }
+        cp_async_commit();
+        to = to + kSlot == ring + kDepth * kSlot ? ring : to + kSlot;
+    }
+    // The two eights of the pass that is due; its slot is filled again.
+    __device__ __forceinline__ void take(Eight<T> (&e)[2]) {
+        cp_async_wait<kDepth - 1>();
+        uint4 r[sizeof(T)];
+#pragma unroll
+        for (int k = 0; k < (int)sizeof(T); ++k) r[k] = *reinterpret_cast<const uint4*>(from + 16 * k);
+        from = from + kSlot == s_ring + kDepth * kSlot ? s_ring : from + kSlot;
+        __syncwarp();
+        if constexpr (sizeof(T) == 2) {
+            e[0].r = r[0];
+            e[1].r = r[1];
+        } else {
+            e[0].a = *reinterpret_cast<float4*>(&r[0]);
+            e[1].a = *reinterpret_cast<float4*>(&r[1]);
+            e[0].b = *reinterpret_cast<float4*>(&r[2]);
+            e[1].b = *reinterpret_cast<float4*>(&r[3]);
+        }
+        fetch();
+    }
+    // Passes p0, p0 + parts, .. below p1 of token t.
+    __device__ __forceinline__ void run(int t, int p0, int p1, const float* s_cos, const float* s_sin, unsigned char* s_tile) {
+        const bool norm = (a.flags & TQB_ROPE_NO_NORM) == 0, turn = a.rot_dim > 0, inter = (a.flags & TQB_ROPE_INTERLEAVED) != 0;
+        float co[8], si[8];   // of the lane's pairs: (i, i + 8), or of neighbours
+        if (turn) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int f = inter ? k * (D / 4) + 4 * l : 8 * l + 4 * k;
+                const float4 c = *reinterpret_cast<const float4*>(s_cos + f), n = *reinterpret_cast<const float4*>(s_sin + f);
+                co[4 * k] = c.x; co[4 * k + 1] = c.y; co[4 * k + 2] = c.z; co[4 * k + 3] = c.w;
+                si[4 * k] = n.x; si[4 * k + 1] = n.y; si[4 * k + 2] = n.z; si[4 * k + 3] = n.w;
+            }
+        }
+        Eight<T> w[2];
+        bool weighted = false, fresh = true;
+        for (int p = p0; p < p1; p += parts) {
+            const bool keys = p >= passes_q;
+            const RowSpan& s = keys ? a.k : a.q;
+            const int h = (keys ? p - passes_q : p) * HPW + sub;
+            if (fresh || (keys && p - parts < passes_q)) {   // a tensor begins
+                fresh = false;
+                weighted = norm && s.weight != nullptr;
+                if (weighted) {
+                    w[0].load(reinterpret_cast<const T*>(s.weight) + 8 * l);
+                    w[1].load(reinterpret_cast<const T*>(s.weight) + D / 2 + 8 * l);
+                }
+            }
+            Eight<T> e[2];
+            take(e);
+            if (norm || turn) {
+                float x[2][8];
+                e[0].get(x[0]);
+                e[1].get(x[1]);
+                if (norm) {
+                    F2 ss = f2(0.0f);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const F2 v = f2(x[i >> 2][2 * (i & 3)], x[i >> 2][2 * (i & 3) + 1]);
+                        ss = fma2(v, v, ss);
+                    }
+                    const float2 u = halves(ss);
+                    float sum = u.x + u.y;
+#pragma unroll
+                    for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    const float inv = rsqrtf(sum * (1.0f / D) + a.eps);   // (two steps of 2^-24)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        float wk[8];
+                        if (weighted) w[k].get(wk);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            x[k][i] *= inv;
+                            if (weighted) x[k][i] *= wk[i];
+                        }
+                    }
+                }
+                if (turn) {
+                    if (inter) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float y = x[i >> 2][2 * (i & 3)], z = x[i >> 2][2 * (i & 3) + 1];
+                            x[i >> 2][2 * (i & 3)] = fmaf(y, co[i], -(z * si[i]));
+                            x[i >> 2][2 * (i & 3) + 1] = fmaf(z, co[i], y * si[i]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float y = x[0][i], z = x[1][i];
+                            x[0][i] = fmaf(y, co[i], -(z * si[i]));
+                            x[1][i] = fmaf(z, co[i], y * si[i]);
+                        }
+                    }
+                }
+                e[0].set(x[0]);
+                e[1].set(x[1]);
+            }
+            if (h < s.heads) {
+                if (s.out != nullptr) {
+                    T* out = reinterpret_cast<T*>(s.out) + t * s.out_token + h * s.out_head + 8 * l;
+                    e[0].store(out);
+                    e[1].store(out + D / 2);
+                }
+                if (STORE && keys) {
+                    unsigned char* at = s_tile + (size_t)(h * NB + (l >> 2)) * Tile<T>::kPitch + 8 * (l & 3) * sizeof(T);
+                    e[0].store(reinterpret_cast<T*>(at));
+                    e[1].store(reinterpret_cast<T*>(at + NB / 2 * Tile<T>::kPitch));
+                }
+            }
+        }
+    }
+};
+
+constexpr int kRingBytes = 4096;   // of a warp: Rows::kDepth * Rows::kSlot
+
+// Cosines and sines of a token's angles, by `all` threads of which this is number `me`.
+__device__ __forceinline__ void angles(const RowArgs& a, int t, float* s_cos, float* s_sin, int me, int all) {
+    const double pos = (a.flags & TQB_ROPE_POSITIONS_64) ? (double)reinterpret_cast<const long long*>(a.positions)[t]
+                                                        : (double)reinterpret_cast<const int*>(a.positions)[t];
+    for (int f = me; f < a.rot_dim >> 1; f += all) {
+        const double turns = pos * (double)a.inv_freq[f] * 0.15915494309189535;
+        float si, co;
+        sincospif((float)(2.0 * (turns - rint(turns))), &si, &co);
+        s_cos[f] = co;
+        s_sin[f] = si;
+    }
+}
+
+// Norm and rotation alone, whole rows turning: every warp takes an equal run of the passes, a token's angles for itself.  By
+// whole tokens a warp 8,191 tokens were two or three rounds: 45 us.
+template <typename T, int LPH>
+__global__ void __launch_bounds__(kRowThreads, 3) turn_kernel(const __grid_constant__ RowArgs a) {
+    using R = Rows<T, LPH, false>;
+    extern __shared__ __align__(16) unsigned char s_dyn[];   // [warp]: ring, cosines, sines
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    unsigned char* const mine = s_dyn + warp * (kRingBytes + R::D * (int)sizeof(float));
+    float* const s_cos = reinterpret_cast<float*>(mine + kRingBytes);
+    float* const s_sin = s_cos + R::D / 2;
+    const int passes = R::passes_of(a.q.heads) + R::passes_of(a.k.heads);
+    const long long total = (long long)a.tokens * passes, warps = (long long)gridDim.x * kRowWarps, w = (long long)blockIdx.x * kRowWarps + warp;
+    const long long quot = total / warps, rem = total - quot * warps, begin = w * quot + (w < rem ? w : rem);
+    int left = (int)(quot + (w < rem ? 1 : 0));
+    if (left == 0) return;
+    int t = (int)(begin / passes), p = (int)(begin - (long long)t * passes);
+    R rows(a, t, p, left, 0, 1, 1, mine);
+    for (; left > 0; ++t, p = 0) {
+        const int n = min(left, passes - p);
+        if (a.rot_dim > 0) {
+            angles(a, t, s_cos, s_sin, lane, 32);
+            __syncwarp();
+        }
+        rows.run(t, p, p + n, s_cos, s_sin, nullptr);
+        __syncwarp();   // the angles have been read
+        left -= n;
+    }
+}
+
+// Rows that are packed (BITS != 0), or of which only the first rot_dim elements turn (PART): a token a warp; where there are few
+// tokens (`shared_token`), a token a CTA.
+template <typename T, int LPH, int BITS, bool PART>
+__global__ void __launch_bounds__(kRowThreads, 3) rows_kernel(const __grid_constant__ RowArgs a, const __grid_constant__ Codebook cb) {
     constexpr int D = LPH * 8, NB = D / 32;
+    using R = Rows<T, LPH, true>;
     extern __shared__ __align__(16) unsigned char s_dyn[];
     __shared__ float2 s_cells[BITS == 3 ? kCells * 32 : 1];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, l = lane % LPH;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int half = a.rot_dim >> 1, part = a.shared_token ? warp : 0, parts = a.shared_token ? kRowWarps : 1;
     const int me = a.shared_token ? tid : lane, all = a.shared_token ? kRowThreads : 32;
-    unsigned char* const mine = s_dyn + (a.shared_token ? 0 : (size_t)warp * a.token_bytes);   // [cosines][sines][keys' blocks]
+    unsigned char* const mine = s_dyn + (PART ? 0 : kRowWarps * kRingBytes) + (a.shared_token ? 0 : (size_t)warp * a.token_bytes);   // [cosines][sines][keys' blocks]
     float* const s_cos = reinterpret_cast<float*>(mine);
-    float* const s_sin = s_cos + D;
-    unsigned char* const s_tile = mine + (half > 0 ? 2 * D * sizeof(float) : 0);
+    float* const s_sin = s_cos + D / 2;
+    unsigned char* const s_tile = mine + (half > 0 ? D * sizeof(float) : 0);
     auto sync = [&]() {
         if (a.shared_token) __syncthreads();
         else __syncwarp();
@@ -485,38 +699,22 @@ __global__ void __launch_bounds__(kRowThreads, BITS == 0 ? 4 : 3) rows_kernel(co
         build_cell_table(cb, cb.n - 1, s_cells, tid, kRowThreads);
         __syncthreads();
     }
-    const int per_cta = a.shared_token ? 1 : kRowWarps;
-    for (int t = blockIdx.x * per_cta + (a.shared_token ? 0 : warp); t < a.tokens; t += gridDim.x * per_cta) {
-        if (half > 0) {
-            const double pos = (a.flags & TQB_ROPE_POSITIONS_64) ? (double)reinterpret_cast<const long long*>(a.positions)[t]
-                                                                : (double)reinterpret_cast<const int*>(a.positions)[t];
-            const bool inter = (a.flags & TQB_ROPE_INTERLEAVED) != 0;
-            for (int f = me; f < half; f += all) {
-                const double ang = pos * (double)a.inv_freq[f];
-                const double turns = rint(ang * 0.15915494309189535);
-                float si, co;
-                sincosf((float)fma(turns, -6.283185307179586, ang), &si, &co);
-                const int first = inter ? 2 * f : f, second = first + (inter ? 1 : half);
-                s_cos[first] = s_cos[second] = co;
-                s_sin[first] = -si;
-                s_sin[second] = si;
-            }
+    const int per_cta = a.shared_token ? 1 : kRowWarps, step = gridDim.x * per_cta;
+    for (int t = blockIdx.x * per_cta + (a.shared_token ? 0 : warp); t < a.tokens; t += step) {
+        if constexpr (PART) {
+            angles(a, t, s_cos, s_sin, me, all);
             sync();
-        }
-        F2 co[4], si[4];
-        if (half > 0) {
-            const float4* c = reinterpret_cast<const float4*>(s_cos + 8 * l);
-            const float4* n = reinterpret_cast<const float4*>(s_sin + 8 * l);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                co[2 * i] = f2(c[i].x, c[i].y);
-                co[2 * i + 1] = f2(c[i].z, c[i].w);
-                si[2 * i] = f2(n[i].x, n[i].y);
-                si[2 * i + 1] = f2(n[i].z, n[i].w);
+            if (a.q.heads > 0) do_rows_part<T, LPH, false>(a, a.q, t, part, parts, s_cos, s_sin, s_tile);
+            if (a.k.heads > 0) do_rows_part<T, LPH, BITS != 0>(a, a.k, t, part, parts, s_cos, s_sin, s_tile);
+        } else {
+            const int passes = R::passes_of(a.q.heads) + R::passes_of(a.k.heads);
+            R rows(a, t, part, max(0, (passes - part + parts - 1) / parts), part, parts, 1, s_dyn + (size_t)warp * kRingBytes);
+            if (half > 0) {
+                angles(a, t, s_cos, s_sin, me, all);
+                sync();
             }
+            rows.run(t, part, passes, s_cos, s_sin, s_tile);
         }
-        if (a.q.heads > 0) do_rows<T, LPH, false>(a, a.q, t, part, parts, co, si, s_tile);
-        if (a.k.heads > 0) do_rows<T, LPH, BITS != 0>(a, a.k, t, part, parts, co, si, s_tile);
         if constexpr (BITS != 0) {
             sync();
             const int per_side = a.kv_heads * NB;
@@ -653,16 +851,33 @@ int launch_rows_one(RowArgs& a, const Codebook& cb, cudaStream_t s) {
             return TQB_OK;
         }
     }
-    const size_t token = (BITS == 0 ? 0 : (size_t)blocks_of_token * Tile<T>::kPitch) + (a.rot_dim > 0 ? (size_t)LPH * 8 * 2 * sizeof(float) : 0);
+    const size_t token = (BITS == 0 ? 0 : (size_t)blocks_of_token * Tile<T>::kPitch) + (a.rot_dim > 0 ? (size_t)LPH * 8 * sizeof(float) : 0);
     if (token > 128 * 1024) return TQB_ERR_UNSUPPORTED;
     a.token_bytes = (int)token;
     // A warp has some 20 passes a token: below as many tokens as two warps an SM scheduler want, and where eight tokens take too
     // much room, a CTA shares them.
     a.shared_token = a.tokens < 148 * 8 || token * kRowWarps > 72 * 1024 ? 1 : 0;
-    const int bytes = (int)(token * (a.shared_token ? 1 : kRowWarps));
-    if (int st = allow_shared<rows_kernel<T, LPH, BITS>>(bytes, 128 * 1024)) return st;
+    const bool partly = a.rot_dim > 0 && a.rot_dim < LPH * 8;
+    const int bytes = (int)(token * (a.shared_token ? 1 : kRowWarps)) + (partly ? 0 : kRowWarps * kRingBytes);
+    if constexpr (BITS == 0) {
+        if (!partly) {
+            using R = Rows<T, LPH, false>;
+            const int dyn = kRowWarps * (kRingBytes + R::D * (int)sizeof(float));
+            if (int st = allow_shared<turn_kernel<T, LPH>>(dyn)) return st;
+            const long long passes = (long long)a.tokens * (R::passes_of(a.q.heads) + R::passes_of(a.k.heads)), want = (passes + kRowWarps - 1) / kRowWarps;
+            turn_kernel<T, LPH><<<(unsigned)(want < 148 * 3 ? want : 148 * 3), kRowThreads, dyn, s>>>(a);
+            return check_launch(s);
+        }
+    }
     const long long want = a.shared_token ? a.tokens : (a.tokens + kRowWarps - 1) / kRowWarps;
-    rows_kernel<T, LPH, BITS><<<(unsigned)(want < 148 * 32 ? want : 148 * 32), kRowThreads, bytes, s>>>(a, cb);
+    const unsigned grid = (unsigned)(want < 148 * 32 ? want : 148 * 32);
+    if (partly) {
+        if (int st = allow_shared<rows_kernel<T, LPH, BITS, true>>(bytes, 160 * 1024)) return st;
+        rows_kernel<T, LPH, BITS, true><<<grid, kRowThreads, bytes, s>>>(a, cb);
+    } else if constexpr (BITS != 0) {
+        if (int st = allow_shared<rows_kernel<T, LPH, BITS, false>>(bytes, 160 * 1024)) return st;
+        rows_kernel<T, LPH, BITS, false><<<grid, kRowThreads, bytes, s>>>(a, cb);
+    }
     return check_launch(s);
 }
 template <typename T, int LPH>
