@@ -214,7 +214,7 @@ struct Divisor {
         while ((1ull << s) < d) ++s;
         m = (unsigned)(((1ull << (31 + s)) / d) + 1);
     }
-    Divisor() : d(1), m(0), s(0) {}
+    __host__ __device__ Divisor() : d(1), m(0x80000001u), s(0) {}   // by 1
     __device__ __forceinline__ unsigned of(unsigned x) const { return (unsigned)(((unsigned long long)x * m) >> (31 + s)); }
 };
 
@@ -358,7 +358,7 @@ __device__ __forceinline__ void pack_block(const RowArgs& a, const Codebook& cb,
 
 // Rows that go into their slots as they are: a block a thread, from where it lies.
 template <typename T, int BITS, int NB>
-__global__ void __launch_bounds__(kRowThreads) append_kernel(const __grid_constant__ RowArgs a, const __grid_constant__ Codebook cb) {
+__global__ void __launch_bounds__(kRowThreads, 3) append_kernel(const __grid_constant__ RowArgs a, const __grid_constant__ Codebook cb) {
     __shared__ float2 s_cells[BITS == 3 ? kCells * 32 : 1];
     if (BITS == 3) {
         build_cell_table(cb, cb.n - 1, s_cells, threadIdx.x, kRowThreads);
@@ -479,6 +479,14 @@ __device__ __forceinline__ void do_rows_part(const RowArgs& a, const RowSpan& s,
 // The same where whole rows turn, or nothing does: a lane has eight elements of the first half of a row and the eight half a
 // row behind them, so that both elements of a pair are its own, and a pass takes 32 / (D / 16) heads.  Half the
 // instructions a row of do_rows_part, which is what bounds this kernel: 8,191 tokens of 32 + 8 heads 45 us with it.
+// What a warp takes in turn: `size` passes of a token, unit after unit `step` apart.
+struct Units {
+    int count, step, size, per_token;
+    Divisor by_token;
+    __device__ __forceinline__ int token_of(int unit) const { return (int)by_token.of((unsigned)unit); }
+    __device__ __forceinline__ int first_pass(int unit, int token) const { return (unit - token * per_token) * size; }
+};
+
 // A pass is 32 / (D / 16) heads of queries, or of keys, of a token; passes are numbered token after token, queries before keys.
 // They are copied to a ring in shared memory, kDepth of them ahead; a lane reads what it has copied itself.
 template <typename T, int LPH, bool STORE>
@@ -486,24 +494,31 @@ struct Rows {
     static constexpr int D = LPH * 8, LPR = LPH / 2, HPW = 32 / LPR, NB = D / 32;
     static constexpr int kDepth = 8 / (int)sizeof(T), kLane = 16 * (int)sizeof(T), kSlot = 32 * kLane;   // passes in flight, bytes a lane and a pass
     const RowArgs& a;
-    const int sub, l, passes_q, passes, part, parts;   // of a token's passes the warp takes part, part + parts, ..
-    int token, pass, left, token_step;                 // what is copied next, and how many passes still
+    const int sub, l, passes_q, passes, part, parts;   // the warp takes passes part, part + parts, .. of a unit
+    const Units& u;
+    int unit, pass, pass_end;                    // what is copied next
+    int token;
     uint32_t to, ring;                                 // shared addresses of the lane's next slot and of its first
     const unsigned char *from, *s_ring;                // the lane's slot that is read next, and its first
 
     static __host__ __device__ __forceinline__ int passes_of(int heads) { return (heads + HPW - 1) / HPW; }
 
-    __device__ __forceinline__ Rows(const RowArgs& args, int token_, int pass_, int left_, int part_, int parts_, int step, unsigned char* space)
+    __device__ __forceinline__ Rows(const RowArgs& args, const Units& units, int first, int part_, int parts_, unsigned char* space)
         : a(args), sub((threadIdx.x & 31) / LPR), l((threadIdx.x & 31) % LPR), passes_q(passes_of(args.q.heads)),
-          passes(passes_q + passes_of(args.k.heads)), part(part_), parts(parts_), token(token_), pass(pass_), left(left_), token_step(step) {
+          passes(passes_q + passes_of(args.k.heads)), part(part_), parts(parts_), u(units), unit(first) {
+        begin();
         s_ring = from = space + (threadIdx.x & 31) * kLane;
         to = ring = (uint32_t)__cvta_generic_to_shared(s_ring);
 #pragma unroll 1
         for (int k = 0; k < kDepth; ++k) fetch();
     }
+    __device__ __forceinline__ void begin() {
+        token = unit < u.count ? u.token_of(unit) : 0;
+        pass = u.first_pass(unit, token) + part;
+        pass_end = unit < u.count ? min(passes, pass - part + u.size) : 0;
+    }
     __device__ __forceinline__ void fetch() {
-        if (left > 0) {
-            --left;
+        if (pass < pass_end) {
             const RowSpan& s = pass < passes_q ? a.q : a.k;
             const int h = min((pass < passes_q ? pass : pass - passes_q) * HPW + sub, s.heads - 1);   // (a lane without a head reads the last one)
             const T* in = reinterpret_cast<const T*>(s.in) + token * s.in_token + h * s.in_head + 8 * l;
@@ -513,9 +528,9 @@ struct Rows {
                 cp_async16(to + 32 * k + 16, reinterpret_cast<const unsigned char*>(in + D / 2) + 16 * k);
             }
             pass += parts;
-            if (pass >= passes) {
-                pass = part;
-                token += token_step;
+            if (pass >= pass_end && unit < u.count) {
+                unit += u.step;
+                begin();
             }
         }
         cp_async_commit();
@@ -632,6 +647,7 @@ struct Rows {
     }
 };
 
+constexpr int kTurnWarps = 4, kTurnCtas = 5;   // of turn_kernel: CTAs of an SM
 constexpr int kRingBytes = 4096;   // of a warp: Rows::kDepth * Rows::kSlot
 
 // Cosines and sines of a token's angles, by `all` threads of which this is number `me`.
@@ -647,10 +663,9 @@ __device__ __forceinline__ void angles(const RowArgs& a, int t, float* s_cos, fl
     }
 }
 
-// Norm and rotation alone, whole rows turning: every warp takes an equal run of the passes, a token's angles for itself.  By
-// whole tokens a warp 8,191 tokens were two or three rounds: 45 us.
+// Norm and rotation alone, whole rows turning: warps take units of a token's passes in turn, neighbours neighbouring ones.
 template <typename T, int LPH>
-__global__ void __launch_bounds__(kRowThreads, 3) turn_kernel(const __grid_constant__ RowArgs a) {
+__global__ void __launch_bounds__(32 * kTurnWarps, kTurnCtas) turn_kernel(const __grid_constant__ RowArgs a, const __grid_constant__ Units u) {
     using R = Rows<T, LPH, false>;
     extern __shared__ __align__(16) unsigned char s_dyn[];   // [warp]: ring, cosines, sines
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -658,28 +673,29 @@ __global__ void __launch_bounds__(kRowThreads, 3) turn_kernel(const __grid_const
     float* const s_cos = reinterpret_cast<float*>(mine + kRingBytes);
     float* const s_sin = s_cos + R::D / 2;
     const int passes = R::passes_of(a.q.heads) + R::passes_of(a.k.heads);
-    const long long total = (long long)a.tokens * passes, warps = (long long)gridDim.x * kRowWarps, w = (long long)blockIdx.x * kRowWarps + warp;
-    const long long quot = total / warps, rem = total - quot * warps, begin = w * quot + (w < rem ? w : rem);
-    int left = (int)(quot + (w < rem ? 1 : 0));
-    if (left == 0) return;
-    int t = (int)(begin / passes), p = (int)(begin - (long long)t * passes);
-    R rows(a, t, p, left, 0, 1, 1, mine);
-    for (; left > 0; ++t, p = 0) {
-        const int n = min(left, passes - p);
+    int unit = blockIdx.x * kTurnWarps + warp;
+    if (unit >= u.count) return;
+    R rows(a, u, unit, 0, 1, mine);
+    for (; unit < u.count; unit += u.step) {
+        const int t = u.token_of(unit), p = u.first_pass(unit, t);
         if (a.rot_dim > 0) {
             angles(a, t, s_cos, s_sin, lane, 32);
             __syncwarp();
         }
-        rows.run(t, p, p + n, s_cos, s_sin, nullptr);
+        rows.run(t, p, min(passes, p + u.size), s_cos, s_sin, nullptr);
         __syncwarp();   // the angles have been read
-        left -= n;
     }
 }
+
+struct NoRows {   // (do_rows_part reads for itself)
+    template <typename... A>
+    __device__ __forceinline__ NoRows(const A&...) {}
+};
 
 // Rows that are packed (BITS != 0), or of which only the first rot_dim elements turn (PART): a token a warp; where there are few
 // tokens (`shared_token`), a token a CTA.
 template <typename T, int LPH, int BITS, bool PART>
-__global__ void __launch_bounds__(kRowThreads, 3) rows_kernel(const __grid_constant__ RowArgs a, const __grid_constant__ Codebook cb) {
+__global__ void __launch_bounds__(kRowThreads, PART ? 3 : 2) rows_kernel(const __grid_constant__ RowArgs a, const __grid_constant__ Codebook cb) {
     constexpr int D = LPH * 8, NB = D / 32;
     using R = Rows<T, LPH, true>;
     extern __shared__ __align__(16) unsigned char s_dyn[];
@@ -700,6 +716,9 @@ __global__ void __launch_bounds__(kRowThreads, 3) rows_kernel(const __grid_const
         __syncthreads();
     }
     const int per_cta = a.shared_token ? 1 : kRowWarps, step = gridDim.x * per_cta;
+    const int passes = R::passes_of(a.q.heads) + R::passes_of(a.k.heads);
+    const Units u{a.tokens, step, passes, 1, Divisor()};   // whole tokens
+    typename std::conditional<PART, NoRows, R>::type rows(a, u, blockIdx.x * per_cta + (a.shared_token ? 0 : warp), part, parts, s_dyn + (size_t)warp * kRingBytes);
     for (int t = blockIdx.x * per_cta + (a.shared_token ? 0 : warp); t < a.tokens; t += step) {
         if constexpr (PART) {
             angles(a, t, s_cos, s_sin, me, all);
@@ -707,8 +726,6 @@ __global__ void __launch_bounds__(kRowThreads, 3) rows_kernel(const __grid_const
             if (a.q.heads > 0) do_rows_part<T, LPH, false>(a, a.q, t, part, parts, s_cos, s_sin, s_tile);
             if (a.k.heads > 0) do_rows_part<T, LPH, BITS != 0>(a, a.k, t, part, parts, s_cos, s_sin, s_tile);
         } else {
-            const int passes = R::passes_of(a.q.heads) + R::passes_of(a.k.heads);
-            R rows(a, t, part, max(0, (passes - part + parts - 1) / parts), part, parts, 1, s_dyn + (size_t)warp * kRingBytes);
             if (half > 0) {
                 angles(a, t, s_cos, s_sin, me, all);
                 sync();
@@ -862,15 +879,26 @@ int launch_rows_one(RowArgs& a, const Codebook& cb, cudaStream_t s) {
     if constexpr (BITS == 0) {
         if (!partly) {
             using R = Rows<T, LPH, false>;
-            const int dyn = kRowWarps * (kRingBytes + R::D * (int)sizeof(float));
+            const int dyn = kTurnWarps * (kRingBytes + R::D * (int)sizeof(float));
             if (int st = allow_shared<turn_kernel<T, LPH>>(dyn)) return st;
-            const long long passes = (long long)a.tokens * (R::passes_of(a.q.heads) + R::passes_of(a.k.heads)), want = (passes + kRowWarps - 1) / kRowWarps;
-            turn_kernel<T, LPH><<<(unsigned)(want < 148 * 3 ? want : 148 * 3), kRowThreads, dyn, s>>>(a);
+            // Half a token a unit, so that the last round is a short one (8,191 whole tokens are two or three a warp: 45 us); single
+            // passes where there are few.
+            const int passes = R::passes_of(a.q.heads) + R::passes_of(a.k.heads), warps = 148 * kTurnCtas * kTurnWarps;
+            Units u;
+            u.size = (long long)a.tokens * passes <= warps ? 1 : (passes + 1) / 2;
+            u.per_token = (passes + u.size - 1) / u.size;
+            const long long units = (long long)a.tokens * u.per_token;
+            if (units >= (1ll << 31) - 2 * warps) return TQB_ERR_TOO_LARGE;
+            u.count = (int)units;
+            u.by_token = Divisor((unsigned)u.per_token);
+            const int want = (u.count + kTurnWarps - 1) / kTurnWarps, grid = want < 148 * kTurnCtas ? want : 148 * kTurnCtas;
+            u.step = grid * kTurnWarps;
+            turn_kernel<T, LPH><<<grid, 32 * kTurnWarps, dyn, s>>>(a, u);
             return check_launch(s);
         }
     }
     const long long want = a.shared_token ? a.tokens : (a.tokens + kRowWarps - 1) / kRowWarps;
-    const unsigned grid = (unsigned)(want < 148 * 32 ? want : 148 * 32);
+    const unsigned grid = (unsigned)(want < 148 * 2 || a.shared_token ? want : 148 * 2);
     if (partly) {
         if (int st = allow_shared<rows_kernel<T, LPH, BITS, true>>(bytes, 160 * 1024)) return st;
         rows_kernel<T, LPH, BITS, true><<<grid, kRowThreads, bytes, s>>>(a, cb);
