@@ -44,6 +44,21 @@ __device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2;\n" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
 
+// A token's NB scales, two a word.
+template <int NB, int OFF>
+__device__ __forceinline__ void load_scales(uint32_t at, uint32_t (&w)[NB / 2]) {
+    if constexpr (NB == 2) {
+        w[0] = lds32_o<OFF>(at);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NB / 4; ++i) {
+            const uint2 v = i == 0 ? lds64_o<OFF>(at) : lds64_o<OFF + 8>(at);
+            w[2 * i] = v.x;
+            w[2 * i + 1] = v.y;
+        }
+    }
+}
+
 // x[i]: half2 of code i of the two tokens in the halves of w, as the subnormals c 2^-23 (i even), c 2^-19 (i odd).
 __device__ __forceinline__ void codes_to_subnormals(uint32_t w, uint32_t (&x)[4]) {
     const uint32_t w1 = w << 1, w7 = w >> 7;
@@ -139,8 +154,7 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG, BITS>::kCtas) paged
 
     // ---- copies: segment after segment without a break, a step ahead of the products ----
     Segment s{};
-    bool more = line.next(s);
-    int to_copy = s.t0, copy_end = s.t1;      // of the segment whose copies are being made
+    int to_copy = 0, copy_end = 0;            // of the segment whose copies are being made
     int page_now = 0, page_next = 0, page0 = 0;   // pages page0 + 32 k + lane of it, for this k and the next
     const int32_t* table = a.table;
     uint32_t head = 0;
@@ -205,28 +219,26 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG, BITS>::kCtas) paged
         to_copy += kGroupTokens;
     };
 
-    if (more) {
-        open(s);
-#pragma unroll 1
-        for (int u = 0; u < kStepGroups; ++u) fill(ring + u * G::kStage);
-    }
+    // One more turn than there are segments: the first has nothing to work on and begins the copies.  (What is written once
+    // here is fetched once: a second copy of this code costs a short call more than the turn.)
     uint32_t st = ring;
-    while (more) {
+    for (bool have = false;; have = true) {
         // ---- the next segment; copies go over to it by themselves ----
         bool bad = bad_copy;                  // of this segment
         Segment next{};
-        more = line.next(next);
+        const bool more = line.next(next);
+        if (!have && !more) break;
         __syncwarp();                         // (s_next has been read)
         if (lane == 0) s_next[warp] = next;
         bool ahead = false;                   // copies have gone over
-        cp_async_wait<kInFlight - 1>();       // the first group, and the queries
+        if (have) cp_async_wait<kInFlight - 1>();   // the first group, and the queries
         __syncwarp();
         // ---- queries: rotated, scaled to integers, cut into digits ----
         float qsc[kE];
-        {
-            const float inv_sqrt = 1.0f / sqrtf((float)kBlock), sg = block_sign(lane, a.sign_mag);
 #pragma unroll
-            for (int e = 0; e < kE; ++e) qsc[e] = 0.0f;
+        for (int e = 0; e < kE; ++e) qsc[e] = 0.0f;
+        if (have) {
+            const float inv_sqrt = 1.0f / sqrtf((float)kBlock), sg = block_sign(lane, a.sign_mag);
             // Fragment (b, 4n' + j') of column n' has eight dims from 32 b + 8 j' on, a byte each.  4-bit: the even ones (k-slots 4j' ..)
             // in its first word, the odd ones (k-slots 16 + 4j' ..) in the second; 3-bit: the first four, the last four.
             unsigned char* const at = s_digits + (lane >> 3) * 8 + (BITS == 4 ? (lane & 1) * 4 + ((lane >> 1) & 3) : lane & 7);
@@ -283,7 +295,7 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG, BITS>::kCtas) paged
                 for (int m = 0; m < 2; ++m)
 #pragma unroll
                     for (int i = 0; i < kO; ++i) o[b][m][i] = 0.0f;
-            for (int t0 = s.t0; t0 < s.t1; t0 += kStepGroups * kGroupTokens) {
+            for (int t0 = s.t0; !have || t0 < s.t1; t0 += kStepGroups * kGroupTokens) {
                 const uint32_t st_other = halves - st;
                 if (to_copy >= copy_end && more && !ahead) {   // this segment's copies are under way: the next one's
                     bad |= bad_copy;
@@ -292,6 +304,10 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG, BITS>::kCtas) paged
                 }
 #pragma unroll
                 for (int u = 0; u < kStepGroups; ++u) fill(st_other + u * G::kStage);
+                if (!have) {
+                    st = st_other;
+                    break;
+                }
                 cp_async_wait<kInFlight>();
                 __syncwarp();
                 // ---- scores ----
@@ -304,11 +320,14 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG, BITS>::kCtas) paged
                     for (int t = 0; t < 2; ++t)
 #pragma unroll
                         for (int e = 0; e < kE; ++e) acc[t][e] = 0.0f;
+                    uint32_t ks[2][kPairs];   // scales of tokens n, n + 8
+                    load_scales<NB, 0>(stu + off_s, ks[0]);
+                    load_scales<NB, 8 * G::kSc>(stu + off_s, ks[1]);
                     static_for<0, kPairs>([&](auto p_) {
                         constexpr int p = decltype(p_)::value;
                         uint32_t kw[4];
                         if (BITS == 4) ldsm4_o<0>(stu + (off_k ^ (32 * p)), kw);
-                        const uint32_t sa = lds32_o<4 * p>(stu + off_s) & 0x7fff7fffu, sb = lds32_o<4 * p + 8 * G::kSc>(stu + off_s) & 0x7fff7fffu;
+                        const uint32_t sa = ks[0][p] & 0x7fff7fffu, sb = ks[1][p] & 0x7fff7fffu;
                         static_for<0, 2>([&](auto i_) {
                             constexpr int i = decltype(i_)::value, b = 2 * p + i;
                             const float ka = i ? __high2float(u32_as_h2(sa)) : __low2float(u32_as_h2(sa));
@@ -394,9 +413,10 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG, BITS>::kCtas) paged
                     constexpr int u = decltype(u_)::value;
                     static_for<0, 2>([&](auto t_) {
                         constexpr int t = decltype(t_)::value;
+                        load_scales<NB, 16 * G::kSc + 8 * t * G::kSc>(st + u * G::kStage + off_s, sv[u][t]);
                         static_for<0, kPairs>([&](auto p_) {
                             constexpr int pr = decltype(p_)::value;
-                            sv[u][t][pr] = lds32_o<16 * G::kSc + 8 * t * G::kSc + 4 * pr>(st + u * G::kStage + off_s) & sv_mask[u][t];
+                            sv[u][t][pr] &= sv_mask[u][t];
                             sv_top = h2_as_u32(__hmax2(u32_as_h2(sv_top), u32_as_h2(sv[u][t][pr])));
                         });
                     });
@@ -535,6 +555,10 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG, BITS>::kCtas) paged
             }
         }
 
+        if (!have) {
+            s = s_next[warp];
+            continue;
+        }
         // ---- the segment's end ----
         // A whole segment's outputs pass through the half of the ring that holds nothing yet: the copies in flight are in `st`.
         const bool whole = s.whole();
@@ -576,6 +600,7 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG, BITS>::kCtas) paged
             }
             __syncwarp();
         }
+        if (!more) break;
         s = s_next[warp];
     }
     finish<NB>(a, s_frag, [&](int c, int x) { return reinterpret_cast<const float4*>(fragment(c))[x]; });

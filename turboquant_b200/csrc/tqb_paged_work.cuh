@@ -1,6 +1,6 @@
 // How the kernels of the paged attention share their work, and how the shares are joined.
 //
-// The work of a call is a line of groups of 16 tokens: request after request, within a request KV head after KV head (a group
+// The work of a call is a line of groups of 16 tokens (16 << unit_shift, where 2^31 units could not count the widest table): request after request, within a request KV head after KV head (a group
 // of more than eight query heads counts as several), within a head token after token; kOpenCost units stand before each
 // (request, head) for what it takes to begin one.  Every WARP takes an equal run of the line, whatever the lengths are,
 // worked out on the device from the lengths, so that a captured launch serves any batch.  A run is cut into segments, one
@@ -19,14 +19,8 @@
 namespace tqb {
 
 constexpr int kRunTokens = 16;       // of a group
-#ifndef OPENCOST
-#define OPENCOST 6
-#endif
-#ifndef MINRUN
-#define MINRUN 4
-#endif
-constexpr int kOpenCost = OPENCOST;  // groups that beginning a segment is worth
-constexpr int kMinRun = MINRUN;      // units of a run, at least
+constexpr int kOpenCost = 6;         // groups that beginning a segment is worth
+constexpr int kMinRun = 4;           // units of a run, at least
 constexpr int kSegHeads = 8;         // query heads of a segment, at most
 constexpr int kWorkWarps = 4;
 constexpr int kWorkThreads = 32 * kWorkWarps;
@@ -49,7 +43,7 @@ struct PagedArgs {
     float* round_ml;     // the same of joined parts, where two rounds are needed
     float* part_out;     // [kMaxCtas][2][kSegHeads][D], rotated domain
     long long q_stride, table_stride;
-    int requests, max_blocks, max_len, page_shift, num_pages, hkv, group, vheads, splits;   // vheads = hkv * splits
+    int requests, max_blocks, max_len, unit_shift, page_shift, num_pages, hkv, group, vheads, splits;   // vheads = hkv * splits
     int q_dtype, out_dtype;
     float qk_const;      // softmax_scale * log2(e)
     float sign_mag;
@@ -69,99 +63,95 @@ struct Segment {
     __device__ __forceinline__ bool whole() const { return begins && ends; }
 };
 
-typedef unsigned long long Units;
-// x / y for quotients below 2^21: up to 2^31 the f32 quotient is off by less than 1/2, so one step mends it.  (Integer
-// divisions are 50 to 100 instructions one behind the other, and a run begins with seven of them.)
-__device__ __forceinline__ Units divide(Units x, Units y) {
-    if (((x | y) >> 31) != 0) return x / y;
-    const unsigned n = (unsigned)x, d = (unsigned)y;
-    unsigned q = (unsigned)__fdividef((float)n, (float)d);
-    const int r = (int)(n - q * d);
-    q += r < 0 ? -1 : r >= (int)d ? 1 : 0;
+// x / y below 2^31, for quotients below 2^21: the f32 quotient is then off by less than 1/2, so one step mends it.  (An integer
+// division is some 50 instructions one behind the other, and a run begins with seven of them.)
+__device__ __forceinline__ unsigned divide(unsigned x, unsigned y) {
+    unsigned q = (unsigned)__fdividef((float)x, (float)y);
+    const int r = (int)(x - q * y);
+    q += r < 0 ? -1 : r >= (int)y ? 1 : 0;
     return q;
 }
 
 // A warp's run of the line.
 struct WorkLine {
     const PagedArgs& a;
-    Units total, quot, rem;       // a run has quot units, the first `rem` runs one more
-    Units cur, end, base;         // base: where request `req` begins
+    unsigned quot, rem;              // a run has quot units, the first `rem` runs one more
+    unsigned cur, end, base;         // base: where request `req` begins
     int req, len;
 
     __device__ __forceinline__ int length(int r) const { return min(max(a.lens[r], 0), a.max_len); }
-    static __device__ __forceinline__ unsigned groups_of(int len) { return (unsigned)(len + kRunTokens - 1) / kRunTokens; }
-    static __device__ __forceinline__ unsigned units_of(int len) { return len > 0 ? kOpenCost + groups_of(len) : 0u; }
-    __device__ __forceinline__ int owner(Units x) const {   // the run that unit x belongs to
-        const Units split = rem * (quot + 1);
+    __device__ __forceinline__ unsigned groups_of(int l) const { return ((unsigned)l + (kRunTokens << a.unit_shift) - 1) / kRunTokens >> a.unit_shift; }
+    __device__ __forceinline__ unsigned units_of(int l) const { return l > 0 ? kOpenCost + groups_of(l) : 0u; }
+    __device__ __forceinline__ int owner(unsigned x) const {   // the run that unit x belongs to
+        const unsigned split = rem * (quot + 1);
         return (int)(x < split ? divide(x, quot + 1) : rem + divide(x - split, quot));
     }
 
     // All threads of the CTA.  Reads every request's length (4 bytes each, from L2): two block barriers.
     __device__ __forceinline__ explicit WorkLine(const PagedArgs& args) : a(args) {
-        __shared__ Units s_sum[kWorkWarps], s_begin[kWorkThreads];
+        __shared__ unsigned s_sum[kWorkWarps], s_begin[kWorkThreads];
         const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
         const int per = (a.requests + kWorkThreads - 1) / kWorkThreads, r0 = min(tid * per, a.requests), r1 = min(r0 + per, a.requests);
-        Units mine = 0;
+        unsigned mine = 0;
+#pragma unroll 1
         for (int r = r0; r < r1; ++r) mine += units_of(length(r));
-        Units incl = mine;
-#pragma unroll
+        unsigned incl = mine;
+#pragma unroll 1
         for (int o = 1; o < 32; o <<= 1) {
-            const Units x = __shfl_up_sync(0xffffffffu, incl, o);
+            const unsigned x = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += x;
         }
         if (lane == 31) s_sum[warp] = incl;
         __syncthreads();
-        total = 0;
-        Units before = incl - mine;
+        unsigned total = 0, before = incl - mine;
 #pragma unroll
         for (int w = 0; w < kWorkWarps; ++w) {
             if (w < warp) before += s_sum[w];
             total += s_sum[w];
         }
-        s_begin[tid] = before;
+        s_begin[tid] = before * a.vheads;
         __syncthreads();
         total *= a.vheads;
         // as many runs as the longest run needs: it is no longer with them, and fewer parts are joined
         const unsigned most = gridDim.x * kWorkWarps, i = blockIdx.x * kWorkWarps + warp;
-        const Units longest = max(divide(total + most - 1, most), (Units)min(total, (Units)kMinRun)), runs = longest > 0 ? divide(total + longest - 1, longest) : 0;
+        const unsigned longest = max(divide(total + most - 1, most), min(total, (unsigned)kMinRun));
+        const unsigned runs = longest > 0 ? divide(total + longest - 1, longest) : 0;
         cur = end = base = 0;
         quot = rem = 0;
         req = len = 0;
         if (i >= runs) return;
         quot = divide(total, runs);
         rem = total - quot * runs;
-        cur = i * quot + min((Units)i, rem);
+        cur = i * quot + min(i, rem);
         end = cur + quot + (i < rem ? 1 : 0);
         // the last of the threads' requests that begin at or before `cur`: four threads a lane, then their requests
         int chunk = 0;
 #pragma unroll
-        for (int k = 0; k < kWorkWarps; ++k) chunk += __popc(__ballot_sync(0xffffffffu, s_begin[32 * k + lane] * a.vheads <= cur));
+        for (int k = 0; k < kWorkWarps; ++k) chunk += __popc(__ballot_sync(0xffffffffu, s_begin[32 * k + lane] <= cur));
         --chunk;   // (threads behind the last request begin at the total)
-        Units b = s_begin[chunk] * a.vheads;
+        base = s_begin[chunk];
         req = min(chunk * per, a.requests - 1);
         len = length(req);
-        while (req + 1 < a.requests && cur >= b + (Units)units_of(len) * a.vheads) {
-            b += (Units)units_of(len) * a.vheads;
+        while (req + 1 < a.requests && cur >= base + units_of(len) * a.vheads) {
+            base += units_of(len) * a.vheads;
             len = length(++req);
         }
-        base = b;
         if (len == 0) end = cur;   // not reached while the lengths stay as they are
     }
 
     // The next segment; false at the run's end.
     __device__ __forceinline__ bool next(Segment& s) {
         while (cur < end) {
-            const unsigned groups = groups_of(len), units = kOpenCost + groups, vh = (unsigned)divide(cur - base, units);
-            const Units start = base + (Units)vh * units;
-            const unsigned u0 = (unsigned)(cur - start), u1 = (unsigned)min((Units)units, u0 + (end - cur));
+            const unsigned groups = groups_of(len), units = kOpenCost + groups, vh = divide(cur - base, units), start = base + vh * units;
+            const unsigned u0 = cur - start, u1 = min(units, u0 + (end - cur));
             const unsigned g0 = max(u0, (unsigned)kOpenCost) - kOpenCost, g1 = max(u1, (unsigned)kOpenCost) - kOpenCost;
             s.req = req;
             s.kvh = a.splits == 1 ? (int)vh : (int)vh / a.splits;
             const int h0 = ((int)vh - s.kvh * a.splits) * kSegHeads;
             s.head0 = s.kvh * a.group + h0;
             s.heads = min(a.group - h0, kSegHeads);
-            s.t0 = (int)g0 * kRunTokens;
-            s.t1 = min((int)g1 * kRunTokens, len);
+            s.t0 = (int)(g0 << a.unit_shift) * kRunTokens;
+            s.t1 = g1 == groups ? len : (int)(g1 << a.unit_shift) * kRunTokens;
             s.begins = g0 == 0;
             s.ends = g1 == groups;
             s.cta0 = s.ctas = 0;
@@ -170,7 +160,7 @@ struct WorkLine {
                 s.ctas = owner(start + units - 1) / kWorkWarps - s.cta0 + 1;
             }
             cur += u1 - u0;
-            if (cur < end && cur == base + (Units)units * a.vheads) {
+            if (cur < end && cur == base + units * a.vheads) {
                 base = cur;
                 len = 0;
                 while (len == 0 && req + 1 < a.requests) len = length(++req);
