@@ -52,7 +52,9 @@ __device__ __forceinline__ uint32_t lop3_xor_select(uint32_t a, uint32_t mask, u
     return d;
 }
 __device__ __forceinline__ uint32_t bit_select(uint32_t a, uint32_t b, uint32_t mask) {
-    return (a & mask) | (b & ~mask);   // one LOP3
+    uint32_t d;   // (a & mask) | (b & ~mask); written out, since the compiler may make two instructions of a constant mask
+    asm("lop3.b32 %0, %1, %2, %3, 0xCA;\n" : "=r"(d) : "r"(mask), "r"(a), "r"(b));
+    return d;
 }
 
 __device__ __forceinline__ float ex2(float x) {

@@ -73,6 +73,12 @@ __device__ __forceinline__ uint32_t nibbles_of_codes(uint32_t w) {
     const uint32_t b = bit_select(a, a << 2, 0x003f003fu);
     return bit_select(b, b << 1, 0x07070707u) & 0x77777777u;
 }
+// The bytes of (lo, hi) that the low four nibbles of c, 0 .. 7 each, name.
+__device__ __forceinline__ uint32_t byte_of_table(uint32_t lo, uint32_t hi, uint32_t c) {
+    uint32_t d;
+    asm("prmt.b32 %0, %1, %2, %3;\n" : "=r"(d) : "r"(lo), "r"(hi), "r"(c));
+    return d;
+}
 constexpr uint32_t kCentreEven = 0x800f800fu;   // -7.5 2^-23 as a subnormal f16, twice
 constexpr uint32_t kCentreOdd = 0x80f080f0u;    // -7.5 2^-19
 
@@ -140,10 +146,13 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG, BITS>::kCtas) paged
     // 3-bit: K codes 8j .. 8j + 7 are the 24 bits at byte 3j of a block, V codes 4n .. 4n + 3 the 12 bits at bit 12 n
     const uint32_t off_k3 = n * G::kRow + 4 * ((3 * j) >> 2), off_k3h = off_k3 + (j < 3 ? 4 : 0), sh_k3 = ((3 * j) & 3) * 8;
     const uint32_t off_v3 = G::kIdx + 2 * j * G::kRow + 4 * ((12 * n) >> 5), sh_v3 = (12 * n) & 31, off_v3h = off_v3 + (sh_v3 > 20 ? 4 : 0);
+    // those of the other token, three bits up: from bit 12 n - 3 on (n = 0: the word before; what comes from there is masked)
+    const int bit_w3 = 12 * n - 3;
+    const uint32_t off_w3 = G::kIdx + (2 * j + 1) * G::kRow + 4 * (bit_w3 >> 5), sh_w3 = bit_w3 & 31, off_w3h = off_w3 + (sh_w3 > 17 ? 4 : 0);
     const uint32_t off_ps = 2 * G::kIdx + lane * G::kSc;   // K scales of tokens 0..15, V scales behind them
     const int mask = (1 << a.page_shift) - 1;
     auto pair_of = [&](uint32_t at) {   // table entry, in bits 7 .. 12 of `at`
-        return *reinterpret_cast<const uint32_t*>(reinterpret_cast<const unsigned char*>(s_pairs) + ((at & 0x1f80u) | (lane * 4)));
+        return *reinterpret_cast<const uint32_t*>(reinterpret_cast<const unsigned char*>(s_pairs) + bit_select(at, lane * 4, 0x1f80u));
     };
 
     if (BITS == 3)
@@ -351,10 +360,10 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG, BITS>::kCtas) paged
                                 static_for<0, 2>([&](auto t_) {
                                     constexpr int t = decltype(t_)::value;
                                     const uint32_t c = nibbles_of_codes(__funnelshift_r(lds32_o<12 * b + 8 * t * G::kRow>(stu + off_k3), lds32_o<12 * b + 8 * t * G::kRow>(stu + off_k3h), sh_k3));
-                                    x[t][0] = __byte_perm(a.digits[0], a.digits[1], c);
-                                    x[t][1] = __byte_perm(a.digits[0], a.digits[1], c >> 16);
-                                    x[t][2] = __byte_perm(a.digits[2], a.digits[3], c);
-                                    x[t][3] = __byte_perm(a.digits[2], a.digits[3], c >> 16);
+                                    x[t][0] = byte_of_table(a.digits[0], a.digits[1], c);
+                                    x[t][1] = byte_of_table(a.digits[0], a.digits[1], c >> 16);
+                                    x[t][2] = byte_of_table(a.digits[2], a.digits[3], c);
+                                    x[t][3] = byte_of_table(a.digits[2], a.digits[3], c >> 16);
                                 });
                                 const uint2 qb = lds64_o<(NB + b) * 256>(digits);
                                 imma16832(hi, x[0][0], x[1][0], x[0][1], x[1][1], qa.x, qa.y);
@@ -528,14 +537,14 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG, BITS>::kCtas) paged
                                 static_for<0, 2>([&](auto o_) {
                                     constexpr int o8 = decltype(o_)::value, off = 12 * b + 8 * o8 * G::kRow + u * G::kStage;
                                     const uint32_t ya = __funnelshift_r(lds32_o<off>(st + off_v3), lds32_o<off>(st + off_v3h), sh_v3);
-                                    const uint32_t yb = __funnelshift_r(lds32_o<off + G::kRow>(st + off_v3), lds32_o<off + G::kRow>(st + off_v3h), sh_v3);
-                                    // six-bit pairs (token 2j | token 2j + 1 << 3): codes 0 and 2, codes 1 and 3
-                                    const uint32_t z0 = bit_select(ya, yb << 3, 0x1c7u), z1 = bit_select(ya >> 3, yb, 0x1c7u);
+                                    const uint32_t yb = __funnelshift_r(lds32_o<off>(st + off_w3), lds32_o<off>(st + off_w3h), sh_w3);
+                                    // six-bit pairs (token 2j | token 2j + 1 << 3): codes 0 and 2, codes 1 and 3 (3 bits up)
+                                    const uint32_t z0 = bit_select(ya, yb, 0x1c7u), z1 = bit_select(ya, yb, 0xe38u);
                                     uint32_t* x = o8 == 0 ? xa : xb;
                                     x[0] = pair_of(z0 << 7);
-                                    x[1] = pair_of(z1 << 7);
+                                    x[1] = pair_of(z1 << 4);
                                     x[2] = pair_of(z0 << 1);
-                                    x[3] = pair_of(z1 << 1);
+                                    x[3] = pair_of(z1 >> 2);
                                 });
                             }
 #pragma unroll
