@@ -463,12 +463,12 @@ template <typename T, int BITS>
 __global__ void __launch_bounds__(kThreads)
 block_dequantize_lane_kernel(DequantArgs a, Codebook cb) {
     constexpr int kPitch = 32 * (int)sizeof(T) + 16;              // a lane's staged row: 16-byte pieces of 8 lanes in 32 banks
-    __shared__ __align__(2048) unsigned char s_tab[2 * DequantTable<BITS>::kBytes];
+    __shared__ __align__(128) unsigned char s_tab[2 * DequantTable<BITS>::kBytes];
     __shared__ __align__(16) unsigned char s_stage[kThreads * kPitch];
     const int lane = threadIdx.x & 31;
     build_dequant_table<BITS>(cb, a.sign_mag, s_tab, threadIdx.x, kThreads);
     __syncthreads();
-    const uint32_t tab = (uint32_t)__cvta_generic_to_shared(s_tab) + lane * 4;
+    const uint32_t tab = (uint32_t)__cvta_generic_to_shared(s_tab), lane4 = lane * 4;
     unsigned char* stage = s_stage + (threadIdx.x >> 5) * 32 * kPitch;
     const unsigned total = (unsigned)(a.n_rows * a.nblk), nblk = (unsigned)a.nblk;
     for (unsigned blk0 = (blockIdx.x * kThreads + threadIdx.x) & ~31u; blk0 < total; blk0 += gridDim.x * kThreads) {
@@ -488,7 +488,7 @@ block_dequantize_lane_kernel(DequantArgs a, Codebook cb) {
         }
         const F2 as = f2(fabsf(f16_bits_to_f32(__ldg(a.scales + sblk))));
         float v[32];
-        dequantize_values<BITS>(w, as, tab, v);
+        dequantize_values<BITS>(w, as, tab, lane4, v);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             float e[8];
