@@ -552,7 +552,8 @@ size_t tqb_kv_cache_fp16_equivalent_memory(const tqb_kv_cache *c); /* attention.
 
 /* The arrays of one layer: indices [num_pages, num_kv_heads, page_size, head_dim*bits/8] u8 and scales
  * [num_pages, num_kv_heads, page_size, head_dim/32] u16, each 16-byte aligned.  head_dim 64, 128 or 256; bits 3 or 4;
- * page_size a power of two from 16 to 1024. */
+ * page_size a power of two from 16 to 1024; fewer than 2^32 rows (num_pages * num_kv_heads * page_size) of each,
+ * TQB_ERR_TOO_LARGE otherwise. */
 typedef struct tqb_paged_layer {
     uint8_t *k_indices;
     uint16_t *k_scales;
@@ -583,7 +584,8 @@ typedef struct tqb_paged_layer {
  *   kv_lens [num_requests]   seq_lens + new_tokens; may be seq_lens itself
  *   state_out                the new state; may be `state` itself.  state[1] is used during the call and left 0.
  * Where the step cannot be planned state_out[2] says why, no page is taken, no table entry written, every slot is
- * -1, cu is 0 and kv_lens = seq_lens.  Calls that share `state` must be ordered. */
+ * -1, cu is 0 and kv_lens = seq_lens.  state[1] must be 0 before the first call.  Calls that share `state` must be ordered.
+ * capacity up to 2^30. */
 int tqb_paged_plan(const int32_t *seq_lens, const int32_t *new_tokens, int32_t num_requests, int32_t *block_table,
                    int64_t table_stride, int32_t max_blocks, const int32_t *free_pages, int32_t *state, int32_t page_size,
                    int64_t *slots, int32_t *positions, int32_t capacity, int32_t *cu, int32_t *kv_lens,
@@ -628,7 +630,9 @@ int tqb_paged_append(const tqb_paged_layer *layer, const void *k, int64_t k_toke
                      const void *v, int64_t v_token_stride, int64_t v_head_stride, int32_t dtype, const int64_t *slots,
                      int32_t num_tokens, tqb_stream_t stream);
 /* tqb_qk_norm_rope with the keys going into their slots instead of k_out (rounded to `dtype` first: the bytes are those
- * of the two calls one after the other), and the values with them.  p->k_out is written too unless NULL. */
+ * of the two calls one after the other), and the values with them.  p->k_out is written too unless NULL.  A token's keys are
+ * staged in shared memory: TQB_ERR_UNSUPPORTED beyond 128 KB (some 1,600 32-blocks of two-byte elements), TQB_ERR_TOO_LARGE beyond
+ * 2^30 tokens. */
 int tqb_paged_append_rope(const tqb_paged_layer *layer, const tqb_rope_params *p, const void *v, int64_t v_token_stride,
                           int64_t v_head_stride, const int64_t *slots, tqb_stream_t stream);
 /* The rows at n slots, dequantized (the values of tqb_block_dequantize): k_out, v_out [n, num_kv_heads, head_dim] of
@@ -641,7 +645,8 @@ int tqb_paged_dequantize(const tqb_paged_layer *layer, const int64_t *slots, int
  *   block_table [num_requests, max_blocks], rows table_stride entries apart;  kv_lens [num_requests]
  * Request r attends to its first kv_lens[r] tokens (the new one stored already).  A request without tokens gets
  * zeros.  Lengths beyond max_blocks * page_size are cut there, and the tokens of a page outside [0, num_pages) are left out.
- * The work is split over the lengths on the device, so that a captured call serves any lengths later.
+ * The work is split over the lengths on the device, so that a captured call serves any lengths later.  out may be q where
+ * their types are the same and q is dense.
  * scratch: tqb_paged_scratch_bytes() bytes whose first TQB_PAGED_TICKET_BYTES the caller has zero-filled once; every
  * completed call leaves them zero.  Two calls that may run at the same time need a scratch each. */
 #define TQB_PAGED_TICKET_BYTES 16384

@@ -129,3 +129,36 @@ def test_caches_of_other_formats_are_refused():
             tq.PagedPqoCache(tq.CacheConfig(4, 128, 8, 1, **kw), 4)
     with pytest.raises(tq.DimensionMismatch):
         tq.PagedPqoCache(tq.CacheConfig(4, 128, 8, 1, batch=2), 4)
+
+
+MANY = (1 << 30) + 1
+
+
+def test_counts_beyond_32_bits_are_refused():
+    ref = ctypes.byref(layer())
+    args = [A, A, 3, A, 4, 4, A, A, 16, A, A, MANY, A, A, A, None]
+    assert lib.tqb_paged_plan(*args) == 12
+    for change in (dict(), dict(rot_dim=64), dict(q=None)):
+        assert lib.tqb_qk_norm_rope(ctypes.byref(rope_params(num_tokens=MANY, **change)), None) == 12
+        assert lib.tqb_paged_append_rope(ref, ctypes.byref(rope_params(num_tokens=MANY, **change)), A, 256, 128, A, None) == 12
+    big = layer(num_pages=1 << 20, num_kv_heads=256)   # 2^32 rows
+    assert attend(lay=big) == 12
+    assert lib.tqb_paged_append(ctypes.byref(big), A, 1 << 15, 128, A, 1 << 15, 128, 2, A, 3, None) == 12
+    assert lib.tqb_paged_dequantize(ctypes.byref(big), A, 3, A, A, 2, None) == 12
+    assert attend(dict(num_q_heads=1 << 30)) == 12
+
+
+def test_append_rope_of_keys_beyond_shared_memory_is_refused():
+    wide = layer(num_kv_heads=410)   # 410 * 4 blocks of 80 bytes
+    p = rope_params(num_kv_heads=410, k_token_stride=410 * 128)
+    assert lib.tqb_paged_append_rope(ctypes.byref(wide), ctypes.byref(p), A, 410 * 128, 128, A, None) == 9
+
+
+def test_packed_arguments_are_the_c_structures():
+    from turboquant_b200 import paged
+    for packed, c in ((paged._LAYER, TqbPagedLayer), (paged._ROPE, TqbRopeParams), (paged._ATTEND, TqbPagedAttentionParams)):
+        assert packed.size == ctypes.sizeof(c)
+        names = [n for n, _ in c._fields_]
+        values = [0.25 * (i + 1) if t is ctypes.c_float else i + 1 for i, (_, t) in enumerate(c._fields_)]
+        made = c.from_buffer_copy(packed.pack(*values))
+        assert [getattr(made, n) for n in names] == values

@@ -14,6 +14,7 @@ namespace {
 // need.  Every CTA does the two prefix sums over the requests for itself (8 bytes a request from L2) and then takes its
 // share of the tokens and of the new table entries; nobody waits for anybody.  What may be updated in place - lengths and
 // state - is written by the CTA that finishes last, when all have read it.  Bound: launch and two dependent loads.
+constexpr int kMostCounted = 1 << 30;   // tokens of a plan or of rows that turn: an index and a grid's stride stay below 2^31
 constexpr int kPlanThreads = 256;
 constexpr int kPlanTokens = 1024;   // tokens a CTA
 
@@ -908,6 +909,7 @@ int launch_rows_one(RowArgs& a, const Codebook& cb, cudaStream_t s) {
             return TQB_OK;
         }
     }
+    if (a.tokens > kMostCounted) return TQB_ERR_TOO_LARGE;
     const size_t token = (BITS == 0 ? 0 : (size_t)blocks_of_token * Tile<T>::kPitch) + (a.rot_dim > 0 ? (size_t)LPH * 8 * sizeof(float) : 0);
     if (token > 128 * 1024) return TQB_ERR_UNSUPPORTED;
     a.token_bytes = (int)token;
@@ -1060,6 +1062,7 @@ int tqb_paged_plan(const int32_t* seq_lens, const int32_t* new_tokens, int32_t n
     int st = check_plan_shape(num_requests, table_stride, max_blocks, page_size);
     if (st != TQB_OK) return st;
     if (capacity < 0) return TQB_ERR_INVALID_ARGUMENT;
+    if (capacity > kMostCounted) return TQB_ERR_TOO_LARGE;
     if (!state || !state_out || !cu) return TQB_ERR_NULL_POINTER;
     if (num_requests > 0 && (!seq_lens || !new_tokens || !kv_lens || (max_blocks > 0 && (!block_table || !free_pages)))) return TQB_ERR_NULL_POINTER;
     if (capacity > 0 && (!slots || !positions)) return TQB_ERR_NULL_POINTER;

@@ -169,9 +169,10 @@ int tqb_paged_attention(const tqb_paged_layer* layer, const tqb_paged_attention_
     a.group = p->num_q_heads / layer->num_kv_heads;
     a.splits = (a.group + kSegHeads - 1) / kSegHeads;
     a.vheads = a.hkv * a.splits;
+    // (below 2^30 units the quotients of divide() stay below 2^21)
     auto units = [&](int shift) { return (double)a.requests * (kOpenCost + 1 + (double)((a.max_len / kRunTokens) >> shift)) * a.vheads; };
-    while (units(a.unit_shift) >= 2147483648.0 && a.unit_shift < 24) ++a.unit_shift;
-    if (units(a.unit_shift) >= 2147483648.0) return TQB_ERR_TOO_LARGE;
+    while (units(a.unit_shift) >= 1073741824.0 && a.unit_shift < 24) ++a.unit_shift;
+    if (units(a.unit_shift) >= 1073741824.0) return TQB_ERR_TOO_LARGE;
     a.q_dtype = p->q_dtype;
     a.out_dtype = p->out_dtype;
     a.qk_const = p->softmax_scale * 1.4426950408889634f;

@@ -1,10 +1,10 @@
 // How the kernels of the paged attention share their work, and how the shares are joined.
 //
-// The work of a call is a line of groups of 16 tokens (16 << unit_shift, where 2^31 units could not count the widest table): request after request, within a request KV head after KV head (a group
-// of more than eight query heads counts as several), within a head token after token; kOpenCost units stand before each
-// (request, head) for what it takes to begin one.  Every WARP takes an equal run of the line, whatever the lengths are,
-// worked out on the device from the lengths, so that a captured launch serves any batch.  A run is cut into segments, one
-// for each (request, head) that it touches.  A warp writes a segment that is the whole of its (request, head) to the
+// The work of a call is a line of units: groups of 16 tokens (16 << unit_shift, where 2^30 units could not count the widest
+// table), request after request, within a request KV head after KV head (a group of more than eight query heads counts as
+// several), within a head token after token; kOpenCost units stand before each (request, head) for what it takes to begin
+// one.  Every WARP takes an equal run of the line, whatever the lengths are, worked out on the device from the lengths, so
+// that a captured launch serves any batch.  A run is cut into segments, one for each (request, head) that it touches.  A warp writes a segment that is the whole of its (request, head) to the
 // output by itself.  It has at most two others: one that began before it and one that goes on behind it.  These stay in
 // shared memory until the CTA's four warps are done and are joined there, and what crosses the CTA's ends goes to the
 // scratch (again at most two parts), where the CTA that arrives last at the (request, head)'s ticket joins the parts in the
@@ -63,7 +63,8 @@ struct Segment {
     __device__ __forceinline__ bool whole() const { return begins && ends; }
 };
 
-// x / y below 2^31, for quotients below 2^21: the f32 quotient is then off by less than 1/2, so one step mends it.  (An integer
+// x / y for quotients below 2^21: the f32 quotient (x, y rounded to 2^-24, __fdividef good to 2 ulp: 2^-21.4 in all) is then off
+// by less than 1, so one step mends it.  (An integer
 // division is some 50 instructions one behind the other, and a run begins with seven of them.)
 __device__ __forceinline__ unsigned divide(unsigned x, unsigned y) {
     unsigned q = (unsigned)__fdividef((float)x, (float)y);
