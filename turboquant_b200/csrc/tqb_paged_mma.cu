@@ -500,8 +500,8 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG, BITS>::kCtas) paged
                             if constexpr (HG == 4) {   // columns 2j, 2j + 1: head j with the scales of blocks 2 pr, 2 pr + 1
                                 pq[u][pr][t] = movmatrix_trans(product(ph, w));
                             } else {                   // columns 2j, 2j + 1: heads 2j, 2j + 1
-                                pq[u][2 * pr][t] = movmatrix_trans(product(ph, __byte_perm(w, w, 0x1010)));
-                                pq[u][2 * pr + 1][t] = movmatrix_trans(product(ph, __byte_perm(w, w, 0x3232)));
+                                pq[u][2 * pr][t] = movmatrix_trans(product(ph, h2_as_u32(__low2half2(u32_as_h2(w)))));
+                                pq[u][2 * pr + 1][t] = movmatrix_trans(product(ph, h2_as_u32(__high2half2(u32_as_h2(w)))));
                             }
                         });
                     });
