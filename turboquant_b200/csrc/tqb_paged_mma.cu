@@ -37,6 +37,7 @@ constexpr int kStepGroups = 2;
 constexpr int kInFlight = kRing - kStepGroups;
 constexpr float kShift = 6.0f, kLazy = 4.0f;
 constexpr uint32_t kScaleTop = 0x50005000u;   // 2^(15 - kShift - kLazy) = 32, twice
+constexpr uint32_t kSignBits = 0xB1A6D4B2u;   // bit d: dim d of a block changes its sign (src/cache/precomputed/rotation.rs:16-20)
 constexpr float kQMax = 32639.0f;   // 127 * 256 + 127
 
 template <int BYTES>
@@ -247,43 +248,85 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG, BITS>::kCtas) paged
 #pragma unroll
         for (int e = 0; e < kE; ++e) qsc[e] = 0.0f;
         if (have) {
-            const float inv_sqrt = 1.0f / sqrtf((float)kBlock), sg = block_sign(lane, a.sign_mag);
-            // Fragment (b, 4n' + j') of column n' has eight dims from 32 b + 8 j' on, a byte each.  4-bit: the even ones (k-slots 4j' ..)
-            // in its first word, the odd ones (k-slots 16 + 4j' ..) in the second; 3-bit: the first four, the last four.
-            unsigned char* const at = s_digits + (lane >> 3) * 8 + (BITS == 4 ? (lane & 1) * 4 + ((lane >> 1) & 3) : lane & 7);
+            // A lane takes 16 dims of a block: four stages of the butterfly are its own, one is a shuffle away, and its digits are 16
+            // bytes of each of the fragments.  (A dim a lane, 80 shuffles and 32 byte stores a segment: 2.7 us instead of 1.2.)
+            const float inv_sqrt = 1.0f / sqrtf((float)kBlock);
+            constexpr int kHeads = 16 / NB;       // of a pass
+            const int b = (lane >> 1) % NB, part = lane & 1;
+            const uint32_t neg = kSignBits >> (16 * part);
 #pragma unroll 1
-            for (int h = 0; h < HG; ++h) {
-                float v[NB];
+            for (int h0 = 0; h0 < HG; h0 += kHeads) {
+                const int h = h0 + (lane >> 1) / NB;
+                uint4 raw[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    raw[k] = h < s.heads ? *reinterpret_cast<const uint4*>(s_queries + (h * D + b * 32 + part * 16 + 8 * k) * 2) : make_uint4(0u, 0u, 0u, 0u);
+                float v[16];
+                const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float2 f = __half22float2(u32_as_h2(w[i]));
+                    const bool half = a.q_dtype == TQB_F16;
+                    v[2 * i] = half ? f.x : __uint_as_float(w[i] << 16);
+                    v[2 * i + 1] = half ? f.y : __uint_as_float(w[i] & 0xffff0000u);
+                }
+#pragma unroll
+                for (int m = 1; m < 16; m <<= 1)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if ((i & m) == 0) {
+                            const float x = v[i], y = v[i + m];
+                            v[i] = x + y;
+                            v[i + m] = x - y;
+                        }
                 uint32_t top = 0;   // of the bits, so that NaN is above infinity
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    v[b] = h < s.heads ? load_as_f32(s_queries, a.q_dtype, h * D + b * 32 + lane) : 0.0f;
-                    v[b] = wht32_across(v[b], lane) * inv_sqrt * sg;
-                    top = max(top, __float_as_uint(v[b]) & 0x7fffffffu);
+                for (int i = 0; i < 16; ++i) {
+                    const float other = __shfl_xor_sync(0xffffffffu, v[i], 1);
+                    v[i] = (part ? other - v[i] : v[i] + other) * inv_sqrt * a.sign_mag;
+                    top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+                    v[i] = __uint_as_float(__float_as_uint(v[i]) ^ ((neg << (31 - i)) & 0x80000000u));
                 }
-                float m = __uint_as_float(__reduce_max_sync(0xffffffffu, top));
-                if (!(m <= FLT_MAX)) m = __uint_as_float(0x7fc00000u);   // not finite: every score is NaN
-                const float inv = m > 0.0f ? kQMax / m : 0.0f;
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    // (inv is infinite where the largest component is below 1e-34)
-                    const int x = inv <= FLT_MAX ? __float2int_rn(v[b] * inv) : 0;
-                    const int lo = (int)(signed char)(x & 0xff), hi = (x - lo) >> 8;
+                for (int o = 1; o < 2 * NB; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                float m = __uint_as_float(top);
+                if (!(m <= FLT_MAX)) m = __uint_as_float(0x7fc00000u);   // not finite: every score is NaN
+                float inv = m > 0.0f ? kQMax / m : 0.0f;
+                if (!(inv <= FLT_MAX)) inv = 0.0f;                       // the largest component is below 1e-34, or not finite
+                // x = 256 hi + lo, both signed: hi is byte 1 of x + 128.  Fragment (b, 4n' + j') of column n' has eight dims from
+                // 32 b + 8 j' on, a byte each.  4-bit: the even ones (k-slots 4j' ..) in its first word, the odd ones (k-slots
+                // 16 + 4j' ..) in the second; 3-bit: the first four, the last four.
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t x[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] = (uint32_t)__float2int_rn(v[BITS == 4 ? 8 * (k >> 1) + 2 * i + (k & 1) : 4 * k + i] * inv);
+                    lo[k] = __byte_perm(__byte_perm(x[0], x[1], 0x0040), __byte_perm(x[2], x[3], 0x0040), 0x5410);
+                    hi[k] = __byte_perm(__byte_perm(x[0] + 128u, x[1] + 128u, 0x0051), __byte_perm(x[2] + 128u, x[3] + 128u, 0x0051), 0x5410);
+                }
+                const uint4 hi4 = make_uint4(hi[0], hi[1], hi[2], hi[3]), lo4 = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                if (h < HG) {
+                    unsigned char* const at = s_digits + b * 256 + part * 16;   // column 0
                     if (HG == 4) {
-                        at[b * 256 + (2 * h) * 32] = (unsigned char)hi;
-                        at[b * 256 + (2 * h + 1) * 32] = (unsigned char)lo;
+                        *reinterpret_cast<uint4*>(at + 2 * h * 32) = hi4;
+                        *reinterpret_cast<uint4*>(at + (2 * h + 1) * 32) = lo4;
                         if (BITS == 3) {
-                            at[(NB + b) * 256 + (2 * h) * 32] = 0;
-                            at[(NB + b) * 256 + (2 * h + 1) * 32] = (unsigned char)hi;
+                            *reinterpret_cast<uint4*>(at + NB * 256 + 2 * h * 32) = make_uint4(0u, 0u, 0u, 0u);
+                            *reinterpret_cast<uint4*>(at + NB * 256 + (2 * h + 1) * 32) = hi4;
                         }
                     } else {
-                        at[b * 256 + h * 32] = (unsigned char)hi;
-                        at[(NB + b) * 256 + h * 32] = (unsigned char)lo;
+                        *reinterpret_cast<uint4*>(at + h * 32) = hi4;
+                        *reinterpret_cast<uint4*>(at + NB * 256 + h * 32) = lo4;
                     }
                 }
 #pragma unroll
-                for (int e = 0; e < kE; ++e)
-                    if (h == (HG == 4 ? j : 2 * j + e)) qsc[e] = m * (a.qk_const * (BITS == 4 ? step / (kQMax * 16.0f) : a.cent[7] * 256.0f / (kQMax * kQMax)));
+                for (int e = 0; e < kE; ++e) {
+                    const int mine = (HG == 4 ? j : 2 * j + e) - h0;   // the lane's head, counted from the pass's first
+                    const float mh = __shfl_sync(0xffffffffu, m, mine * 2 * NB);
+                    if (mine >= 0 && mine < kHeads)
+                        qsc[e] = mh * (a.qk_const * (BITS == 4 ? step / (kQMax * 16.0f) : a.cent[7] * 256.0f / (kQMax * kQMax)));
+                }
             }
             __syncwarp();
         }
