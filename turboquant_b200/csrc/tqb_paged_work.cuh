@@ -348,7 +348,7 @@ __device__ __forceinline__ void finish(const PagedArgs& a, const Fragments& f, F
         // the fragments of one (request, head): up to the next odd slot
         const unsigned odd = used & 0xaau & ~((2u << c0) - 1), mine = used & (odd != 0 ? (odd & (0u - odd)) - 1 : ~0u);
         used &= ~mine;
-        const int last = 31 - __clz(mine);
+        const int last = 31 - __clz(mine), count = __popc(mine);
         const Segment& s = f.seg[c0];
         const bool done = s.begins && f.seg[last].ends;
         const int side = s.begins ? 1 : 0;
@@ -358,14 +358,25 @@ __device__ __forceinline__ void finish(const PagedArgs& a, const Fragments& f, F
 #pragma unroll 1
         for (int x0 = warp * 32; x0 < quads; x0 += kWorkThreads) {
             const int x = min(x0 + lane, quads - 1), hh = x / (D / 4);
-            Running r;
-#pragma unroll 1
-            for (unsigned m = mine; m != 0; m &= m - 1) r.M = fmaxf(r.M, f.m[__ffs(m) - 1][hh]);
-#pragma unroll 1
-            for (unsigned m = mine; m != 0; m &= m - 1) {
-                const int c = __ffs(m) - 1;
-                r.add(f.m[c][hh], f.l[c][hh], quad(c, x));
+            // at most one fragment of a warp: read together (past the last: that one again, with weight 0)
+            float m[kWorkWarps], l[kWorkWarps];
+            float4 o[kWorkWarps];
+            unsigned left = mine;
+            int c = c0;
+#pragma unroll
+            for (int k = 0; k < kWorkWarps; ++k) {
+                c = left != 0 ? __ffs(left) - 1 : c;
+                left &= left - 1;
+                m[k] = f.m[c][hh];
+                l[k] = f.l[c][hh];
+                o[k] = quad(c, x);
             }
+            Running r;
+#pragma unroll
+            for (int k = 0; k < kWorkWarps; ++k) r.M = fmaxf(r.M, m[k]);
+#pragma unroll
+            for (int k = 0; k < kWorkWarps; ++k)
+                if (k < count) r.add(m[k], l[k], o[k]);
             if (done) {
                 write_quad(a.out, a.out_dtype, quad_at<NB>(a, s, x), x0 + lane < quads, r.O, r.L, a.sign_mag);
             } else if (x0 + lane < quads) {
