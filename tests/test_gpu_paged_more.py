@@ -183,3 +183,28 @@ def test_cache_decodes_under_capture_and_on_streams():
     captured.zero_()
     graph.replay()
     assert torch.equal(other, want) and torch.equal(captured, want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_attention_of_lengths_beyond_the_table_and_below_zero(dtype):
+    g, dt, page, dim, hkv, group = gen(9), DT[dtype], 32, 64, 3, 5
+    layer = filled(20, hkv, page, dim, 4, g)
+    table = table_of([96, 96, 96], page, 20, g)
+    q = torch.randn((3, hkv * group, dim), generator=g, device="cuda").to(dt)
+    out = layer.attend(q, table, torch.tensor([97, -5, 2 ** 31 - 1], dtype=torch.int32, device="cuda"), 0.1)
+    cut = torch.tensor([96, 0, 96], dtype=torch.int32, device="cuda")
+    assert torch.equal(out, layer.attend(q, table, cut, 0.1)) and bool((out[1] == 0).all())
+    check_attention(out, q, layer, table, cut, 0.1, dt)
+
+
+@pytest.mark.parametrize("bits,group,page", [(3, 3, 1024), (4, 17, 16), (3, 20, 256), (4, 1, 512)])
+@pytest.mark.parametrize("scale", [0.0, -0.1, 0.5])
+def test_attention_of_odd_groups_pages_and_scales(bits, group, page, scale):
+    lens = [1500, 1, 0, 777, 16]
+    for dim, dtype in ((64, "f16"), (128, "bf16"), (256, "f32")):
+        g, dt, hkv = gen(dim + group), DT[dtype], 3
+        pages = sum(-(-n // page) for n in lens)
+        layer, table = filled(pages, hkv, page, dim, bits, g), table_of(lens, page, pages, g)
+        ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        q = torch.randn((5, hkv * group, dim), generator=g, device="cuda").to(dt)
+        check_attention(layer.attend(q, table, ln, scale), q, layer, table, ln, scale, dt)
