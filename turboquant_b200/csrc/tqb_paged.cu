@@ -206,9 +206,10 @@ __global__ void __launch_bounds__(kReleaseThreads) release_kernel(const uint8_t*
 //   (pqo_quantize_values), 16 or 12 bytes of codes.  Four lanes a block with the butterfly's last stages as shuffles needs three
 //   times the instructions.
 // Bound: instructions and the latency of the passes: 8,191 tokens of 32 + 8 heads, head_dim 128, normed and rotated 43 us (3.9
-// TB/s; a plain copy of these bytes takes 32), one token 2.8 us; 6,007 tokens of 16 + 8 heads rotated and packed to 3 bits 30 us.
+// TB/s; a plain copy of these bytes takes 32), one token 2.8 us; 6,007 tokens of 16 + 8 heads rotated and packed to 3 bits 28.5 us.
 constexpr int kRowThreads = 256;
-constexpr int kRowWarps = kRowThreads / 32;
+constexpr int kRowWarps = kRowThreads / 32, kRowWarpsLog = 3;
+static_assert(kRowWarps == 1 << kRowWarpsLog, "");
 
 // x / d for x below 2^31 by a multiplication: m = floor(2^(31 + s) / d) + 1 with 2^(s - 1) < d <= 2^s errs by less than 1 / d
 // (Granlund and Montgomery, PLDI 1994).
@@ -238,7 +239,8 @@ struct RowArgs {
     uint16_t* sc[2];
     long long num_slots;
     int tokens, rot_dim, flags, kv_heads, page_shift;
-    int shared_token, token_bytes;   // rows_kernel: a CTA for each token; shared memory for a token
+    int at_once, token_bytes;        // rows_kernel: the CTA takes 1 << at_once tokens at a time; shared memory for a token
+    int per_cta, one_more;           // tokens of a CTA; the first CTAs take one more
     unsigned total;         // append_kernel: blocks of K (or V), below 2^31 - 2^20
     Divisor by_kv;
     float eps;
@@ -734,56 +736,71 @@ struct NoRows {   // (do_rows_part reads for itself)
     __device__ __forceinline__ NoRows(const A&...) {}
 };
 
-// Rows that are packed (BITS != 0), or of which only the first rot_dim elements turn (PART): a token a warp; where there are few
-// tokens (`shared_token`), a token a CTA.
+// Rows that are packed (BITS != 0), or of which only the first rot_dim elements turn (PART).  A CTA takes tokens blockIdx.x +
+// i gridDim.x: eight at a time, a warp each (fewer where the tiles need more room); if not more than half of that are left, the
+// warps share them, so that a last round with few tokens is a short one.  (1,183 tokens of 16 + 8 heads to 3 bits: 7.9 us; with a
+// CTA for each token 14.8; 2,401 tokens 13.7 us, with a warp for each 16.5.)
 template <typename T, int LPH, int BITS, bool PART>
 __global__ void __launch_bounds__(kRowThreads, PART ? 3 : 2) rows_kernel(const __grid_constant__ RowArgs a, const __grid_constant__ Codebook cb) {
     constexpr int D = LPH * 8, NB = D / 32;
     using R = Rows<T, LPH, true>;
-    extern __shared__ __align__(16) unsigned char s_dyn[];
+    extern __shared__ __align__(16) unsigned char s_dyn[];   // [rings][token: cosines, sines, keys' blocks]
     __shared__ float2 s_cells[BITS == 3 ? kCells * 32 : 1];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int half = a.rot_dim >> 1, part = a.shared_token ? warp : 0, parts = a.shared_token ? kRowWarps : 1;
-    const int me = a.shared_token ? tid : lane, all = a.shared_token ? kRowThreads : 32;
-    unsigned char* const mine = s_dyn + (PART ? 0 : kRowWarps * kRingBytes) + (a.shared_token ? 0 : (size_t)warp * a.token_bytes);   // [cosines][sines][keys' blocks]
-    float* const s_cos = reinterpret_cast<float*>(mine);
-    float* const s_sin = s_cos + D / 2;
-    unsigned char* const s_tile = mine + (half > 0 ? D * sizeof(float) : 0);
-    auto sync = [&]() {
-        if (a.shared_token) __syncthreads();
-        else __syncwarp();
-    };
+    const int half = a.rot_dim >> 1, passes = R::passes_of(a.q.heads) + R::passes_of(a.k.heads);
     if (BITS == 3) {
         build_cell_table(cb, cb.n - 1, s_cells, tid, kRowThreads);
         __syncthreads();
     }
-    const int per_cta = a.shared_token ? 1 : kRowWarps, step = gridDim.x * per_cta;
-    const int passes = R::passes_of(a.q.heads) + R::passes_of(a.k.heads);
-    const Units u{a.tokens, step, passes, 1, Divisor()};   // whole tokens
-    typename std::conditional<PART, NoRows, R>::type rows(a, u, blockIdx.x * per_cta + (a.shared_token ? 0 : warp), part, parts, s_dyn + (size_t)warp * kRingBytes);
-    for (int t = blockIdx.x * per_cta + (a.shared_token ? 0 : warp); t < a.tokens; t += step) {
-        if constexpr (PART) {
-            angles(a, t, s_cos, s_sin, me, all);
-            sync();
-            if (a.q.heads > 0) do_rows_part<T, LPH, false>(a, a.q, t, part, parts, s_cos, s_sin, s_tile);
-            if (a.k.heads > 0) do_rows_part<T, LPH, BITS != 0>(a, a.k, t, part, parts, s_cos, s_sin, s_tile);
-        } else {
-            if (half > 0) {
+    const int mine = a.per_cta + ((int)blockIdx.x < a.one_more ? 1 : 0);
+    int shift = a.at_once, rounds = (mine >> shift) + (2 * (mine & ((1 << shift) - 1)) > 1 << shift ? 1 : 0);
+#pragma unroll 1
+    for (int done = 0; done < mine; rounds = 0) {
+        if (rounds == 0) {
+            rounds = 1;
+            shift = 0;
+            while (1 << shift < mine - done) ++shift;
+        }
+        const int parts = kRowWarps >> shift, group = warp >> (kRowWarpsLog - shift), part = warp & (parts - 1);   // `parts` warps share a token
+        const int me = tid - group * parts * 32, all = parts * 32;
+        auto sync = [&]() {
+            if (parts == 1) __syncwarp();
+            else asm volatile("bar.sync %0, %1;\n" ::"r"(1 + group), "r"(all) : "memory");
+        };
+        unsigned char* const space = s_dyn + (PART ? 0 : kRowWarps * kRingBytes) + (size_t)group * a.token_bytes;
+        float* const s_cos = reinterpret_cast<float*>(space);
+        float* const s_sin = s_cos + D / 2;
+        unsigned char* const s_tile = space + (half > 0 ? D * sizeof(float) : 0);
+        const int first = blockIdx.x + (done + group) * gridDim.x, step = gridDim.x << shift;
+        done += rounds << shift;
+        const int end = min(a.tokens, (int)(blockIdx.x + done * gridDim.x));
+        const Units u{end, step, passes, 1, Divisor()};   // whole tokens
+        typename std::conditional<PART, NoRows, R>::type rows(a, u, first, part, parts, s_dyn + (size_t)warp * kRingBytes);
+        for (int t = first; t < end; t += step) {
+            if constexpr (PART) {
                 angles(a, t, s_cos, s_sin, me, all);
                 sync();
+                if (a.q.heads > 0) do_rows_part<T, LPH, false>(a, a.q, t, part, parts, s_cos, s_sin, s_tile);
+                if (a.k.heads > 0) do_rows_part<T, LPH, BITS != 0>(a, a.k, t, part, parts, s_cos, s_sin, s_tile);
+            } else {
+                if (half > 0) {
+                    angles(a, t, s_cos, s_sin, me, all);
+                    sync();
+                }
+                rows.run(t, part, passes, s_cos, s_sin, s_tile);
             }
-            rows.run(t, part, passes, s_cos, s_sin, s_tile);
-        }
-        if constexpr (BITS != 0) {
-            sync();
-            const int per_side = a.kv_heads * NB;
-            for (int i = me; i < 2 * per_side; i += all) {   // [K, V][head][block]
-                const int side = i >= per_side ? 1 : 0, at = i - side * per_side;
-                pack_block<T, BITS, NB>(a, cb, side, t, (unsigned)at / NB, (unsigned)at % NB, side == 0 ? s_tile + (size_t)at * Tile<T>::kPitch : nullptr,
-                                        BITS == 3 ? s_cells + lane : nullptr);
+            if constexpr (BITS != 0) {
+                sync();
+                const int per_side = a.kv_heads * NB;
+                for (int i = me; i < 2 * per_side; i += all) {   // [K, V][head][block]
+                    const int side = i >= per_side ? 1 : 0, at = i - side * per_side;
+                    pack_block<T, BITS, NB>(a, cb, side, t, (unsigned)at / NB, (unsigned)at % NB, side == 0 ? s_tile + (size_t)at * Tile<T>::kPitch : nullptr,
+                                            BITS == 3 ? s_cells + lane : nullptr);
+                }
             }
+            sync();   // angles and tile are free again
         }
-        sync();   // angles and tile are free again
+        if (done < mine) __syncthreads();   // other warps share a space next
     }
 }
 
@@ -918,11 +935,10 @@ int launch_rows_one(RowArgs& a, const Codebook& cb, cudaStream_t s) {
     const size_t token = (BITS == 0 ? 0 : (size_t)blocks_of_token * Tile<T>::kPitch) + (a.rot_dim > 0 ? (size_t)LPH * 8 * sizeof(float) : 0);
     if (token > 128 * 1024) return TQB_ERR_UNSUPPORTED;
     a.token_bytes = (int)token;
-    // A warp has some 20 passes a token: below as many tokens as two warps an SM scheduler want, and where eight tokens take too
-    // much room, a CTA shares them.
-    a.shared_token = a.tokens < 148 * 8 || token * kRowWarps > 72 * 1024 ? 1 : 0;
+    a.at_once = kRowWarpsLog;
+    while (a.at_once > 0 && token << a.at_once > 72 * 1024) --a.at_once;
     const bool partly = a.rot_dim > 0 && a.rot_dim < LPH * 8;
-    const int bytes = (int)(token * (a.shared_token ? 1 : kRowWarps)) + (partly ? 0 : kRowWarps * kRingBytes);
+    const int bytes = (int)(token << a.at_once) + (partly ? 0 : kRowWarps * kRingBytes);
     if constexpr (BITS == 0) {
         if (!partly) {
             using R = Rows<T, LPH, false>;
@@ -944,8 +960,10 @@ int launch_rows_one(RowArgs& a, const Codebook& cb, cudaStream_t s) {
             return check_launch(s);
         }
     }
-    const long long want = a.shared_token ? a.tokens : (a.tokens + kRowWarps - 1) / kRowWarps;
-    const unsigned grid = (unsigned)(want < 148 * 2 || a.shared_token ? want : 148 * 2);
+    const int most = 148 * (partly && bytes <= 64 * 1024 ? 3 : 2);
+    const int grid = a.tokens < most ? a.tokens : most;
+    a.per_cta = a.tokens / grid;
+    a.one_more = a.tokens % grid;
     if (partly) {
         if (int st = allow_shared<rows_kernel<T, LPH, BITS, true>>(bytes, 160 * 1024)) return st;
         rows_kernel<T, LPH, BITS, true><<<grid, kRowThreads, bytes, s>>>(a, cb);
