@@ -806,9 +806,9 @@ __global__ void __launch_bounds__(kRowThreads, PART ? 3 : 2) rows_kernel(const _
 
 // ---- rows back from pages ----------------------------------------------------------------------------------------------
 // One lane a 32-block as in tqb_block_dequantize, whose values these are; the warp's 32 blocks leave through shared memory as
-// dense 512-byte stores, and the next blocks' codes are in flight.  Bound: instructions (a shift, a selection and a look-up for
-// each value), then HBM: 32,768 tokens of 8 heads, head_dim 128, 4 bits to bf16 41 us (4.1 TB/s; stages with a padded pitch, whose
-// reads met in banks, 43.6).
+// dense 512-byte stores, and the next blocks' codes are in flight.  Bound: HBM writes: 32,768 tokens of 8 heads, head_dim 128, 4
+// bits to bf16 41.5 us, where a fill of the 134 MB that are written takes 35 (stages with a padded pitch, whose reads met in banks:
+// 43.6; 4-bit centroids computed from the codes instead of looked up: 43.4).
 struct BackArgs {
     const uint8_t* idx[2];
     const uint16_t* sc[2];
