@@ -468,7 +468,7 @@ block_dequantize_lane_kernel(DequantArgs a, Codebook cb) {
     const int lane = threadIdx.x & 31;
     build_dequant_table<BITS>(cb, a.sign_mag, s_tab, threadIdx.x, kThreads);
     __syncthreads();
-    const uint32_t tab = (uint32_t)__cvta_generic_to_shared(s_tab), lane4 = lane * 4;
+    const uint32_t lane4 = lane * 4;
     unsigned char* stage = s_stage + (threadIdx.x >> 5) * 32 * kPitch;
     const unsigned total = (unsigned)(a.n_rows * a.nblk), nblk = (unsigned)a.nblk;
     for (unsigned blk0 = (blockIdx.x * kThreads + threadIdx.x) & ~31u; blk0 < total; blk0 += gridDim.x * kThreads) {
@@ -488,7 +488,7 @@ block_dequantize_lane_kernel(DequantArgs a, Codebook cb) {
         }
         const F2 as = f2(fabsf(f16_bits_to_f32(__ldg(a.scales + sblk))));
         float v[32];
-        dequantize_values<BITS>(w, as, tab, lane4, v);
+        dequantize_values<BITS>(w, as, s_tab, lane4, v);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             float e[8];

@@ -807,7 +807,7 @@ __global__ void __launch_bounds__(kRowThreads, PART ? 3 : 2) rows_kernel(const _
 // ---- rows back from pages ----------------------------------------------------------------------------------------------
 // One lane a 32-block as in tqb_block_dequantize, whose values these are; the warp's 32 blocks leave through shared memory as
 // dense 512-byte stores, and the next blocks' codes are in flight.  Bound: HBM writes: 32,768 tokens of 8 heads, head_dim 128, 4
-// bits to bf16 41.5 us, where a fill of the 134 MB that are written takes 35 (stages with a padded pitch, whose reads met in banks:
+// bits to bf16 41.0 us, where a fill of the 134 MB that are written takes 35 (stages with a padded pitch, whose reads met in banks:
 // 43.6; 4-bit centroids computed from the codes instead of looked up: 43.4).
 struct BackArgs {
     const uint8_t* idx[2];
@@ -831,7 +831,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) back_kernel(const __grid_const
     const int tid = threadIdx.x, lane = tid & 31, side = blockIdx.y;
     build_dequant_table<BITS>(cb, a.sign_mag, s_tab, tid, kRowThreads);
     __syncthreads();
-    const uint32_t tab = (uint32_t)__cvta_generic_to_shared(s_tab), lane4 = lane * 4;
+    const uint32_t lane4 = lane * 4;
     unsigned char* stage = s_stage + (tid >> 5) * 32 * kPitch;
     const unsigned total = a.total, step = gridDim.x * kRowThreads;
     uint32_t w[4] = {0u, 0u, 0u, 0u};
@@ -860,7 +860,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) back_kernel(const __grid_const
     if (blk0 + step < total) slot = slot_of(blk0 + step);
     for (; blk0 < total; blk0 += step) {
         float v[32];
-        dequantize_values<BITS>(w, f2(scale), tab, lane4, v);
+        dequantize_values<BITS>(w, f2(scale), s_tab, lane4, v);
         const bool live = in;
         if (blk0 + step < total) {
             fetch(blk0 + step, slot);

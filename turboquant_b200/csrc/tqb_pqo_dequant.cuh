@@ -25,10 +25,10 @@ __device__ __forceinline__ void build_dequant_table(const Codebook& cb, float si
     }
 }
 
-// w: the block's packed codes; as: (|scale|, |scale|); tab: shared address of the table; lane4: 4 * lane.  (The address is added,
-// not or-ed in: a block's shared memory need not begin at a multiple of 2048.  A constant, it costs nothing.)
+// w: the block's packed codes; as: (|scale|, |scale|); tab: the table, in shared memory; lane4: 4 * lane.  (The table's address is
+// added to the row's, as a constant of the load: it need not be a multiple of the table's size.)
 template <int BITS>
-__device__ __forceinline__ void dequantize_values(const uint32_t (&w)[4], F2 as, uint32_t tab, uint32_t lane4, float (&v)[32]) {
+__device__ __forceinline__ void dequantize_values(const uint32_t (&w)[4], F2 as, const unsigned char* tab, uint32_t lane4, float (&v)[32]) {
     using D = DequantTable<BITS>;
     const F2 inv_sqrt = f2(1.0f / sqrtf((float)kBlock));
 #pragma unroll
@@ -36,9 +36,8 @@ __device__ __forceinline__ void dequantize_values(const uint32_t (&w)[4], F2 as,
         // the code moved to bits 7.. (its row of 128 bytes), the lane's bank below it
         const int k = (BITS * i) >> 5, sh = (BITS * i) & 31;
         const uint32_t m = sh < 7 ? w[k] << (7 - sh) : (sh + BITS <= 32 ? w[k] >> (sh - 7) : __funnelshift_r(w[k], w[k < 3 ? k + 1 : 3], sh - 7));
-        const uint32_t addr = ((m & ((D::kCodes - 1) << 7)) | lane4) + tab;
-        if ((kSignMask >> i) & 1u) asm("ld.shared.f32 %0, [%1+%2];" : "=f"(v[i]) : "r"(addr), "n"(D::kBytes) : "memory");
-        else asm("ld.shared.f32 %0, [%1];" : "=f"(v[i]) : "r"(addr) : "memory");
+        const float* const row = reinterpret_cast<const float*>(tab + ((m & ((D::kCodes - 1) << 7)) | lane4));
+        v[i] = row[((kSignMask >> i) & 1u) ? D::kBytes / 4 : 0];
     }
     F2 p[16];
 #pragma unroll
