@@ -14,10 +14,10 @@ namespace {
 // need.  Every CTA does the two prefix sums over the requests for itself (8 bytes a request from L2) and then takes its
 // share of the tokens and of the new table entries; nobody waits for anybody.  What may be updated in place - lengths and
 // state - is written by the CTA that finishes last, when all have read it.  Bound: launch and dependent loads: 64 requests of a
-// token each 3.6 us, 211 requests that bring up to 511 tokens each 4.5 us.
+// token each 3.8 us, 211 requests that bring up to 511 tokens each 5.2 us.
 constexpr int kMostCounted = 1 << 30;   // tokens of a plan or of rows that turn: an index and a grid's stride stay below 2^31
 constexpr int kPlanThreads = 256;
-constexpr int kPlanTokens = 256;    // tokens a CTA, up to 148 CTAs (1,024: 6.5 us for the 211 requests)
+constexpr int kPlanTokens = 256;    // tokens a CTA, up to 148 CTAs (1,024: 7.2 us for the 211 requests)
 
 struct PlanArgs {
     const int32_t* seq;

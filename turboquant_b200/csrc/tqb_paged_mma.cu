@@ -115,7 +115,7 @@ struct Plan {
     static constexpr int kQueries = HG * NB * 32 * 2;             // the next segment's queries as they are
     static constexpr int kWarpBytes = G::kWarpRing + kFragment + kDigits + kQueries;   // [ring][fragment that began before][digits][queries]
     static constexpr int kBytes = kWorkWarps * kWarpBytes;
-    // CTAs of an SM: by shared memory, and so that registers do not spill
+    // CTAs of an SM: by shared memory, and by registers (up to 12 words a thread spill)
     static constexpr int kByShared = 228 * 1024 / (kBytes + 1024 + 2560 + (BITS == 3 ? 8192 : 0)), kByRegs = NB == 8 ? (HG == 8 ? 2 : 3) : HG == 8 ? 4 : NB == 2 ? 5 : 4;
     static constexpr int kCtas = kByShared < kByRegs ? kByShared : kByRegs;
 };
