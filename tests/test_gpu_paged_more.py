@@ -208,3 +208,18 @@ def test_attention_of_odd_groups_pages_and_scales(bits, group, page, scale):
         ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
         q = torch.randn((5, hkv * group, dim), generator=g, device="cuda").to(dt)
         check_attention(layer.attend(q, table, ln, scale), q, layer, table, ln, scale, dt)
+
+
+@pytest.mark.parametrize("dtype,bits", [("bf16", 4), ("f32", 3)])
+@pytest.mark.parametrize("every", [0, 1, 97])
+def test_attention_of_as_many_requests_as_may_be(every, dtype, bits):
+    """4,096 requests: none with tokens, all, and a few of a padded batch."""
+    g, dt, page, dim, hkv, group, n = gen(10), DT[dtype], 16, 64, 1, 2, 4096
+    lens = [(1 + i * 31 % 70) if every and i % every == every - 1 else 0 for i in range(n)]
+    pages = sum(-(-x // page) for x in lens) + 1
+    layer = filled(pages, hkv, page, dim, bits, g)
+    table, ln = table_of(lens, page, pages, g), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q = torch.randn((n, hkv * group, dim), generator=g, device="cuda").to(dt)
+    out = layer.attend(q, table, ln, 0.1, out=torch.full_like(q, 7))
+    check_attention(out, q, layer, table, ln, 0.1, dt)
+    assert bool((out[ln == 0] == 0).all())
