@@ -22,9 +22,9 @@
 //   of the MMA's adder relative to 7.5 sum P'.
 //   Where some |s_v| is above 32, so that a product could leave f16, the warp lowers kShift by as much.
 //
-// Measured (8 KV heads, head_dim 128, 4 bits, bf16): 64 requests of 8,192 tokens, four query heads a KV head 103 us (5.9 TB/s, 0.9
-// of a copy); 64 of 531 to 8,192 tokens 45.4 us (of which 6 us until the first products and 6 for the joins); one of 131,072
-// tokens 38.5 us.  What binds then is HBM.  Eight query heads 58 us and 48 us: instructions, on 12 warps an SM (registers and
+// Measured (8 KV heads, head_dim 128, 4 bits, bf16): 64 requests of 8,192 tokens, four query heads a KV head 101.5 us (6.0 TB/s, 0.91
+// of a copy); 64 of 531 to 8,192 tokens 43.9 us (of which 6 us until the first products and 5 for the joins); one of 131,072
+// tokens 36.9 us.  What binds then is HBM.  Eight query heads 59 us and 50 us: instructions, on 12 warps an SM (registers and
 // shared memory); three bits 72 us, 97 requests of up to 2,003 tokens 39.4 us: instructions, twice as many a token as with four
 // bits, for codes that cross words and whose centroids come out of tables.
 #include "tqb_common.cuh"
@@ -115,8 +115,9 @@ struct Plan {
     static constexpr int kQueries = HG * NB * 32 * 2;             // the next segment's queries as they are
     static constexpr int kWarpBytes = G::kWarpRing + kFragment + kDigits + kQueries;   // [ring][fragment that began before][digits][queries]
     static constexpr int kBytes = kWorkWarps * kWarpBytes;
-    // CTAs of an SM: by shared memory, and by registers (up to 12 words a thread spill)
-    static constexpr int kByShared = 228 * 1024 / (kBytes + 1024 + 2560 + (BITS == 3 ? 8192 : 0)), kByRegs = NB == 8 ? (HG == 8 ? 2 : 3) : HG == 8 ? 4 : NB == 2 ? 5 : 4;
+    // CTAs of an SM: by shared memory, and three, so that registers hardly spill and fewer parts are joined (two for head_dim 256).
+    // 64 requests of 531 to 8,192 tokens, four heads: 43.9 us; with two 46.7, with four 45.2; head_dim 64 32.8, with five 33.8.
+    static constexpr int kByShared = 228 * 1024 / (kBytes + 1024 + 2560 + (BITS == 3 ? 8192 : 0)), kByRegs = NB == 8 ? 2 : 3;
     static constexpr int kCtas = kByShared < kByRegs ? kByShared : kByRegs;
 };
 
