@@ -4,11 +4,11 @@
 // table), request after request, within a request KV head after KV head (a group of more than eight query heads counts as
 // several), within a head token after token; kOpenCost units stand before each (request, head) for what it takes to begin
 // one.  Every WARP takes an equal run of the line, whatever the lengths are, worked out on the device from the lengths, so
-// that a captured launch serves any batch.  A run is cut into segments, one for each (request, head) that it touches.  A warp writes a segment that is the whole of its (request, head) to the
-// output by itself.  It has at most two others: one that began before it and one that goes on behind it.  These stay in
-// shared memory until the CTA's four warps are done and are joined there, and what crosses the CTA's ends goes to the
-// scratch (again at most two parts), where the CTA that arrives last at the (request, head)'s ticket joins the parts in the
-// order of the CTAs.  The result depends on the lengths alone.
+// that a captured launch serves any batch.  A run is cut into segments, one for each (request, head) that it touches.  A warp
+// writes a segment that is the whole of its (request, head) to the output by itself.  It has at most two others: one that began
+// before it and one that goes on behind it.  These stay in shared memory until the CTA's four warps are done and are joined
+// there, and what crosses the CTA's ends goes to the scratch (again at most two parts), where the CTA that arrives last at the
+// (request, head)'s ticket joins the parts in the order of the CTAs.  The result depends on the lengths alone.
 //
 // Measured at 128 requests of 62 to 1,000 tokens (8 KV heads, 4-bit): with CTAs instead of warps taking the runs, every
 // short segment paid its loads' latency and eight block barriers: 64 us.
@@ -19,8 +19,11 @@
 namespace tqb {
 
 constexpr int kRunTokens = 16;       // of a group
+// Measured with 3, 4, 5, 6, 8 groups: 64 requests of 531 to 8,192 tokens 44.6, 44.7, 44.3, 43.8, 43.9 us, 256 of 19 to 300 tokens
+// 21.9, 20.9, 20.6, 21.0, 21.1; and with runs of at least 2, 4, 6, 8 units: one request of 1,000 tokens 9.3, 10.3, 10.0, 10.7, four of
+// them 11.0, 10.3, 10.0, 10.7.
 constexpr int kOpenCost = 6;         // groups that beginning a segment is worth
-constexpr int kMinRun = 4;           // units of a run, at least
+constexpr int kMinRun = 6;           // units of a run, at least
 constexpr int kSegHeads = 8;         // query heads of a segment, at most
 constexpr int kWorkWarps = 4;
 constexpr int kWorkThreads = 32 * kWorkWarps;
