@@ -223,3 +223,29 @@ def test_attention_of_as_many_requests_as_may_be(every, dtype, bits):
     out = layer.attend(q, table, ln, 0.1, out=torch.full_like(q, 7))
     check_attention(out, q, layer, table, ln, 0.1, dt)
     assert bool((out[ln == 0] == 0).all())
+
+
+@pytest.mark.parametrize("rot", [128, 64])
+@pytest.mark.parametrize("tokens", [5, 1500])
+def test_queries_or_keys_may_be_missing(tokens, rot):
+    """At the C entry points: a null q or k is left out, and the rotated keys of an append are written too where wanted."""
+    from turboquant_b200.paged import _call, lib
+    g, dt, hq, hkv, d = gen(rot), torch.bfloat16, 6, 2, 128
+    q, k, v = (torch.randn((tokens, h, d), generator=g, device="cuda").to(dt) for h in (hq, hkv, hkv))
+    w = torch.randn(d, generator=g, device="cuda").to(dt)
+    rope = tq.QkNormRope(1.0 / torch.arange(1, rot // 2 + 1, device="cuda"), w, w)
+    pos = torch.arange(tokens, device="cuda")
+    qo, ko = rope(q, k, pos)
+    none, rows = (0, 0, 0), lambda t: (t.data_ptr(), t.stride(0), t.stride(1))
+    a, b = torch.zeros_like(q), torch.zeros_like(k)
+    _call(0, lib.tqb_qk_norm_rope, rope._params(rows(q), rows(a), none, none, tokens, hq, hkv, d, dt, pos))
+    _call(0, lib.tqb_qk_norm_rope, rope._params(none, none, rows(k), rows(b), tokens, hq, hkv, d, dt, pos))
+    assert torch.equal(a, qo) and torch.equal(b, ko)
+    one, two = (layer_of(100, hkv, 16, d, 4) for _ in range(2))
+    slots = torch.randperm(1600, generator=g, device="cuda")[:tokens]
+    one.append(ko, v, slots)
+    c = torch.zeros_like(k)
+    _call(0, lib.tqb_paged_append_rope, two._c, rope._params(none, none, rows(k), rows(c), tokens, hq, hkv, d, dt, pos), *rows(v), slots.data_ptr())
+    assert torch.equal(c, ko)
+    for x, y in zip(one.tensors, two.tensors):
+        assert torch.equal(x, y)
