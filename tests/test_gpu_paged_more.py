@@ -249,3 +249,35 @@ def test_queries_or_keys_may_be_missing(tokens, rot):
     assert torch.equal(c, ko)
     for x, y in zip(one.tensors, two.tensors):
         assert torch.equal(x, y)
+
+
+def test_arguments_that_do_not_fit_are_refused():
+    dt, i32 = torch.bfloat16, dict(dtype=torch.int32, device="cuda")
+    layer = layer_of(4, 2, 16, 64, 4)
+    k = torch.zeros((3, 2, 64), dtype=dt, device="cuda")
+    q, slots, pos = torch.zeros((3, 4, 64), dtype=dt, device="cuda"), torch.arange(3, device="cuda"), torch.arange(3, device="cuda")
+    rope = tq.QkNormRope(torch.ones(32, device="cuda"), torch.ones(64, dtype=dt, device="cuda"))
+    table, lens = torch.zeros((3, 2), **i32), torch.ones(3, **i32)
+    wrong = (tq.DimensionMismatch, TypeError, ValueError, tq.TqbRuntimeError)
+    before = [t.clone() for t in layer.tensors]
+    for call in (lambda: layer.append(k, k[:2], slots), lambda: layer.append(k, k.float(), slots), lambda: layer.append(k, k, slots[:2]),
+                 lambda: layer.append(k, k, slots.int()), lambda: layer.append(k[:, :1], k[:, :1], slots), lambda: layer.append(k.double(), k.double(), slots),
+                 lambda: layer.append(k.cpu(), k, slots), lambda: layer.append_rope(rope, q.float(), k, k, pos, slots),
+                 lambda: layer.append_rope(rope, q, k, k, pos[:2], slots), lambda: layer.append_rope(rope, q, k, k, pos.float(), slots),
+                 lambda: layer.append_rope(rope, q, k, k, pos, slots, q_out=q[:2]), lambda: layer.append_rope(rope, q, k, k, pos, slots, q_out=q.transpose(0, 1)),
+                 lambda: rope(q, k, pos, q_out=q[:1].expand(3, 4, 64)), lambda: rope(q, k.half(), pos), lambda: rope(q.half(), k.half(), pos),
+                 lambda: rope(q[..., :32], k[..., :32], pos), lambda: rope(q[0], k, pos),
+                 lambda: layer.attend(q, table, lens.long(), 0.1), lambda: layer.attend(q, table[:2], lens, 0.1), lambda: layer.attend(q[..., :32], table, lens, 0.1),
+                 lambda: layer.attend(q[:, :3], table, lens, 0.1), lambda: layer.attend(q, table.t().contiguous().t(), lens, 0.1),
+                 lambda: layer.attend(q, table, lens, 0.1, scratch=torch.zeros(64, dtype=torch.uint8, device="cuda")),
+                 lambda: layer.attend(q, table, lens, 0.1, out=q[:2]), lambda: layer.attend(q, table, lens, 0.1, out=q.double()),
+                 lambda: layer.attend(q.double(), table, lens, 0.1), lambda: layer.dequantize(slots.int()), lambda: layer.dequantize(slots, torch.float64),
+                 lambda: tq.paged_plan(lens, lens[:2], table, lens, torch.zeros(4, **i32), 16, 3),
+                 lambda: tq.paged_plan(lens, lens, table, lens, torch.zeros(3, **i32), 16, 3), lambda: tq.paged_plan(lens, lens, table, lens, torch.zeros(4, **i32), 15, 3),
+                 lambda: tq.paged_plan(lens, lens, table, lens, torch.zeros(4, **i32), 16, -1),
+                 lambda: tq.PagedLayer(*layer.tensors, 5), lambda: tq.PagedLayer(*layer.tensors, 3), lambda: tq.PagedLayer(*layer.tensors[:3], layer.tensors[3].half(), 4),
+                 lambda: tq.QkNormRope(torch.ones(31, device="cuda"))(q, k, pos), lambda: tq.QkNormRope(torch.ones(64, device="cuda"))(q, k, pos)):
+        with pytest.raises(wrong):
+            call()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(before, layer.tensors))
