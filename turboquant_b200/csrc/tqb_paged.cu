@@ -205,8 +205,8 @@ __global__ void __launch_bounds__(kReleaseThreads) release_kernel(const uint8_t*
 // Blocks: one thread packs one 32-block of the tile, or of the values where they lie, as tqb_block_quantize does
 //   (pqo_quantize_values), 16 or 12 bytes of codes.  Four lanes a block with the butterfly's last stages as shuffles needs three
 //   times the instructions.
-// Bound: instructions and the latency of the passes: 8,191 tokens of 32 + 8 heads, head_dim 128, normed and rotated 43 us (3.9
-// TB/s; a plain copy of these bytes takes 32), one token 2.8 us; 6,007 tokens of 16 + 8 heads rotated and packed to 3 bits 28.5 us.
+// Bound: HBM, at the pace of the slower SMs (without norm and rotation, rows copied by the same kernel take as long): 8,191 tokens
+// of 32 + 8 heads, head_dim 128, normed and rotated 42 us (4.0 TB/s; a plain copy of these bytes takes 32 to 36), one token 2.8 us; 6,007 tokens of 16 + 8 heads rotated and packed to 3 bits 28.5 us.
 constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32, kRowWarpsLog = 3;
 static_assert(kRowWarps == 1 << kRowWarpsLog, "");
@@ -692,6 +692,7 @@ struct Rows {
 };
 
 constexpr int kTurnWarps = 4, kTurnCtas = 5;   // of turn_kernel: CTAs of an SM
+constexpr int kTurnPasses = 13;                // passes that a warp has at least, where there are more CTAs than places
 constexpr int kRingBytes = 4096;   // of a warp: Rows::kDepth * Rows::kSlot
 
 // Cosines and sines of a token's angles, by `all` threads of which this is number `me`.
@@ -954,7 +955,13 @@ int launch_rows_one(RowArgs& a, const Codebook& cb, cudaStream_t s) {
             if (units >= (1ll << 31) - 2 * warps) return TQB_ERR_TOO_LARGE;
             u.count = (int)units;
             u.by_token = Divisor((unsigned)u.per_token);
-            const int want = (u.count + kTurnWarps - 1) / kTurnWarps, grid = want < 148 * kTurnCtas ? want : 148 * kTurnCtas;
+            // A CTA for each place on the SMs, or several, as long as a warp keeps kTurnPasses passes: SMs get through their shares at
+            // different speeds, and who is done early takes another CTA.  (8,191 tokens of 40 heads, head_dim 256: 76.8 us, with one
+            // for each place 85.0; 16,384 of 128: 77.6 and 83.9.  But 4,096 of 128, 14 passes a warp: 22.9 us with two, 21.6 with one;
+            // 6,007 with one and a half 35.6, with one 33.0.)
+            const long long want = (u.count + kTurnWarps - 1) / kTurnWarps, times = (long long)a.tokens * passes / (warps * kTurnPasses);
+            const long long most = 148 * kTurnCtas * (times > 1 ? times : 1);
+            const int grid = (int)(want < most ? want : most);
             u.step = grid * kTurnWarps;
             turn_kernel<T, LPH><<<grid, 32 * kTurnWarps, dyn, s>>>(a, u);
             return check_launch(s);
