@@ -668,6 +668,12 @@ typedef struct tqb_paged_attention_params {
 } tqb_paged_attention_params;
 size_t tqb_paged_scratch_bytes(int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim);
 int tqb_paged_attention(const tqb_paged_layer *layer, const tqb_paged_attention_params *p, tqb_stream_t stream);
+/* The same where q and out have a row for each token of a step, [num_rows, num_q_heads, head_dim], as tqb_paged_append_rope
+ * leaves the queries: cu [num_requests + 1] is that of tqb_paged_plan, and the row of a request that brings one token is
+ * cu[r].  Requests that bring no token or several are left out, and so is a row outside [0, num_rows); rows of `out` that no
+ * request has stay as they are. */
+int tqb_paged_attention_rows(const tqb_paged_layer *layer, const tqb_paged_attention_params *p, const int32_t *cu,
+                             int32_t num_rows, tqb_stream_t stream);
 
 #ifdef __cplusplus
 }

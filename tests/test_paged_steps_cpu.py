@@ -1,0 +1,19 @@
+"""Refusals of the paged cache's entry points that are decided on the host, before any launch."""
+import ctypes
+
+import pytest
+
+from test_paged_cpu import A, layer
+from turboquant_b200._lib import TqbPagedAttentionParams, lib
+
+
+def attention(**kw):
+    d = dict(q=A, out=A, block_table=A, kv_lens=A, scratch=A, scratch_bytes=1 << 30, q_row_stride=0, table_stride=4, max_blocks=4,
+             num_requests=3, num_q_heads=8, q_dtype=2, out_dtype=2, softmax_scale=0.1)
+    return TqbPagedAttentionParams(**{**d, **kw})
+
+
+@pytest.mark.parametrize("cu,rows,change,status", [(None, 3, {}, 6), (A + 2, 3, {}, 8), (A, -1, {}, 7), (A, 0, {}, 0), (A, 3, dict(num_requests=0), 0),
+                                                   (A, 3, dict(num_requests=4097), 12), (A, 3, dict(q=None), 6), (A, 3, dict(num_q_heads=7), 3)])
+def test_rows_of_a_step(cu, rows, change, status):
+    assert lib.tqb_paged_attention_rows(ctypes.byref(layer()), ctypes.byref(attention(**change)), cu, rows, None) == status

@@ -163,6 +163,7 @@ def _declare(lib):
         "tqb_paged_dequantize": (c_int, [P, P, L, P, P, I, P]),
         "tqb_paged_scratch_bytes": (S, [I, I, I]),
         "tqb_paged_attention": (c_int, [P, P, P]),
+        "tqb_paged_attention_rows": (c_int, [P, P, P, I, P]),
         "tqb_kv_cache_create": (c_int, [P, I, U, P]),
         "tqb_kv_cache_destroy": (None, [P]),
         "tqb_kv_cache_push_batch": (c_int, [P, I, P, P, L, L, P]),

@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(kWorkThreads, F32Plan<NB, H, BITS>::kCtas) pag
         for (int h = 0; h < H; ++h)
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                const float q = h < s.heads ? load_as_f32(a.q, a.q_dtype, (size_t)s.req * a.q_stride + (size_t)(s.head0 + h) * D + b * 32 + lane) : 0.0f;
+                const float q = h < s.heads ? load_as_f32(a.q, a.q_dtype, (size_t)known_row(a, s.req) * a.q_stride + (size_t)(s.head0 + h) * D + b * 32 + lane) : 0.0f;
                 s_q[(b * 32 + lane) * H + h] = wht32_across(q, lane) * (1.0f / sqrtf((float)kBlock)) * block_sign(lane, a.sign_mag) * a.qk_const;
             }
         float o[H][NB], m[H], l[H];   // l: of the lane's tokens
@@ -237,20 +237,8 @@ int launch_f32_heads(const PagedArgs& a, cudaStream_t s) {
 
 size_t part_bytes(int head_dim) { return sizeof(float) * (size_t)kMaxCtas * 2 * kSegHeads * (2 + 2 + head_dim); }
 
-}  // namespace
-}  // namespace tqb
-
-using namespace tqb;
-
-extern "C" {
-
-size_t tqb_paged_scratch_bytes(int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim) {
-    if (num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0) return 0;
-    return TQB_PAGED_TICKET_BYTES + part_bytes(head_dim);
-}
-
-int tqb_paged_attention(const tqb_paged_layer* layer, const tqb_paged_attention_params* p, tqb_stream_t stream) {
-    TQB_NVTX_RANGE();
+// cu, rows: of tqb_paged_attention_rows, or nullptr.
+int attention(const tqb_paged_layer* layer, const tqb_paged_attention_params* p, const int32_t* cu, int rows, cudaStream_t s) {
     int st = check_paged_layer(layer);
     if (st != TQB_OK) return st;
     if (!p) return TQB_ERR_NULL_POINTER;
@@ -261,7 +249,7 @@ int tqb_paged_attention(const tqb_paged_layer* layer, const tqb_paged_attention_
     if (p->num_q_heads % layer->num_kv_heads != 0) return TQB_ERR_DIMENSION_MISMATCH;
     if (p->q_row_stride != 0 && p->q_row_stride < (int64_t)p->num_q_heads * layer->head_dim) return TQB_ERR_INVALID_ARGUMENT;
     if (p->num_requests > TQB_PAGED_MAX_REQUESTS) return TQB_ERR_TOO_LARGE;
-    if (p->num_requests == 0) return TQB_OK;
+    if (p->num_requests == 0 || (cu && rows == 0)) return TQB_OK;
     if (!p->q || !p->out || !p->kv_lens || !p->scratch || (!p->block_table && p->max_blocks > 0)) return TQB_ERR_NULL_POINTER;
     const int64_t elem = p->q_dtype == TQB_F32 ? 4 : 2;
     if ((uintptr_t)p->q % 16 != 0 || (p->q_row_stride * elem) % 16 != 0 || (uintptr_t)p->out % 16 != 0 || (uintptr_t)p->scratch % 16 != 0 ||
@@ -279,6 +267,8 @@ int tqb_paged_attention(const tqb_paged_layer* layer, const tqb_paged_attention_
     a.vs = layer->v_scales;
     a.table = p->block_table;
     a.lens = p->kv_lens;
+    a.cu = cu;
+    a.rows = rows;
     a.tickets = reinterpret_cast<unsigned*>(p->scratch);
     a.part_ml = reinterpret_cast<float*>(reinterpret_cast<char*>(p->scratch) + TQB_PAGED_TICKET_BYTES);
     a.round_ml = a.part_ml + (size_t)kMaxCtas * 2 * kSegHeads * 2;
@@ -304,7 +294,6 @@ int tqb_paged_attention(const tqb_paged_layer* layer, const tqb_paged_attention_
     a.qk_const = p->softmax_scale * 1.4426950408889634f;
     a.sign_mag = block_sign_magnitude();
     for (int i = 0; i < 16; ++i) a.cent[i] = cb.c[i];
-    cudaStream_t s = as_stream(stream);
     if (p->q_dtype != TQB_F32 && layer->num_pages > 0) return launch_paged_mma(a, layer->head_dim, layer->bits, s);
     switch (layer->head_dim * 10 + layer->bits) {
         case 643: return launch_f32_heads<2, 3>(a, s);
@@ -314,6 +303,32 @@ int tqb_paged_attention(const tqb_paged_layer* layer, const tqb_paged_attention_
         case 2563: return launch_f32_heads<8, 3>(a, s);
         default: return launch_f32_heads<8, 4>(a, s);
     }
+}
+
+}  // namespace
+}  // namespace tqb
+
+using namespace tqb;
+
+extern "C" {
+
+size_t tqb_paged_scratch_bytes(int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim) {
+    if (num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0) return 0;
+    return TQB_PAGED_TICKET_BYTES + part_bytes(head_dim);
+}
+
+int tqb_paged_attention(const tqb_paged_layer* layer, const tqb_paged_attention_params* p, tqb_stream_t stream) {
+    TQB_NVTX_RANGE();
+    return attention(layer, p, nullptr, 0, as_stream(stream));
+}
+
+int tqb_paged_attention_rows(const tqb_paged_layer* layer, const tqb_paged_attention_params* p, const int32_t* cu, int32_t num_rows,
+                             tqb_stream_t stream) {
+    TQB_NVTX_RANGE();
+    if (!cu) return TQB_ERR_NULL_POINTER;
+    if ((uintptr_t)cu % 4 != 0) return TQB_ERR_MISALIGNED;
+    if (num_rows < 0) return TQB_ERR_INVALID_ARGUMENT;
+    return attention(layer, p, cu, num_rows, as_stream(stream));
 }
 
 }  // extern "C"

@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG, BITS>::kCtas) paged
         bad_copy = false;
         fresh = true;
         // the queries ride along with the first group
-        const uint8_t* q = reinterpret_cast<const uint8_t*>(a.q) + ((size_t)x.req * a.q_stride + (size_t)x.head0 * D) * 2;
+        const uint8_t* q = reinterpret_cast<const uint8_t*>(a.q) + ((size_t)known_row(a, x.req) * a.q_stride + (size_t)x.head0 * D) * 2;
 #pragma unroll
         for (int i = 0; i < (L::kQueries / 16 + 31) / 32; ++i) {
             const int piece = 32 * i + lane;

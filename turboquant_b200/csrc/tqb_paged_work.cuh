@@ -41,12 +41,13 @@ struct PagedArgs {
     const uint16_t* vs;
     const int32_t* table;
     const int32_t* lens;
+    const int32_t* cu;   // [requests + 1] first token of each request in the step whose tokens are the rows of q and out, or nullptr: row r is request r
     unsigned* tickets;
     float* part_ml;      // [kMaxCtas][2][kSegHeads][2]: maximum (log2 units), sum
     float* round_ml;     // the same of joined parts, where two rounds are needed
     float* part_out;     // [kMaxCtas][2][kSegHeads][D], rotated domain
     long long q_stride, table_stride;
-    int requests, max_blocks, max_len, unit_shift, page_shift, num_pages, hkv, group, vheads, splits;   // vheads = hkv * splits
+    int requests, rows, max_blocks, max_len, unit_shift, page_shift, num_pages, hkv, group, vheads, splits;   // vheads = hkv * splits
     int q_dtype, out_dtype;
     float qk_const;      // softmax_scale * log2(e)
     float sign_mag;
@@ -57,6 +58,14 @@ struct PagedArgs {
 };
 
 int launch_paged_mma(const PagedArgs& a, int head_dim, int bits, cudaStream_t s);   // 16-bit queries, some page
+
+// The row of request r, or -1 where it has none: among the tokens of a step a request that brings exactly one has that one.
+__device__ __forceinline__ int row_of(const PagedArgs& a, int r) {
+    if (a.cu == nullptr) return r;
+    const int row = a.cu[r];
+    return (unsigned)a.cu[r + 1] - (unsigned)row == 1u && (unsigned)row < (unsigned)a.rows ? row : -1;
+}
+__device__ __forceinline__ int known_row(const PagedArgs& a, int r) { return a.cu == nullptr ? r : a.cu[r]; }   // of a request that has one
 
 struct Segment {
     int req, kvh, head0, heads;   // query heads head0 .. head0 + heads - 1 of the request
@@ -83,7 +92,7 @@ struct WorkLine {
     unsigned cur, end, base;         // base: where request `req` begins
     int req, len;
 
-    __device__ __forceinline__ int length(int r) const { return min(max(a.lens[r], 0), a.max_len); }
+    __device__ __forceinline__ int length(int r) const { return row_of(a, r) < 0 ? 0 : min(max(a.lens[r], 0), a.max_len); }
     __device__ __forceinline__ unsigned groups_of(int l) const { return ((unsigned)l + (kRunTokens << a.unit_shift) - 1) / kRunTokens >> a.unit_shift; }
     __device__ __forceinline__ unsigned units_of(int l) const { return l > 0 ? kOpenCost + groups_of(l) : 0u; }
     __device__ __forceinline__ int owner(unsigned x) const {   // the run that unit x belongs to
@@ -246,7 +255,7 @@ static __device__ __noinline__ void write_quad(void* out, int dtype, size_t i, b
 }
 template <int NB>
 __device__ __forceinline__ size_t quad_at(const PagedArgs& a, const Segment& s, int x) {   // element 4 x of the segment's heads
-    return ((size_t)s.req * a.hkv * a.group + s.head0) * (NB * 32) + 4 * x;
+    return ((size_t)known_row(a, s.req) * a.hkv * a.group + s.head0) * (NB * 32) + 4 * x;
 }
 
 // How many of a (request, head)'s parts are joined at a time: up to 24 at once, more of them in two rounds.  (A round is a
@@ -431,13 +440,15 @@ __device__ __forceinline__ void finish(const PagedArgs& a, const Fragments& f, F
     }
 }
 
-// Requests without tokens get zeros.
+// Requests without tokens get zeros; rows that no request has stay as they are.
 template <int NB>
 __device__ __forceinline__ void write_empty(const PagedArgs& a) {
     const int row = a.hkv * a.group * NB * 32;
     for (int r = blockIdx.x; r < a.requests; r += gridDim.x) {
         if (a.lens[r] > 0 && a.max_len > 0) continue;
-        for (int i = threadIdx.x; i < row; i += kWorkThreads) store_as(a.out, a.out_dtype, (size_t)r * row + i, 0.0f);
+        const int to = row_of(a, r);
+        if (to < 0) continue;
+        for (int i = threadIdx.x; i < row; i += kWorkThreads) store_as(a.out, a.out_dtype, (size_t)to * row + i, 0.0f);
     }
 }
 

@@ -310,9 +310,12 @@ class PagedLayer:
         scratch[:_TICKET_BYTES].zero_()
         return scratch
 
-    def attend(self, q, block_table, kv_lens, softmax_scale, out=None, scratch=None):
+    def attend(self, q, block_table, kv_lens, softmax_scale, out=None, scratch=None, cu=None):
         """Attention of one new token of each request over its pages: q [requests, query heads, dim] -> the same shape.
-        block_table [requests, blocks] and kv_lens [requests] int32; a request without tokens gets zeros."""
+        block_table [requests, blocks] and kv_lens [requests] int32; a request without tokens gets zeros.
+
+        With cu [requests + 1] (a PagedStep's) the rows of q and out are the step's tokens: row cu[r] is that of request r, if
+        it brings exactly one token.  Other rows of a given `out` stay as they are; of one made here they are zeros."""
         index, d = self.index, self.head_dim
         n, hq, _ = _three("q", q)
         qi, at, s0, s1 = _rows("q", q, (n, hq, d), index)
@@ -321,19 +324,22 @@ class PagedLayer:
             at, s0 = qi.data_ptr(), hq * d
         if block_table.dim() != 2:
             raise DimensionMismatch(f"block_table: expected [requests, blocks], got {tuple(block_table.shape)}")
-        blocks = block_table.shape[1]
-        table = _want("block_table", block_table, torch.int32, (n, blocks), index)
-        lens = _want("kv_lens", kv_lens, torch.int32, (n,), index)
+        requests, blocks = n if cu is None else block_table.shape[0], block_table.shape[1]
+        table = _want("block_table", block_table, torch.int32, (requests, blocks), index)
+        lens = _want("kv_lens", kv_lens, torch.int32, (requests,), index)
         if out is None:
-            out = _empty_like(q, n, hq, d)
+            out = _empty_like(q, n, hq, d) if cu is None else q.new_zeros((n, hq, d))
             to = out.data_ptr()
         else:
             to = _want("out", out, out.dtype, (n, hq, d), index)
         if scratch is None:
             scratch = self.attend_scratch(hq)
         work = _want("scratch", scratch, torch.uint8, scratch.shape, index)
-        _call(index, lib.tqb_paged_attention, self._c, _ATTEND.pack(at, to, table, lens, work, scratch.numel(), s0 if n > 1 else 0, blocks, blocks,
-                                                                    n, hq, _code(q.dtype), _code(out.dtype), softmax_scale))
+        p = _ATTEND.pack(at, to, table, lens, work, scratch.numel(), s0 if n > 1 else 0, blocks, blocks, requests, hq, _code(q.dtype), _code(out.dtype), softmax_scale)
+        if cu is None:
+            _call(index, lib.tqb_paged_attention, self._c, p)
+        elif n:
+            _call(index, lib.tqb_paged_attention_rows, self._c, p, _want("cu", cu, torch.int32, (requests + 1,), index), n)
         return out
 
 
@@ -343,7 +349,7 @@ class PagedPqoCache:
 
         step = cache.plan(new_tokens, capacity)                # once a step
         q = cache.append_rope(layer, rope, q, k, v, step)      # each layer
-        out = cache.decode(layer, q, step, att).fused          # steps of one token a request
+        out = cache.decode_tokens(layer, q, step, att).fused   # of the requests that bring one token
     """
 
     def __init__(self, config, num_pages, page_size=64, max_requests=64, max_blocks=None, device=None):
@@ -389,15 +395,25 @@ class PagedPqoCache:
         return self._layer(layer).dequantize(slots, dtype)
 
     def decode(self, layer, q, step, config, out=None, scratch=None):
-        """Attention of q [max_requests, query heads, dim] over everything stored: DecodeOutput with `fused` set.
+        """Attention of q [max_requests, query heads, dim] over everything stored, row r being request r's: DecodeOutput with
+        `fused` set.  (The rows that append_rope returns are the step's tokens, which is something else as soon as a request
+        is idle: they go to decode_tokens.)
         Without `scratch` the cache keeps one for each stream, and a call that is being captured gets its own."""
+        return self._decode(layer, q, step, config, out, scratch, None)
+
+    def decode_tokens(self, layer, q, step, config, out=None, scratch=None):
+        """The same for the step's tokens: q [tokens, query heads, dim] as append_rope returns it, padding behind the last
+        token included.  Rows of requests that bring one token are computed; of other rows see PagedLayer.attend."""
+        return self._decode(layer, q, step, config, out, scratch, step.cu)
+
+    def _decode(self, layer, q, step, config, out, scratch, cu):
         at = self._layer(layer)
         if scratch is None and not torch.cuda.is_current_stream_capturing():
             stream = torch.cuda.current_stream(self.device).cuda_stream
             scratch = self._scratch.get(stream)
             if scratch is None:
                 scratch = self._scratch[stream] = at.attend_scratch(q.shape[1])
-        return DecodeOutput(fused=at.attend(q, self.block_table, step.kv_lens, config.softmax_scale, out=out, scratch=scratch))
+        return DecodeOutput(fused=at.attend(q, self.block_table, step.kv_lens, config.softmax_scale, out=out, scratch=scratch, cu=cu))
 
     def _layer(self, layer):
         if not 0 <= layer < len(self.layers):
