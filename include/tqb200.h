@@ -591,7 +591,10 @@ int tqb_paged_plan(const int32_t *seq_lens, const int32_t *new_tokens, int32_t n
                    int64_t *slots, int32_t *positions, int32_t capacity, int32_t *cu, int32_t *kv_lens,
                    int32_t *state_out, tqb_stream_t stream);
 /* Gives the pages of the requests with mask[r] != 0 back: appended to free_pages (room for free_capacity entries) in the
- * order of requests and blocks; their seq_lens become 0 and their table entries -1. */
+ * order of requests and blocks; their seq_lens become 0 and their table entries -1.  Requests may share whole pages (a common
+ * beginning that the caller has entered in several rows of the table): a page that a request which goes on holds in the
+ * entries of its length is not given back, and one that several ended requests hold is given back once.  Entries below 0
+ * are no pages. */
 int tqb_paged_release(const uint8_t *mask, int32_t *seq_lens, int32_t num_requests, int32_t *block_table,
                       int64_t table_stride, int32_t max_blocks, int32_t *free_pages, int32_t free_capacity, int32_t *state,
                       int32_t page_size, tqb_stream_t stream);

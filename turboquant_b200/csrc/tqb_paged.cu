@@ -150,48 +150,176 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanArgs a) {
     }
 }
 
-// The pages of finished requests back onto the list, by one CTA: a release is rare and short.
+// The pages of finished requests back onto the list, by one CTA: a release is rare and short.  A page that a request that stays
+// holds too stays with it, and one that several ended requests hold goes back once, for the first of its entries.  Who holds what
+// is told by a bit for each page of a range of 2^20, marked by the requests that stay and then by the entries in their order;
+// ranges without a page to give back are passed over.  64 requests of 128 pages, one of which ends: 19 us between two events (9 for
+// a kernel that gives back whatever it finds), all of which end 27 us (13); an entry a thread and round instead of four 39 us.
 constexpr int kReleaseThreads = 1024;
+constexpr int kMarked = 1 << 20;   // pages of a range: 128 KB of bits
+constexpr int kEach = 4, kChunk = kEach * kReleaseThreads;   // entries of a thread, and of a round
+constexpr int kReleaseBytes = kMarked / 8 + kChunk * 4;
 
-__global__ void __launch_bounds__(kReleaseThreads) release_kernel(const uint8_t* mask, int32_t* seq, int requests, int32_t* table,
-                                                                  long long table_stride, int max_blocks, int32_t* free_pages,
-                                                                  int free_capacity, int32_t* state, int sh) {
-    __shared__ int s_start[TQB_PAGED_MAX_REQUESTS + 1];
-    const int tid = threadIdx.x;
-    const long long limit = min((long long)max_blocks << sh, 0x7fffffffll), avail = max(state[0], 0);
-    const int per = (requests + kReleaseThreads - 1) / kReleaseThreads, r0 = min(tid * per, requests), r1 = min(r0 + per, requests);
-    long long np = 0, unused = 0, pages, unused_total;
+struct ReleaseArgs {
+    const uint8_t* mask;
+    int32_t* seq;
+    int32_t* table;
+    long long table_stride;
+    int32_t* free_pages;
+    int32_t* state;
+    int requests, max_blocks, free_capacity, page_shift;
+};
+
+__global__ void __launch_bounds__(kReleaseThreads) release_kernel(ReleaseArgs a) {
+    extern __shared__ uint32_t s_mark[];   // [bits][the round's entries]
+    int* const s_entry = reinterpret_cast<int*>(s_mark + kMarked / 32);
+    __shared__ int s_start[2][TQB_PAGED_MAX_REQUESTS + 1];   // first entry of each request: of those that end, of those that stay
+    __shared__ int s_high;
+    __shared__ unsigned s_low;
+    const int tid = threadIdx.x, R = a.requests, sh = a.page_shift;
+    const long long limit = min((long long)a.max_blocks << sh, 0x7fffffffll), avail = max(a.state[0], 0);
+    const int per = (R + kReleaseThreads - 1) / kReleaseThreads, r0 = min(tid * per, R), r1 = min(r0 + per, R);
+    auto held = [&](int r) { return pages_of(min(max((long long)a.seq[r], 0ll), limit), sh); };
+    long long going = 0, staying = 0, entries, others;
     int bad = 0;
     for (int r = r0; r < r1; ++r) {
-        if (!mask[r]) continue;
-        if (seq[r] < 0 || seq[r] > limit) bad = 1;
-        else np += pages_of(seq[r], sh);
+        (a.mask[r] ? going : staying) += held(r);
+        if (a.mask[r] && (a.seq[r] < 0 || a.seq[r] > limit)) bad = 1;
     }
     bad = __syncthreads_or(bad);
-    block_scan2<kReleaseThreads>(np, unused, pages, unused_total);
-    const int status = bad ? TQB_PLAN_BAD_LENGTH : avail + pages > free_capacity ? TQB_PLAN_OUT_OF_PAGES : TQB_PLAN_OK;
+    block_scan2<kReleaseThreads>(going, staying, entries, others);
+    int status = bad || entries > kMostCounted || others > kMostCounted ? TQB_PLAN_BAD_LENGTH : TQB_PLAN_OK;
     if (status != TQB_PLAN_OK) {
-        if (tid == 0) state[2] = status;
+        if (tid == 0) a.state[2] = status;
         return;
     }
     for (int r = r0; r < r1; ++r) {
-        s_start[r] = (int)np;
-        if (mask[r]) np += pages_of(seq[r], sh);
+        s_start[0][r] = (int)going;
+        s_start[1][r] = (int)staying;
+        (a.mask[r] ? going : staying) += held(r);
     }
-    if (tid == 0) s_start[requests] = (int)pages;
-    __syncthreads();
-    for (int i = tid; i < (int)pages; i += kReleaseThreads) {
-        const int r = last_not_above(s_start, requests, i);
-        int32_t* e = table + r * table_stride + (i - s_start[r]);
-        free_pages[avail + i] = *e;
-        *e = -1;
-    }
-    __syncthreads();
-    for (int r = r0; r < r1; ++r)
-        if (mask[r]) seq[r] = 0;
     if (tid == 0) {
-        state[0] = (int)(avail + pages);
-        state[2] = TQB_PLAN_OK;
+        s_start[0][R] = (int)entries;
+        s_start[1][R] = (int)others;
+        s_low = ~0u;
+        s_high = -1;
+    }
+    __syncthreads();
+    // kEach entries from i on, of those that end (0) or stay (1); -1 behind the last one and where there is no page
+    auto entries_at = [&](int side, int i, int (&page)[kEach], int32_t* (&at)[kEach]) {
+        const int n = side == 0 ? (int)entries : (int)others;
+        const int* start = s_start[side];
+        int r = i < n ? last_not_above(start, R, i) : 0;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            at[k] = nullptr;
+            if (i + k >= n) continue;
+            while (start[r + 1] <= i + k) ++r;
+            at[k] = a.table + r * a.table_stride + (i + k - start[r]);
+        }
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) page[k] = at[k] != nullptr ? max(*at[k], -1) : -1;
+    };
+    int page[kEach], pages = 0, high = -1;
+    int32_t* at[kEach];
+    unsigned low = ~0u;
+    for (int i = tid * kEach; i < (int)entries; i += kChunk) {
+        entries_at(0, i, page, at);
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            pages += page[k] >= 0;
+            low = min(low, (unsigned)page[k]);   // (-1 is the largest)
+            high = max(high, page[k]);
+        }
+    }
+    atomicMin(&s_low, low);
+    atomicMax(&s_high, high);
+    auto sum = [&](int x) {
+        long long v = x, none = 0, total, unused;
+        __syncthreads();
+        block_scan2<kReleaseThreads>(v, none, total, unused);
+        return total;
+    };
+    const bool roomy = avail + sum(pages) <= a.free_capacity;
+    const unsigned first = s_low;
+    const int last = s_high;
+    __syncthreads();
+    // Entries whose page is not to be given back are turned over (~page), if need be after they have been counted.
+    for (int pass = roomy ? 1 : 0; pass < 2; ++pass) {
+        int back = 0;   // pages that are given back
+        for (long long from = first; from <= last;) {
+            const int words = (int)((min((long long)kMarked, last - from + 1) + 31) / 32);
+            auto bit_of = [&](int x) { return x >= from && x <= last && x - from < kMarked ? (int)(x - from) : -1; };
+            for (int i = tid; i < words; i += kReleaseThreads) s_mark[i] = 0;
+            if (tid == 0) s_low = ~0u;
+            __syncthreads();
+            for (int i = tid * kEach; i < (int)others; i += kChunk) {
+                entries_at(1, i, page, at);
+#pragma unroll
+                for (int k = 0; k < kEach; ++k) {
+                    const int b = bit_of(page[k]);
+                    if (b >= 0) atomicOr(&s_mark[b >> 5], 1u << (b & 31));
+                }
+            }
+            __syncthreads();
+            unsigned next = ~0u;
+            for (int base = 0; base < (int)entries; base += kChunk) {
+                entries_at(0, base + tid * kEach, page, at);
+                int b[kEach];
+                unsigned taken = 0, twice = 0;   // a bit for each k
+#pragma unroll
+                for (int k = 0; k < kEach; ++k) {
+                    b[k] = bit_of(page[k]);
+                    if (page[k] - from >= kMarked) next = min(next, (unsigned)page[k]);
+                    if (b[k] >= 0) taken |= ((s_mark[b[k] >> 5] >> (b[k] & 31)) & 1u) << k;
+                    s_entry[tid * kEach + k] = b[k];
+                }
+                __syncthreads();
+#pragma unroll
+                for (int k = 0; k < kEach; ++k)
+                    if (b[k] >= 0 && !((taken >> k) & 1u)) twice |= (atomicOr(&s_mark[b[k] >> 5], 1u << (b[k] & 31)) >> (b[k] & 31)) & 1u;
+                if (__syncthreads_or(twice))
+#pragma unroll
+                    for (int k = 0; k < kEach; ++k)   // the first of equal ones has the page
+                        for (int i = 0; i < tid * kEach + k && b[k] >= 0 && !((taken >> k) & 1u); ++i) taken |= (s_entry[i] == b[k] ? 1u : 0u) << k;
+#pragma unroll
+                for (int k = 0; k < kEach; ++k) {
+                    back += b[k] >= 0 && !((taken >> k) & 1u);
+                    if (((taken >> k) & 1u) && pass == 1) *at[k] = ~page[k];
+                }
+                __syncthreads();
+            }
+            atomicMin(&s_low, next);
+            __syncthreads();
+            from = s_low;   // (without another page: behind the last one)
+            __syncthreads();
+        }
+        if (pass == 0 && avail + sum(back) > a.free_capacity) {
+            if (tid == 0) a.state[2] = TQB_PLAN_OUT_OF_PAGES;
+            return;
+        }
+    }
+    __syncthreads();
+    long long to = avail;
+    for (int base = 0; base < (int)entries; base += kChunk) {
+        entries_at(0, base + tid * kEach, page, at);
+        long long here = 0, none = 0, total, unused;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) here += page[k] >= 0;
+        block_scan2<kReleaseThreads>(here, none, total, unused);
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            if (page[k] >= 0) a.free_pages[to + here++] = page[k];
+            if (at[k] != nullptr) *at[k] = -1;
+        }
+        to += total;
+        __syncthreads();
+    }
+    for (int r = r0; r < r1; ++r)
+        if (a.mask[r]) a.seq[r] = 0;
+    if (tid == 0) {
+        a.state[0] = (int)to;
+        a.state[2] = TQB_PLAN_OK;
     }
 }
 
@@ -1113,8 +1241,9 @@ int tqb_paged_release(const uint8_t* mask, int32_t* seq_lens, int32_t num_reques
     if (free_capacity < 0) return TQB_ERR_INVALID_ARGUMENT;
     if (!state) return TQB_ERR_NULL_POINTER;
     if (num_requests > 0 && (!mask || !seq_lens || (max_blocks > 0 && (!block_table || !free_pages)))) return TQB_ERR_NULL_POINTER;
-    release_kernel<<<1, kReleaseThreads, 0, as_stream(stream)>>>(mask, seq_lens, num_requests, block_table, table_stride, max_blocks,
-                                                                free_pages, free_capacity, state, log2_of(page_size));
+    if ((st = allow_shared<release_kernel>(kReleaseBytes)) != TQB_OK) return st;
+    const ReleaseArgs a{mask, seq_lens, block_table, table_stride, free_pages, state, num_requests, max_blocks, free_capacity, log2_of(page_size)};
+    release_kernel<<<1, kReleaseThreads, kReleaseBytes, as_stream(stream)>>>(a);
     return check_launch(as_stream(stream));
 }
 

@@ -176,7 +176,8 @@ def paged_plan(seq_lens, new_tokens, block_table, free_pages, state, page_size, 
 
 
 def paged_release(mask, seq_lens, block_table, free_pages, state, page_size):
-    """Gives the pages of the requests with mask[r] back to free_pages (tqb_paged_release): in place."""
+    """Gives the pages of the requests with mask[r] back to free_pages (tqb_paged_release): in place.  A page that requests
+    share goes back once, when the last of them ends."""
     index, n, blocks, seq, table, free, st = _plan_args(seq_lens, block_table, free_pages, state)
     if mask.dtype is torch.bool:
         mask = mask.view(torch.uint8)
@@ -381,7 +382,8 @@ class PagedPqoCache:
                           kv_lens=self.seq_lens, state_out=self.state)
 
     def release(self, mask):
-        """Ends the requests with mask[r] (bool or u8 [max_requests]); their rows may be used by new ones."""
+        """Ends the requests with mask[r] (bool or u8 [max_requests]); their rows may be used by new ones.  Pages that others
+        hold too stay theirs."""
         paged_release(mask, self.seq_lens, self.block_table, self.free_pages, self.state, self.page_size)
 
     def append(self, layer, k, v, step):
