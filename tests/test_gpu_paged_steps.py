@@ -133,3 +133,21 @@ def test_rows_that_do_not_fit_are_refused():
                  lambda: layer.attend(q, table, lens, 0.1, out=q[:3], cu=cu)):
         with pytest.raises(wrong):
             call()
+
+
+@pytest.mark.parametrize("count,status", [(3, 0), (4, 1), (2 ** 31 - 1, 1)])
+@pytest.mark.parametrize("capacity", [40, 5000])
+def test_plan_of_a_count_beyond_its_list(count, status, capacity):
+    """A wrong number of free pages: no page is taken from behind the list, and a step that needs none goes on."""
+    i32 = dict(dtype=torch.int32, device="cuda")
+    seq, table, free = torch.tensor([16, 5], **i32), torch.tensor([[7, -1, -1], [9, -1, -1]], **i32), torch.tensor([0, 1, 2], **i32)
+    state = torch.tensor([count, 0, 0, 0], **i32)
+    step = tq.paged_plan(seq, torch.tensor([20, 3], **i32), table, free, state, 16, capacity)
+    if status:
+        assert step.state.tolist() == [count, 0, 1, 0] and table.tolist() == [[7, -1, -1], [9, -1, -1]] and step.kv_lens.tolist() == [16, 5]
+        assert step.slots.tolist() == [-1] * capacity and step.cu.tolist() == [0, 0, 0]
+    else:
+        assert step.state.tolist() == [1, 0, 0, 0] and table.tolist() == [[7, 2, 1], [9, -1, -1]]
+    table = torch.tensor([[7, -1, -1], [9, -1, -1]], **i32)
+    step = tq.paged_plan(seq, torch.tensor([0, 3], **i32), table, free, state, 16, capacity)
+    assert step.state.tolist() == [count, 0, 0, 0] and step.slots[:3].tolist() == [149, 150, 151]

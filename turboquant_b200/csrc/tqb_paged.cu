@@ -31,7 +31,7 @@ struct PlanArgs {
     int32_t* cu;
     int32_t* kv_lens;
     int32_t* state_out;
-    int requests, max_blocks, page_shift, capacity;
+    int requests, max_blocks, page_shift, capacity, free_capacity;
 };
 
 __device__ __forceinline__ long long pages_of(long long tokens, int shift) { return (tokens + (1ll << shift) - 1) >> shift; }
@@ -93,7 +93,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanArgs a) {
     bad = __syncthreads_or(bad);
     long long tokens, pages;
     block_scan2<kPlanThreads>(nt, np, tokens, pages);
-    const int status = bad ? TQB_PLAN_BAD_LENGTH : tokens > a.capacity ? TQB_PLAN_OVER_CAPACITY : pages > avail ? TQB_PLAN_OUT_OF_PAGES : TQB_PLAN_OK;
+    const int status = bad ? TQB_PLAN_BAD_LENGTH : tokens > a.capacity ? TQB_PLAN_OVER_CAPACITY
+                       : pages > (avail > a.free_capacity ? 0 : avail) ? TQB_PLAN_OUT_OF_PAGES : TQB_PLAN_OK;   // (no list is longer than its room)
     if (status != TQB_PLAN_OK) tokens = pages = 0;   // nothing is planned
     for (int r = r0; r < r1; ++r) {
         s_cu[r] = status == TQB_PLAN_OK ? (int)nt : 0;
@@ -1189,6 +1190,24 @@ int check_plan_shape(int32_t num_requests, int64_t table_stride, int32_t max_blo
     return TQB_OK;
 }
 
+int plan(const int32_t* seq_lens, const int32_t* new_tokens, int32_t num_requests, int32_t* block_table, int64_t table_stride,
+         int32_t max_blocks, const int32_t* free_pages, int32_t free_capacity, int32_t* state, int32_t page_size, int64_t* slots,
+         int32_t* positions, int32_t capacity, int32_t* cu, int32_t* kv_lens, int32_t* state_out, tqb_stream_t stream) {
+    int st = check_plan_shape(num_requests, table_stride, max_blocks, page_size);
+    if (st != TQB_OK) return st;
+    if (capacity < 0 || free_capacity < 0) return TQB_ERR_INVALID_ARGUMENT;
+    if (capacity > kMostCounted) return TQB_ERR_TOO_LARGE;
+    if (!state || !state_out || !cu) return TQB_ERR_NULL_POINTER;
+    if (num_requests > 0 && (!seq_lens || !new_tokens || !kv_lens || (max_blocks > 0 && (!block_table || !free_pages)))) return TQB_ERR_NULL_POINTER;
+    if (capacity > 0 && (!slots || !positions)) return TQB_ERR_NULL_POINTER;
+    PlanArgs a{seq_lens, new_tokens, block_table, table_stride, free_pages, state, slots, positions, cu, kv_lens, state_out,
+               num_requests, max_blocks, log2_of(page_size), capacity, free_capacity};
+    int grid = (capacity + kPlanTokens - 1) / kPlanTokens;
+    grid = grid < 1 ? 1 : grid > 148 ? 148 : grid;
+    plan_kernel<<<grid, kPlanThreads, 0, as_stream(stream)>>>(a);
+    return check_launch(as_stream(stream));
+}
+
 }  // namespace
 
 int check_paged_layer(const tqb_paged_layer* l) {
@@ -1217,19 +1236,17 @@ int tqb_paged_plan(const int32_t* seq_lens, const int32_t* new_tokens, int32_t n
                    int64_t* slots, int32_t* positions, int32_t capacity, int32_t* cu, int32_t* kv_lens, int32_t* state_out,
                    tqb_stream_t stream) {
     TQB_NVTX_RANGE();
-    int st = check_plan_shape(num_requests, table_stride, max_blocks, page_size);
-    if (st != TQB_OK) return st;
-    if (capacity < 0) return TQB_ERR_INVALID_ARGUMENT;
-    if (capacity > kMostCounted) return TQB_ERR_TOO_LARGE;
-    if (!state || !state_out || !cu) return TQB_ERR_NULL_POINTER;
-    if (num_requests > 0 && (!seq_lens || !new_tokens || !kv_lens || (max_blocks > 0 && (!block_table || !free_pages)))) return TQB_ERR_NULL_POINTER;
-    if (capacity > 0 && (!slots || !positions)) return TQB_ERR_NULL_POINTER;
-    PlanArgs a{seq_lens, new_tokens, block_table, table_stride, free_pages, state, slots, positions, cu, kv_lens, state_out,
-               num_requests, max_blocks, log2_of(page_size), capacity};
-    int grid = (capacity + kPlanTokens - 1) / kPlanTokens;
-    grid = grid < 1 ? 1 : grid > 148 ? 148 : grid;
-    plan_kernel<<<grid, kPlanThreads, 0, as_stream(stream)>>>(a);
-    return check_launch(as_stream(stream));
+    return plan(seq_lens, new_tokens, num_requests, block_table, table_stride, max_blocks, free_pages, 0x7fffffff, state, page_size, slots,
+                positions, capacity, cu, kv_lens, state_out, stream);
+}
+
+int tqb_paged_plan_bounded(const int32_t* seq_lens, const int32_t* new_tokens, int32_t num_requests, int32_t* block_table,
+                           int64_t table_stride, int32_t max_blocks, const int32_t* free_pages, int32_t free_capacity,
+                           int32_t* state, int32_t page_size, int64_t* slots, int32_t* positions, int32_t capacity, int32_t* cu,
+                           int32_t* kv_lens, int32_t* state_out, tqb_stream_t stream) {
+    TQB_NVTX_RANGE();
+    return plan(seq_lens, new_tokens, num_requests, block_table, table_stride, max_blocks, free_pages, free_capacity, state, page_size,
+                slots, positions, capacity, cu, kv_lens, state_out, stream);
 }
 
 int tqb_paged_release(const uint8_t* mask, int32_t* seq_lens, int32_t num_requests, int32_t* block_table, int64_t table_stride,

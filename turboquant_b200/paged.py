@@ -143,11 +143,12 @@ def _plan_args(seq_lens, block_table, free_pages, state):
 
 
 def paged_plan(seq_lens, new_tokens, block_table, free_pages, state, page_size, capacity, kv_lens=None, state_out=None):
-    """Block tables, slot map and positions of a step from the requests' lengths (tqb_paged_plan).
+    """Block tables, slot map and positions of a step from the requests' lengths (tqb_paged_plan_bounded).
 
     seq_lens, new_tokens [requests], block_table [requests, blocks] (new entries are written in place), free_pages and
     state int32; the first state[0] entries of free_pages are the free pages.  kv_lens and state_out are made new unless
-    given; they may be seq_lens and state themselves.  Returns a PagedStep; `check()` on it says whether the step fitted."""
+    given; they may be seq_lens and state themselves.  Returns a PagedStep; `check()` on it says whether the step fitted (with
+    state[0] beyond the list's length no page is to be had)."""
     index, n, blocks, seq, table, free, st = _plan_args(seq_lens, block_table, free_pages, state)
     new = _want("new_tokens", new_tokens, torch.int32, (n,), index)
     if capacity < 0:
@@ -170,8 +171,8 @@ def paged_plan(seq_lens, new_tokens, block_table, free_pages, state, page_size, 
         state_out = parts.pop()
     if kv_lens is None:
         kv_lens = parts.pop()
-    _call(index, lib.tqb_paged_plan, seq, new, n, table, blocks, blocks, free, st, page_size, slots.data_ptr(), positions.data_ptr(),
-          capacity, cu.data_ptr(), kv_lens.data_ptr(), state_out.data_ptr())
+    _call(index, lib.tqb_paged_plan_bounded, seq, new, n, table, blocks, blocks, free, free_pages.shape[0], st, page_size, slots.data_ptr(),
+          positions.data_ptr(), capacity, cu.data_ptr(), kv_lens.data_ptr(), state_out.data_ptr())
     return PagedStep(slots, positions, cu, kv_lens, state_out)
 
 
