@@ -591,11 +591,14 @@ int tqb_paged_plan(const int32_t *seq_lens, const int32_t *new_tokens, int32_t n
                    int64_t *slots, int32_t *positions, int32_t capacity, int32_t *cu, int32_t *kv_lens,
                    int32_t *state_out, tqb_stream_t stream);
 /* The same with the number of entries that free_pages has room for: where state[0] is beyond it, no page is to be had
- * (TQB_PLAN_OUT_OF_PAGES for a step that needs one), and nothing behind the list is read.  tqb_paged_plan relies on state[0]. */
+ * (TQB_PLAN_OUT_OF_PAGES for a step that needs one), and nothing behind the list is read.  tqb_paged_plan relies on state[0].
+ * state[2] is that of the last call only.  `failed` (a word of the caller's, or NULL) gets every status that is not
+ * TQB_PLAN_OK, this plan's or the one found in state[2], and is left alone otherwise: a program that replays captured steps
+ * reads it now and then, and sets it and state[2] to 0 again. */
 int tqb_paged_plan_bounded(const int32_t *seq_lens, const int32_t *new_tokens, int32_t num_requests, int32_t *block_table,
                            int64_t table_stride, int32_t max_blocks, const int32_t *free_pages, int32_t free_capacity,
                            int32_t *state, int32_t page_size, int64_t *slots, int32_t *positions, int32_t capacity,
-                           int32_t *cu, int32_t *kv_lens, int32_t *state_out, tqb_stream_t stream);
+                           int32_t *cu, int32_t *kv_lens, int32_t *state_out, int32_t *failed, tqb_stream_t stream);
 /* Gives the pages of the requests with mask[r] != 0 back: appended to free_pages (room for free_capacity entries) in the
  * order of requests and blocks; their seq_lens become 0 and their table entries -1.  Requests may share whole pages (a common
  * beginning that the caller has entered in several rows of the table): a page that a request which goes on holds in the

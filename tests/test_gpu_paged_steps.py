@@ -151,3 +151,39 @@ def test_plan_of_a_count_beyond_its_list(count, status, capacity):
     table = torch.tensor([[7, -1, -1], [9, -1, -1]], **i32)
     step = tq.paged_plan(seq, torch.tensor([0, 3], **i32), table, free, state, 16, capacity)
     assert step.state.tolist() == [count, 0, 0, 0] and step.slots[:3].tolist() == [149, 150, 151]
+
+
+def test_a_step_that_did_not_fit_is_told_after_later_ones():
+    """Also where a captured plan is replayed on and on, and where a release in between was refused."""
+    cache = tq.PagedPqoCache(tq.CacheConfig(4, 64, 1, 1), 4, 16, 2)
+    new = torch.zeros(2, dtype=torch.int32, device="cuda")
+    cache.plan(new, 70)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.plan(new, 70)
+    for some, status in (([20, 20], 0), ([40, 1], 1), ([1, 0], 0), ([60, 11], 2), ([3, 3], 0)):   # (81 tokens are more than the table's 64)
+        new.copy_(torch.tensor(some, dtype=torch.int32))
+        graph.replay()
+        assert int(cache.state[2]) == status
+    assert cache.seq_lens.tolist() == [24, 23]
+    with pytest.raises(tq.TqbRuntimeError) as e:
+        cache.check()
+    assert e.value.status == 2
+    cache.check()
+    graph.replay()
+    cache.check()
+    cache.seq_lens[1] = -1
+    cache.release(torch.tensor([False, True], device="cuda"))   # refused: the length is negative
+    cache.seq_lens[1] = 26
+    graph.replay()
+    assert int(cache.state[2]) == 0
+    with pytest.raises(tq.TqbRuntimeError) as e:
+        cache.check()
+    assert e.value.status == 2
+    cache.seq_lens[1] = -1
+    cache.release(torch.tensor([False, True], device="cuda"))
+    with pytest.raises(tq.TqbRuntimeError):
+        cache.check()
+    cache.check()
+    with pytest.raises(tq.DimensionMismatch):
+        tq.paged_plan(cache.seq_lens, new, cache.block_table, cache.free_pages, cache.state, 16, 4, failed=new)

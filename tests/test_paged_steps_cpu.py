@@ -22,6 +22,6 @@ def test_rows_of_a_step(cu, rows, change, status):
 @pytest.mark.parametrize("at,value,status", [(2, -1, 7), (2, 4097, 12), (4, 3, 7), (7, -1, 7), (9, 24, 7), (12, -1, 7), (12, (1 << 30) + 1, 12), (6, None, 6),
                                              (8, None, 6), (10, None, 6), (13, None, 6), (14, None, 6), (15, None, 6)])
 def test_plan_of_a_list_of_known_length(at, value, status):
-    args = [A, A, 3, A, 4, 4, A, 9, A, 16, A, A, 5, A, A, A, None]
+    args = [A, A, 3, A, 4, 4, A, 9, A, 16, A, A, 5, A, A, A, None, None]
     args[at] = value
     assert lib.tqb_paged_plan_bounded(*args) == status

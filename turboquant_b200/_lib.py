@@ -156,7 +156,7 @@ def _declare(lib):
         "tqb_tq_cache_memory_usage": (S, [P]),
         "tqb_tq_cache_qjl_ptrs": (c_int, [P, I, P, P, P]),
         "tqb_paged_plan": (c_int, [P, P, I, P, L, I, P, P, I, P, P, I, P, P, P, P]),
-        "tqb_paged_plan_bounded": (c_int, [P, P, I, P, L, I, P, I, P, I, P, P, I, P, P, P, P]),
+        "tqb_paged_plan_bounded": (c_int, [P, P, I, P, L, I, P, I, P, I, P, P, I, P, P, P, P, P]),
         "tqb_paged_release": (c_int, [P, P, I, P, L, I, P, I, P, I, P]),
         "tqb_qk_norm_rope": (c_int, [P, P]),
         "tqb_paged_append": (c_int, [P, P, L, L, P, L, L, I, P, I, P]),

@@ -31,6 +31,7 @@ struct PlanArgs {
     int32_t* cu;
     int32_t* kv_lens;
     int32_t* state_out;
+    int32_t* failed;   // or nullptr
     int requests, max_blocks, page_shift, capacity, free_capacity;
 };
 
@@ -143,6 +144,10 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanArgs a) {
     }
     for (int r = tid; r < R; r += kPlanThreads) a.kv_lens[r] = status == TQB_PLAN_OK ? a.seq[r] + a.fresh[r] : a.seq[r];
     if (tid == 0) {
+        if (a.failed != nullptr) {
+            const int was = status != TQB_PLAN_OK ? status : a.state[2];
+            if (was != TQB_PLAN_OK) *a.failed = was;
+        }
         a.state[1] = 0;
         a.state_out[0] = (int)(avail - pages);
         a.state_out[1] = 0;
@@ -1192,7 +1197,7 @@ int check_plan_shape(int32_t num_requests, int64_t table_stride, int32_t max_blo
 
 int plan(const int32_t* seq_lens, const int32_t* new_tokens, int32_t num_requests, int32_t* block_table, int64_t table_stride,
          int32_t max_blocks, const int32_t* free_pages, int32_t free_capacity, int32_t* state, int32_t page_size, int64_t* slots,
-         int32_t* positions, int32_t capacity, int32_t* cu, int32_t* kv_lens, int32_t* state_out, tqb_stream_t stream) {
+         int32_t* positions, int32_t capacity, int32_t* cu, int32_t* kv_lens, int32_t* state_out, int32_t* failed, tqb_stream_t stream) {
     int st = check_plan_shape(num_requests, table_stride, max_blocks, page_size);
     if (st != TQB_OK) return st;
     if (capacity < 0 || free_capacity < 0) return TQB_ERR_INVALID_ARGUMENT;
@@ -1201,7 +1206,7 @@ int plan(const int32_t* seq_lens, const int32_t* new_tokens, int32_t num_request
     if (num_requests > 0 && (!seq_lens || !new_tokens || !kv_lens || (max_blocks > 0 && (!block_table || !free_pages)))) return TQB_ERR_NULL_POINTER;
     if (capacity > 0 && (!slots || !positions)) return TQB_ERR_NULL_POINTER;
     PlanArgs a{seq_lens, new_tokens, block_table, table_stride, free_pages, state, slots, positions, cu, kv_lens, state_out,
-               num_requests, max_blocks, log2_of(page_size), capacity, free_capacity};
+               failed, num_requests, max_blocks, log2_of(page_size), capacity, free_capacity};
     int grid = (capacity + kPlanTokens - 1) / kPlanTokens;
     grid = grid < 1 ? 1 : grid > 148 ? 148 : grid;
     plan_kernel<<<grid, kPlanThreads, 0, as_stream(stream)>>>(a);
@@ -1237,16 +1242,16 @@ int tqb_paged_plan(const int32_t* seq_lens, const int32_t* new_tokens, int32_t n
                    tqb_stream_t stream) {
     TQB_NVTX_RANGE();
     return plan(seq_lens, new_tokens, num_requests, block_table, table_stride, max_blocks, free_pages, 0x7fffffff, state, page_size, slots,
-                positions, capacity, cu, kv_lens, state_out, stream);
+                positions, capacity, cu, kv_lens, state_out, nullptr, stream);
 }
 
 int tqb_paged_plan_bounded(const int32_t* seq_lens, const int32_t* new_tokens, int32_t num_requests, int32_t* block_table,
                            int64_t table_stride, int32_t max_blocks, const int32_t* free_pages, int32_t free_capacity,
                            int32_t* state, int32_t page_size, int64_t* slots, int32_t* positions, int32_t capacity, int32_t* cu,
-                           int32_t* kv_lens, int32_t* state_out, tqb_stream_t stream) {
+                           int32_t* kv_lens, int32_t* state_out, int32_t* failed, tqb_stream_t stream) {
     TQB_NVTX_RANGE();
     return plan(seq_lens, new_tokens, num_requests, block_table, table_stride, max_blocks, free_pages, free_capacity, state, page_size,
-                slots, positions, capacity, cu, kv_lens, state_out, stream);
+                slots, positions, capacity, cu, kv_lens, state_out, failed, stream);
 }
 
 int tqb_paged_release(const uint8_t* mask, int32_t* seq_lens, int32_t num_requests, int32_t* block_table, int64_t table_stride,

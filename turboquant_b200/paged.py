@@ -125,11 +125,14 @@ class PagedStep:
 
     def check(self):
         """Raises if the step could not be planned; waits for the device."""
-        status = int(self.state[2])
-        if status:
-            err = TqbRuntimeError(_PLAN_STATUS.get(status, f"plan status {status}"))
-            err.status = status
-            raise err
+        _check_plan(int(self.state[2]))
+
+
+def _check_plan(status):
+    if status:
+        err = TqbRuntimeError(_PLAN_STATUS.get(status, f"plan status {status}"))
+        err.status = status
+        raise err
 
 
 def _plan_args(seq_lens, block_table, free_pages, state):
@@ -142,13 +145,14 @@ def _plan_args(seq_lens, block_table, free_pages, state):
             _want("free_pages", free_pages, i32, free_pages.shape, index), _want("state", state, i32, (4,), index))
 
 
-def paged_plan(seq_lens, new_tokens, block_table, free_pages, state, page_size, capacity, kv_lens=None, state_out=None):
+def paged_plan(seq_lens, new_tokens, block_table, free_pages, state, page_size, capacity, kv_lens=None, state_out=None, failed=None):
     """Block tables, slot map and positions of a step from the requests' lengths (tqb_paged_plan_bounded).
 
     seq_lens, new_tokens [requests], block_table [requests, blocks] (new entries are written in place), free_pages and
     state int32; the first state[0] entries of free_pages are the free pages.  kv_lens and state_out are made new unless
     given; they may be seq_lens and state themselves.  Returns a PagedStep; `check()` on it says whether the step fitted (with
-    state[0] beyond the list's length no page is to be had)."""
+    state[0] beyond the list's length no page is to be had).  failed [1] int32, if given, gets the status of every plan and
+    release that did not fit, and keeps it when later ones do."""
     index, n, blocks, seq, table, free, st = _plan_args(seq_lens, block_table, free_pages, state)
     new = _want("new_tokens", new_tokens, torch.int32, (n,), index)
     if capacity < 0:
@@ -172,7 +176,8 @@ def paged_plan(seq_lens, new_tokens, block_table, free_pages, state, page_size, 
     if kv_lens is None:
         kv_lens = parts.pop()
     _call(index, lib.tqb_paged_plan_bounded, seq, new, n, table, blocks, blocks, free, free_pages.shape[0], st, page_size, slots.data_ptr(),
-          positions.data_ptr(), capacity, cu.data_ptr(), kv_lens.data_ptr(), state_out.data_ptr())
+          positions.data_ptr(), capacity, cu.data_ptr(), kv_lens.data_ptr(), state_out.data_ptr(),
+          None if failed is None else _want("failed", failed, torch.int32, (1,), index))
     return PagedStep(slots, positions, cu, kv_lens, state_out)
 
 
@@ -374,13 +379,23 @@ class PagedPqoCache:
         self.seq_lens = torch.zeros(max_requests, dtype=torch.int32, device=dev)
         self.free_pages = torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=dev)
         self.state = torch.tensor([num_pages, 0, 0, 0], dtype=torch.int32, device=dev)
+        self.failed = torch.zeros(1, dtype=torch.int32, device=dev)   # status of the last plan or release that did not fit
         self._scratch = {}
 
     def plan(self, new_tokens, capacity):
         """Pages, slots and positions for new_tokens [max_requests] int32 of each request; `step.check()` tells whether
         they fitted.  The step's kv_lens and state are the cache's own and go on with its next plan."""
         return paged_plan(self.seq_lens, new_tokens, self.block_table, self.free_pages, self.state, self.page_size, capacity,
-                          kv_lens=self.seq_lens, state_out=self.state)
+                          kv_lens=self.seq_lens, state_out=self.state, failed=self.failed)
+
+    def check(self):
+        """Raises if any plan or release since the last check did not fit, those of replayed graphs included; waits for the
+        device.  A step that did not fit has stored nothing."""
+        status = int(torch.where(self.failed[0] != 0, self.failed[0], self.state[2]))
+        if status:
+            self.failed.zero_()
+            self.state[2] = 0
+        _check_plan(status)
 
     def release(self, mask):
         """Ends the requests with mask[r] (bool or u8 [max_requests]); their rows may be used by new ones.  Pages that others
