@@ -3,7 +3,7 @@ import ctypes
 
 import pytest
 
-from test_paged_cpu import A, layer
+from test_paged_cpu import A, layer, rope_params
 from turboquant_b200._lib import TqbPagedAttentionParams, lib
 
 
@@ -25,3 +25,9 @@ def test_plan_of_a_list_of_known_length(at, value, status):
     args = [A, A, 3, A, 4, 4, A, 9, A, 16, A, A, 5, A, A, A, None, None]
     args[at] = value
     assert lib.tqb_paged_plan_bounded(*args) == status
+
+
+def test_rotations_whose_units_and_stride_pass_31_bits_are_refused():
+    """Two units a token: 2,147,476,000 of them, and the grid's stride on top."""
+    p = rope_params(num_tokens=1073738000, num_q_heads=1, num_kv_heads=1)
+    assert lib.tqb_qk_norm_rope(ctypes.byref(p), None) == 12

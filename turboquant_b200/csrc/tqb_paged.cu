@@ -827,6 +827,7 @@ struct Rows {
 
 constexpr int kTurnWarps = 4, kTurnCtas = 5;   // of turn_kernel: CTAs of an SM
 constexpr int kTurnPasses = 13;                // passes that a warp has at least, where there are more CTAs than places
+constexpr int kTurnTimes = 32;                 // CTAs for each place, at most: the stride of a warp's units stays small
 constexpr int kRingBytes = 4096;   // of a warp: Rows::kDepth * Rows::kSlot
 
 // Cosines and sines of a token's angles, by `all` threads of which this is number `me`.
@@ -1086,17 +1087,17 @@ int launch_rows_one(RowArgs& a, const Codebook& cb, cudaStream_t s) {
             u.size = (long long)a.tokens * passes <= warps ? 1 : (passes + 1) / 2;
             u.per_token = (passes + u.size - 1) / u.size;
             const long long units = (long long)a.tokens * u.per_token;
-            if (units >= (1ll << 31) - 2 * warps) return TQB_ERR_TOO_LARGE;
-            u.count = (int)units;
             u.by_token = Divisor((unsigned)u.per_token);
             // A CTA for each place on the SMs, or several, as long as a warp keeps kTurnPasses passes: SMs get through their shares at
             // different speeds, and who is done early takes another CTA.  (8,191 tokens of 40 heads, head_dim 256: 76.8 us, with one
             // for each place 85.0; 16,384 of 128: 77.6 and 83.9.  But 4,096 of 128, 14 passes a warp: 22.9 us with two, 21.6 with one;
             // 6,007 with one and a half 35.6, with one 33.0.)
-            const long long want = (u.count + kTurnWarps - 1) / kTurnWarps, times = (long long)a.tokens * passes / (warps * kTurnPasses);
-            const long long most = 148 * kTurnCtas * (times > 1 ? times : 1);
+            const long long want = (units + kTurnWarps - 1) / kTurnWarps, times = (long long)a.tokens * passes / (warps * kTurnPasses);
+            const long long most = 148 * kTurnCtas * (times > kTurnTimes ? kTurnTimes : times > 1 ? times : 1);
             const int grid = (int)(want < most ? want : most);
             u.step = grid * kTurnWarps;
+            if (units + u.step >= 1ll << 31) return TQB_ERR_TOO_LARGE;   // (a unit behind the last one is the largest that is formed)
+            u.count = (int)units;
             turn_kernel<T, LPH><<<grid, 32 * kTurnWarps, dyn, s>>>(a, u);
             return check_launch(s);
         }
