@@ -31,3 +31,11 @@ def test_rotations_whose_units_and_stride_pass_31_bits_are_refused():
     """Two units a token: 2,147,476,000 of them, and the grid's stride on top."""
     p = rope_params(num_tokens=1073738000, num_q_heads=1, num_kv_heads=1)
     assert lib.tqb_qk_norm_rope(ctypes.byref(p), None) == 12
+
+
+@pytest.mark.parametrize("hkv,hq", [(1 << 21, 1 << 21), (2, 1 << 25)])
+def test_heads_beyond_the_quotients_of_the_work_line_are_refused(hkv, hq):
+    """2^21 KV heads, or as many groups of eight query heads, of one request: few units, but too many heads."""
+    few = layer(num_kv_heads=hkv, num_pages=1, page_size=16)
+    p = attention(num_q_heads=hq, num_requests=1, max_blocks=1, table_stride=1)
+    assert lib.tqb_paged_attention(ctypes.byref(few), ctypes.byref(p), None) == 12

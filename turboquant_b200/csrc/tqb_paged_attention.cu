@@ -285,7 +285,8 @@ int attention(const tqb_paged_layer* layer, const tqb_paged_attention_params* p,
     a.group = p->num_q_heads / layer->num_kv_heads;
     a.splits = (a.group + kSegHeads - 1) / kSegHeads;
     a.vheads = a.hkv * a.splits;
-    // (below 2^30 units the quotients of divide() stay below 2^21)
+    // (below 2^30 units and 2^21 heads the quotients of divide() stay below 2^21)
+    if (a.vheads >= 1 << 21) return TQB_ERR_TOO_LARGE;
     auto units = [&](int shift) { return (double)a.requests * (kOpenCost + 1 + (double)((a.max_len / kRunTokens) >> shift)) * a.vheads; };
     while (units(a.unit_shift) >= 1073741824.0 && a.unit_shift < 24) ++a.unit_shift;
     if (units(a.unit_shift) >= 1073741824.0) return TQB_ERR_TOO_LARGE;
