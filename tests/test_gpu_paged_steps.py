@@ -1,5 +1,5 @@
 """Steps of a paged batch in which requests are idle, bring one token or a piece of a prompt: queries and outputs lie in the
-order of the step's tokens."""
+order of the step's tokens.  Plans and attention where they are at their limits."""
 import numpy as np
 import pytest
 import torch
@@ -187,3 +187,21 @@ def test_a_step_that_did_not_fit_is_told_after_later_ones():
     cache.check()
     with pytest.raises(tq.DimensionMismatch):
         tq.paged_plan(cache.seq_lens, new, cache.block_table, cache.free_pages, cache.state, 16, 4, failed=new)
+
+
+@pytest.mark.parametrize("dim,group", [(64, 4), (128, 4), (128, 8), (256, 2)])
+@pytest.mark.parametrize("bits", [3, 4])
+@pytest.mark.parametrize("vscale", [1.0, 1e-4, 1e-6, 3e-7])
+def test_values_of_small_scales_keep_their_precision(vscale, bits, dim, group):
+    """The error's norm, over that of a head's output.  A weight is rounded to f16 twice, each time by up to 2^-11 of itself:
+    2.9e-4 rms and less.  Below 2^-14 a product is off by up to 2^-25 (2^-25 / sqrt(3) rms); the largest weight is held as 2^11 at least, so that
+    700 of them make 2^-25 / sqrt(3) * sqrt(700) / (2^11 * 3e-7) = 7.4e-4 of the output at the smallest scale here."""
+    g, page, hkv, lens = gen(9), 32, 2, [65, 700]
+    layer = filled(30, hkv, page, dim, bits, g, 0.0)
+    layer.tensors[3].copy_((layer.tensors[3].view(torch.float16).float() * vscale).half().view(torch.int16))
+    table, ln = table_of(lens, page, 30, g), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q = torch.randn((2, hkv * group, dim), generator=g, device="cuda").to(torch.bfloat16)
+    out = layer.attend(q, table, ln, dim ** -0.5, out=torch.empty((2, hkv * group, dim), device="cuda"))
+    want, _, _ = ref.attend(q, layer.tensors, bits, table, ln, dim ** -0.5)
+    off = (out.double() - want).norm(dim=-1) / want.norm(dim=-1)
+    assert float(off.mean()) <= 2.0 ** -10, float(off.mean())

@@ -12,7 +12,8 @@
 //   block's scale multiplies the integer sum.
 // Softmax: lane 4n + j has tokens n and n + 8 of head j (heads 2j, 2j + 1).  The reference m is common to the warp and only
 //   raised when some score exceeds it by kShift + kLazy, which a vote finds out: no shuffles otherwise.  p = 2^(s - m), up to
-//   2^(kShift + kLazy), so that f16 holds products with small weights and small scales in its normal range.
+//   2^(kShift + kLazy), as high as f16 allows, so that it holds products with small weights and small scales: rms errors of
+//   700 tokens stay below 3e-4 down to scales of 3e-7 (with kShift 6: 1.2e-3 at 1e-6, 4.4e-3 at 3e-7).
 // O^T = V^T P' (mma.sync f16, K = 16 tokens): P' = p |s_v|, rounded to f16 (once for p, once for the product: 2^-11 each,
 //   below the rounding of a bf16 output and within that of f16).  Up to four heads, the two columns of a head carry the
 //   scales of two neighbouring blocks, one half2 product for both, and one movmatrix turns them into B fragments.
@@ -20,7 +21,8 @@
 //   is taken off by starting each accumulation at -7.5 sum P', itself an MMA with constant rows.  Accumulators live for
 //   32 tokens and are then added to the running output in rounded f32 additions; one long chain would add up the truncation
 //   of the MMA's adder relative to 7.5 sum P'.
-//   Where some |s_v| is above 32, so that a product could leave f16, the warp lowers kShift by as much.
+//   Where some |s_v| is above 1, so that a product could leave f16, the warp lowers kShift by as much (most often with the
+//   first step's maximum, where that costs nothing).
 //
 // Measured (8 KV heads, head_dim 128, 4 bits, bf16): 64 requests of 8,192 tokens, four query heads a KV head 101.5 us (6.0 TB/s, 0.91
 // of a copy); 64 of 531 to 8,192 tokens 43.9 us (of which 6 us until the first products and 5 for the joins); one of 131,072
@@ -41,8 +43,8 @@ constexpr int kGroupTokens = 16;
 constexpr int kRing = 4;     // stages of a warp
 constexpr int kStepGroups = 2;
 constexpr int kInFlight = kRing - kStepGroups;
-constexpr float kShift = 6.0f, kLazy = 4.0f;
-constexpr uint32_t kScaleTop = 0x50005000u;   // 2^(15 - kShift - kLazy) = 32, twice
+constexpr float kShift = 11.0f, kLazy = 4.0f;
+constexpr uint32_t kScaleTop = 0x3c003c00u;   // 2^(15 - kShift - kLazy) = 1, twice
 constexpr uint32_t kSignBits = 0xB1A6D4B2u;   // bit d: dim d of a block changes its sign (src/cache/precomputed/rotation.rs:16-20)
 constexpr float kQMax = 32639.0f;   // 127 * 256 + 127
 
