@@ -2,8 +2,11 @@
 import ctypes
 
 import pytest
+import torch
 
+import turboquant_b200 as tq
 from test_paged_cpu import A, layer, rope_params
+from turboquant_b200 import paged
 from turboquant_b200._lib import TqbPagedAttentionParams, lib
 
 
@@ -39,3 +42,41 @@ def test_heads_beyond_the_quotients_of_the_work_line_are_refused(hkv, hq):
     few = layer(num_kv_heads=hkv, num_pages=1, page_size=16)
     p = attention(num_q_heads=hq, num_requests=1, max_blocks=1, table_stride=1)
     assert lib.tqb_paged_attention(ctypes.byref(few), ctypes.byref(p), None) == 12
+
+
+def test_capture_is_asked_of_the_cache_s_own_device(monkeypatch):
+    """A cache on another device than the current one: whether its stream is being captured, and which one that is, are asked
+    with its device current."""
+    now, used = [0], []
+
+    class On:
+        def __init__(self, device):
+            self.index = torch.device(device).index if not isinstance(device, int) else device
+
+        def __enter__(self):
+            self.before, now[0] = now[0], self.index
+
+        def __exit__(self, *a):
+            now[0] = self.before
+
+    class Layer:
+        def __init__(self, index):
+            self.index = index
+
+        def attend_scratch(self, heads):
+            return "kept"
+
+        def attend(self, q, table, lens, scale, out=None, scratch=None, cu=None):
+            used.append(scratch)
+            return q
+
+    monkeypatch.setattr(torch.cuda, "device", On)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now[0] == 1)   # device 1 captures, device 0 does not
+    monkeypatch.setattr(paged, "_current_device", lambda: now[0])
+    monkeypatch.setattr(paged, "_raw_stream", lambda index: 5)
+    step = tq.PagedStep(None, None, None, None, None)
+    for index, scratch in ((1, None), (0, "kept")):
+        cache = object.__new__(tq.PagedPqoCache)
+        cache.device, cache.layers, cache.block_table, cache._scratch = torch.device("cuda", index), [Layer(index)], None, {}
+        cache.decode(0, torch.zeros(2, 4, 64), step, tq.AttendConfig(0.1))
+        assert used.pop() == scratch

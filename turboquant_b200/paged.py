@@ -45,6 +45,14 @@ def _call(index, fn, *args):
         check(status)
 
 
+def _eager_stream(index):
+    """The handle of the device's current stream, or None while it is being captured."""
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return _eager_stream(index)
+    return None if torch.cuda.is_current_stream_capturing() else _raw_stream(index)
+
+
 def _device(name, t):
     index = t.get_device()
     if index < 0:
@@ -426,11 +434,12 @@ class PagedPqoCache:
 
     def _decode(self, layer, q, step, config, out, scratch, cu):
         at = self._layer(layer)
-        if scratch is None and not torch.cuda.is_current_stream_capturing():
-            stream = torch.cuda.current_stream(self.device).cuda_stream
-            scratch = self._scratch.get(stream)
-            if scratch is None:
-                scratch = self._scratch[stream] = at.attend_scratch(q.shape[1])
+        if scratch is None:
+            stream = _eager_stream(at.index)
+            if stream is not None:
+                scratch = self._scratch.get(stream)
+                if scratch is None:
+                    scratch = self._scratch[stream] = at.attend_scratch(q.shape[1])
         return DecodeOutput(fused=at.attend(q, self.block_table, step.kv_lens, config.softmax_scale, out=out, scratch=scratch, cu=cu))
 
     def _layer(self, layer):
