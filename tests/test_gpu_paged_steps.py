@@ -205,3 +205,24 @@ def test_values_of_small_scales_keep_their_precision(vscale, bits, dim, group):
     want, _, _ = ref.attend(q, layer.tensors, bits, table, ln, dim ** -0.5)
     off = (out.double() - want).norm(dim=-1) / want.norm(dim=-1)
     assert float(off.mean()) <= 2.0 ** -10, float(off.mean())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("tokens,hq,hkv", [(3, 8, 2), (1, 4, 4), (70, 1, 1), (129, 5, 2)])
+def test_rows_that_lie_head_after_head(tokens, hq, hkv, dtype):
+    """Outputs [heads, tokens, dim], new ones and the inputs themselves; rows that overlap are refused."""
+    g, dt, dim = gen(6), DT[dtype], 128
+    rope, pos = rope_of(dim), torch.arange(tokens, device="cuda")
+    q, k = (torch.randn((h, tokens, dim), generator=g, device="cuda").to(dt).transpose(0, 1) for h in (hq, hkv))
+    want = rope(q.contiguous(), k.contiguous(), pos)
+    outs = [torch.zeros((h, tokens, dim), device="cuda", dtype=dt).transpose(0, 1) for h in (hq, hkv)]
+    got = rope(q, k, pos, q_out=outs[0], k_out=outs[1])
+    assert got[0] is outs[0] and torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+    rope(q, k, pos, q_out=q, k_out=k)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+    flat = torch.zeros(1 << 18, device="cuda", dtype=dt)
+    if tokens > 1 and hq > 1:
+        for strides in ((dim, dim, 1), (0, dim, 1), (dim, 0, 1), (2 * dim, dim, 1), (dim // 2, tokens * dim, 1)):
+            if strides[0] < (hq - 1) * strides[1] + dim and strides[1] < (tokens - 1) * strides[0] + dim or min(strides[:2]) < dim:
+                with pytest.raises(ValueError):
+                    rope(q, k, pos, q_out=flat.as_strided((tokens, hq, dim), strides))

@@ -94,7 +94,8 @@ def _out_rows(name, t, like, index):
     if t.get_device() != index:
         raise ValueError(f"{name}: expected a tensor on cuda:{index}, got {t.device}")
     at, (s0, s1, s2), e, (n, h, d) = t.data_ptr(), t.stride(), 16 // t.element_size(), t.shape
-    if s2 != 1 or s0 % e or s1 % e or at % 16 or (h > 1 and s1 < d) or (n > 1 and s0 < (h - 1) * s1 + d):
+    by_token, by_head = n < 2 or s0 >= (h - 1) * s1 + d, h < 2 or s1 >= (n - 1) * s0 + d   # the rows of a token, of a head lie together
+    if s2 != 1 or s0 % e or s1 % e or at % 16 or (h > 1 and s1 < d) or (n > 1 and s0 < d) or not (by_token or by_head):
         raise ValueError(f"{name}: rows must be dense, 16-byte aligned and apart from one another")
     return at, s0, s1
 
