@@ -38,3 +38,17 @@ def test_no_part_of_a_request_is_lost(lens, hkv, group, bits, dtype):
     for _ in range(2):
         assert torch.equal(out, layer.attend(q, table, ln, DIM ** -0.5, out=torch.empty_like(out), scratch=scratch))
     assert bool((scratch[:16384] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("bits", [3, 4])
+@pytest.mark.parametrize("power", [10, 20, 23, 24, 25, 26, 30, 60, 90, 112])
+def test_scores_far_from_zero_still_have_a_softmax(power, bits, dtype):
+    """One token has weight 1 whatever its score is, from -1e36 to 1e36: the value itself, but for the rounding of weight and product."""
+    g, dt, n = gen(power), DT[dtype], 24
+    layer = filled(n, 2, PAGE, DIM, bits, g, 0.0)
+    table, ln = torch.arange(n, dtype=torch.int32, device="cuda")[:, None].contiguous(), torch.ones(n, dtype=torch.int32, device="cuda")
+    q = (torch.randn((n, 8, DIM), generator=g, device="cuda") * 2.0 ** power).to(dt)
+    out = layer.attend(q, table, ln, DIM ** -0.5, out=torch.empty((n, 8, DIM), device="cuda"))
+    want = ref.rows(layer.tensors[2][:, :, 0], layer.tensors[3][:, :, 0], bits).repeat_interleave(4, 1)
+    assert float(((out.double() - want).norm(dim=-1) / want.norm(dim=-1)).max()) <= 2.0 ** -10

@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG, BITS>::kCtas) paged
                         sv_limit += above * 0x04000400u;
                     }
 #pragma unroll
-                    for (int e = 0; e < kE; ++e) {
+                    for (int e = 0; e < kE; ++e) {   // (products rounded as in their maximum, which rounded up keeps x at shift or below: scores may be 2^27 and more)
                         float mx = -INFINITY;
 #pragma unroll
                         for (int u = 0; u < kStepGroups; ++u)
@@ -517,13 +517,13 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG, BITS>::kCtas) paged
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                        const float m_new = fmaxf(m_ref[e] + less, mx - shift), keep = ex2(m_ref[e] - m_new);
+                        const float m_new = fmaxf(m_ref[e] + less, __fadd_ru(mx, -shift)), keep = ex2(m_ref[e] - m_new);
                         m_ref[e] = m_new;
                         l_run[e] *= keep;
 #pragma unroll
                         for (int u = 0; u < kStepGroups; ++u)
 #pragma unroll
-                            for (int t = 0; t < 2; ++t) x[u][t][e] = out[u][t] ? -INFINITY : fmaf(raw[u][t][e], qsc[e], -m_new);
+                            for (int t = 0; t < 2; ++t) x[u][t][e] = out[u][t] ? -INFINITY : raw[u][t][e] * qsc[e] - m_new;
 #pragma unroll
                         for (int b = 0; b < NB; ++b)
 #pragma unroll

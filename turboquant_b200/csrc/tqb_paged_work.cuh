@@ -14,6 +14,8 @@
 // Measured at 128 requests of 62 to 1,000 tokens (8 KV heads, 4-bit): with CTAs instead of warps taking the runs, every
 // short segment paid its loads' latency and eight block barriers: 64 us.
 #pragma once
+#include <float.h>
+
 #include "tqb_common.cuh"
 #include "tqb_paged.cuh"
 
@@ -31,7 +33,7 @@ constexpr int kWorkThreads = 32 * kWorkWarps;
 constexpr int kMaxCtas = 148 * 8;    // of a launch: sizes tickets and partials
 constexpr int kMaxRound = 36;        // parts joined at a time, at most
 static_assert(kMaxCtas * 3 * 4 <= TQB_PAGED_TICKET_BYTES, "tickets of the last round, and of the slots for the one before it");
-constexpr float kNoScore = -1.0e30f; // finite stand-in for -inf: differences of two of them are 0
+constexpr float kNoScore = -FLT_MAX; // finite stand-in for -inf: differences of two of them are 0
 
 struct PagedArgs {
     const void* q;
