@@ -69,9 +69,11 @@ __device__ __forceinline__ __half2 u32_as_h2(uint32_t u) { return *reinterpret_c
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(dst), "l"(src) : "memory");
+template <int BYTES>
+__device__ __forceinline__ void cp_async_ca(uint32_t dst, const void* src) {   // 4, 8 or 16 bytes, kept in L1 too
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;\n" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src) { cp_async_ca<8>(dst, src); }
 // The same with immediate offsets folded into the address operands (no address arithmetic in registers).
 template <int DOFF, int SOFF>
 __device__ __forceinline__ void cp_async16_o(uint32_t dst, const void* src) {

@@ -14,7 +14,7 @@ namespace {
 // need.  Every CTA does the two prefix sums over the requests for itself (8 bytes a request from L2) and then takes its
 // share of the tokens and of the new table entries; nobody waits for anybody.  What may be updated in place - lengths and
 // state - is written by the CTA that finishes last, when all have read it.  Bound: launch and dependent loads: 64 requests of a
-// token each 3.8 us, 211 requests that bring up to 511 tokens each 5.2 us.
+// token each 3.6 us, 211 requests, a third of which bring up to 511 tokens, 4.5 us.
 constexpr int kMostCounted = 1 << 30;   // tokens of a plan or of rows that turn: an index and a grid's stride stay below 2^31
 constexpr int kPlanThreads = 256;
 constexpr int kPlanTokens = 256;    // tokens a CTA, up to 148 CTAs (1,024: 7.2 us for the 211 requests)
@@ -339,8 +339,10 @@ __global__ void __launch_bounds__(kReleaseThreads) release_kernel(ReleaseArgs a)
 // Blocks: one thread packs one 32-block of the tile, or of the values where they lie, as tqb_block_quantize does
 //   (pqo_quantize_values), 16 or 12 bytes of codes.  Four lanes a block with the butterfly's last stages as shuffles needs three
 //   times the instructions.
-// Bound: HBM, at the pace of the slower SMs (without norm and rotation, rows copied by the same kernel take as long): 8,191 tokens
-// of 32 + 8 heads, head_dim 128, normed and rotated 42 us (4.0 TB/s; a plain copy of these bytes takes 32 to 36), one token 2.8 us; 6,007 tokens of 16 + 8 heads rotated and packed to 3 bits 28.5 us.
+// Bound: how the rows are moved, a lane's 16-byte copies and stores and the arithmetic of their addresses: without norm and
+// rotation the same kernel takes as long, with DRAM at 36 % and issue at 61 %.  8,191 tokens of 32 + 8 heads, head_dim 128, normed and
+// rotated 42 us (4.0 TB/s; a plain copy of these bytes takes 32 to 36), one token 2.5 us; 6,007 tokens of 16 + 8 heads rotated and
+// packed to 3 bits 28.5 us.
 constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32, kRowWarpsLog = 3;
 static_assert(kRowWarps == 1 << kRowWarpsLog, "");
@@ -654,9 +656,6 @@ __device__ __forceinline__ void do_rows_part(const RowArgs& a, const RowSpan& s,
     }
 }
 
-// The same where whole rows turn, or nothing does: a lane has eight elements of the first half of a row and the eight half a
-// row behind them, so that both elements of a pair are its own, and a pass takes 32 / (D / 16) heads.  Half the
-// instructions a row of do_rows_part, which is what bounds this kernel: 8,191 tokens of 32 + 8 heads 45 us with it.
 // What a warp takes in turn: `size` passes of a token, unit after unit `step` apart.
 struct Units {
     int count, step, size, per_token;
@@ -665,6 +664,9 @@ struct Units {
     __device__ __forceinline__ int first_pass(int unit, int token) const { return (unit - token * per_token) * size; }
 };
 
+// The same as do_rows_part where whole rows turn, or nothing does: a lane has eight elements of the first half of a row and the
+// eight half a row behind them, so that both elements of a pair are its own.  Half the instructions a row (8,191 tokens of 32 + 8
+// heads took 45 us with do_rows_part).
 // A pass is 32 / (D / 16) heads of queries, or of keys, of a token; passes are numbered token after token, queries before keys.
 // They are copied to a ring in shared memory, kDepth of them ahead; a lane reads what it has copied itself.
 template <typename T, int LPH, bool STORE>

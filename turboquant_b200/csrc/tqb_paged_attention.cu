@@ -37,10 +37,10 @@ struct F32Plan {
 };
 
 template <int BYTES>
-__device__ __forceinline__ void cp_async_bytes(void* dst, const void* src) {
+__device__ __forceinline__ void copy_piece(void* dst, const void* src) {
     const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst);
-    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to), "l"(src) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;\n" ::"r"(to), "l"(src), "n"(BYTES) : "memory");
+    if constexpr (BYTES == 16) cp_async16(to, src);
+    else cp_async_ca<BYTES>(to, src);
 }
 
 // A token's NB scales as f32 magnitudes.
@@ -107,14 +107,14 @@ __global__ void __launch_bounds__(kWorkThreads, F32Plan<NB, H, BITS>::kCtas) pag
             if (live) {
 #pragma unroll
                 for (int i = 0; i < L::kRow; i += kPiece) {
-                    cp_async_bytes<kPiece>(s_k + lane * L::kRow + i, a.kb + row * L::kRow + i);
-                    cp_async_bytes<kPiece>(s_v + lane * L::kRow + i, a.vb + row * L::kRow + i);
+                    copy_piece<kPiece>(s_k + lane * L::kRow + i, a.kb + row * L::kRow + i);
+                    copy_piece<kPiece>(s_v + lane * L::kRow + i, a.vb + row * L::kRow + i);
                 }
             }
-            asm volatile("cp.async.commit_group;\n" ::: "memory");
+            cp_async_commit();
             scales_of<NB>(a.ks + row * NB, live, s_ks + lane * NB);
             scales_of<NB>(a.vs + row * NB, live, s_vs + lane * NB);
-            asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+            cp_async_wait<0>();
             __syncwarp();
             // ---- scores ----
             float x[H];
@@ -153,8 +153,8 @@ __global__ void __launch_bounds__(kWorkThreads, F32Plan<NB, H, BITS>::kCtas) pag
                 float top = x[h];
 #pragma unroll
                 for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
-                const float to = fmaxf(m[h], top), keep = exp2_fast(m[h] - to);
-                x[h] = exp2_fast(x[h] - to);
+                const float to = fmaxf(m[h], top), keep = ex2(m[h] - to);
+                x[h] = ex2(x[h] - to);
                 m[h] = to;
                 l[h] = fmaf(l[h], keep, x[h]);
 #pragma unroll

@@ -48,11 +48,6 @@ constexpr uint32_t kScaleTop = 0x3c003c00u;   // 2^(15 - kShift - kLazy) = 1, tw
 constexpr uint32_t kSignBits = 0xB1A6D4B2u;   // bit d: dim d of a block changes its sign (src/cache/precomputed/rotation.rs:16-20)
 constexpr float kQMax = 32639.0f;   // 127 * 256 + 127
 
-template <int BYTES>
-__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;\n" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
-}
-
 // A token's NB scales, two a word.
 template <int NB, int OFF>
 __device__ __forceinline__ void load_scales(uint32_t at, uint32_t (&w)[NB / 2]) {
@@ -117,7 +112,8 @@ struct Plan {
     static constexpr int kQueries = HG * NB * 32 * 2;             // the next segment's queries as they are
     static constexpr int kWarpBytes = G::kWarpRing + kFragment + kDigits + kQueries;   // [ring][fragment that began before][digits][queries]
     static constexpr int kBytes = kWorkWarps * kWarpBytes;
-    // CTAs of an SM: by shared memory, and three, so that registers hardly spill and fewer parts are joined (two for head_dim 256).
+    // CTAs of an SM: by shared memory, and three, so that registers hardly spill and fewer parts are joined (head_dim 256: two, and
+    // with more than four heads only one has room).
     // 64 requests of 531 to 8,192 tokens, four heads: 43.9 us; with two 46.7, with four 45.2; head_dim 64 32.8, with five 33.8.
     static constexpr int kByShared = 228 * 1024 / (kBytes + 1024 + 2560 + (BITS == 3 ? 8192 : 0)), kByRegs = NB == 8 ? 2 : 3;
     static constexpr int kCtas = kByShared < kByRegs ? kByShared : kByRegs;
@@ -229,7 +225,7 @@ __global__ void __launch_bounds__(kWorkThreads, Plan<NB, HG, BITS>::kCtas) paged
                     cp_async16(d + G::kIdx, vp + p * 512);
                 }
             }
-            cp_async_small<G::kSc>(st + off_ps, sp);
+            cp_async_ca<G::kSc>(st + off_ps, sp);
             kp += G::kIdx;
             vp += G::kIdx;
             sp += kGroupTokens * NB;

@@ -17,6 +17,7 @@
 #include <float.h>
 
 #include "tqb_common.cuh"
+#include "tqb_mma.cuh"
 #include "tqb_paged.cuh"
 
 namespace tqb {
@@ -188,12 +189,6 @@ struct WorkLine {
     }
 };
 
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
-    return y;
-}
-
 __device__ __forceinline__ float wht32_across(float v, int lane) {
 #pragma unroll
     for (int h = 1; h < 32; h <<= 1) {
@@ -274,7 +269,7 @@ struct Running {
     float M = kNoScore, L = 0.0f;
     float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     __device__ __forceinline__ void raise(float m) {
-        const float to = fmaxf(M, m), keep = exp2_fast(M - to);
+        const float to = fmaxf(M, m), keep = ex2(M - to);
         M = to;
         L *= keep;
         O.x *= keep;
@@ -283,7 +278,7 @@ struct Running {
         O.w *= keep;
     }
     __device__ __forceinline__ void add(float m, float l, float4 o) {   // m is not above M
-        const float e = exp2_fast(m - M);
+        const float e = ex2(m - M);
         L = fmaf(l, e, L);
         O.x = fmaf(o.x, e, O.x);
         O.y = fmaf(o.y, e, O.y);
