@@ -657,6 +657,7 @@ int tqb_paged_dequantize(const tqb_paged_layer *layer, const int64_t *slots, int
  *   block_table [num_requests, max_blocks], rows table_stride entries apart;  kv_lens [num_requests]
  * Request r attends to its first kv_lens[r] tokens (the new one stored already).  A request without tokens gets
  * zeros.  Lengths beyond max_blocks * page_size are cut there, and the tokens of a page outside [0, num_pages) are left out.
+ * The cache is read once for every eight query heads of a KV head; 2^21 KV heads times such groups are TQB_ERR_TOO_LARGE.
  * The work is split over the lengths on the device, so that a captured call serves any lengths later.  out may be q where
  * their types are the same and q is dense.
  * scratch: tqb_paged_scratch_bytes() bytes whose first TQB_PAGED_TICKET_BYTES the caller has zero-filled once; every

@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(kReleaseThreads) release_kernel(ReleaseArgs a)
 //   (pqo_quantize_values), 16 or 12 bytes of codes.  Four lanes a block with the butterfly's last stages as shuffles needs three
 //   times the instructions.
 // Bound: how the rows are moved, a lane's 16-byte copies and stores and the arithmetic of their addresses: without norm and
-// rotation the same kernel takes as long, with DRAM at 36 % and issue at 61 %.  8,191 tokens of 32 + 8 heads, head_dim 128, normed and
+// rotation the same kernel takes as long, with DRAM at 35 % and issue at 58 %.  8,191 tokens of 32 + 8 heads, head_dim 128, normed and
 // rotated 42 us (4.0 TB/s; a plain copy of these bytes takes 32 to 36), one token 2.5 us; 6,007 tokens of 16 + 8 heads rotated and
 // packed to 3 bits 28.5 us.
 constexpr int kRowThreads = 256;
